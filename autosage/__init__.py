@@ -10,7 +10,7 @@ import sys
 
 import autosage_b200 as _impl
 
-for _name in ("_auto", "_cache", "_version", "config", "conv", "ops", "utils", "utils.csr"):
+for _name in ("_auto", "_cache", "_version", "config", "conv", "ops", "paged", "utils", "utils.csr"):
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"autosage_b200.{_name}")
 
 from autosage_b200 import *  # noqa: E402,F401,F403
@@ -21,4 +21,5 @@ _cache = sys.modules[f"{__name__}._cache"]
 config = sys.modules[f"{__name__}.config"]
 conv = sys.modules[f"{__name__}.conv"]
 ops = sys.modules[f"{__name__}.ops"]
+paged = sys.modules[f"{__name__}.paged"]
 utils = sys.modules[f"{__name__}.utils"]

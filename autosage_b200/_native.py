@@ -8,6 +8,7 @@ be loaded the callers raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import weakref
 from collections import OrderedDict
@@ -70,7 +71,29 @@ SIGNATURES = {
     "asg_spmm_csr_split_noalloc": (_INT, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _I64, _P]),
     "asg_static_max_rows": (_I64, []),
     "asg_static_status": (_INT, [_P, _P, _P]),
+    "asg_paged_cache_write": (_INT, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
+    "asg_paged_cache_read": (_INT, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
+    "asg_paged_attention_workspace_bytes": (_SZ, [_INT, _INT, _INT]),
+    "asg_paged_attention": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _F32, _I64,
+                                   _INT, _INT, _P, _SZ, _P]),
 }
+
+
+class PagePool(ctypes.Structure):
+    """``asg_page_pool`` of the header."""
+
+    _fields_ = [("data", _P), ("scales", _P), ("page_stride", _I64), ("token_stride", _I64), ("head_stride", _I64),
+                ("scale_page_stride", _I64), ("scale_head_stride", _I64), ("scale_token_stride", _I64)]
+
+
+class TokenRows(ctypes.Structure):
+    """``asg_token_rows`` of the header."""
+
+    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+# ASG_TYPE_* of the header
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
 
 _LIB: Optional[ctypes.CDLL] = None
 _LIB_PATH: Optional[str] = None
@@ -427,6 +450,56 @@ def conv_fused(crow: torch.Tensor, col: torch.Tensor, val: Optional[torch.Tensor
                                    _stream(x.device)))
     _plan_was_built(plan)
     return workspace
+
+
+def _page_pool(pages: torch.Tensor, scales: Optional[torch.Tensor]) -> PagePool:
+    page, token, head, _ = pages.stride()
+    if scales is None:
+        return PagePool(pages.data_ptr(), None, page, token, head, 0, 0, 0)
+    return PagePool(pages.data_ptr(), scales.data_ptr(), page, token, head, *scales.stride())
+
+
+def _token_rows(rows: torch.Tensor) -> TokenRows:
+    return TokenRows(rows.data_ptr(), rows.stride(0), rows.stride(1))
+
+
+def _paged_cache(entry: str, slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
+    k, v = _token_rows(key), _token_rows(value)
+    kp, vp = _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales)
+    check(getattr(library(), entry)(slots.data_ptr(), slots.numel(), ctypes.byref(k), ctypes.byref(v), ctypes.byref(kp),
+                                    ctypes.byref(vp), key_pages.size(0), key_pages.size(1), key_pages.size(2),
+                                    key_pages.size(3), TYPES[key.dtype], TYPES[key_pages.dtype],
+                                    _stream(key_pages.device)))
+
+
+def paged_cache_write(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
+    """Rows [T, heads, dim] into the slots of the pages, quantised where the pages are 8-bit."""
+    _paged_cache("asg_paged_cache_write", slots, key, value, key_pages, value_pages, key_scales, value_scales)
+
+
+def paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
+    """The slots of the pages into the rows key and value."""
+    _paged_cache("asg_paged_cache_read", slots, key, value, key_pages, value_pages, key_scales, value_scales)
+
+
+@functools.lru_cache(maxsize=None)
+def _paged_attention_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(library().asg_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim))
+
+
+def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages, key_scales, value_scales, *,
+                    scale: float, window: int) -> None:
+    """out[r] = softmax(scale q_r K^T) V over the tokens of row r's pages (one query token a row)."""
+    n_rows, n_heads, head_dim = query.shape
+    n_pages, page_size, n_kv_heads, _ = key_pages.shape
+    workspace = scratch(query.device, 0, _paged_attention_bytes(n_heads, n_kv_heads, head_dim))
+    q = _token_rows(query)
+    kp, vp = _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales)
+    check(library().asg_paged_attention(crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(),
+                                        ctypes.byref(q), out.data_ptr(), _ptr(lse), ctypes.byref(kp), ctypes.byref(vp),
+                                        n_pages, page_size, n_heads, n_kv_heads, head_dim, scale, window,
+                                        TYPES[query.dtype], TYPES[key_pages.dtype], workspace.data_ptr(),
+                                        workspace.numel(), _stream(query.device)))
 
 
 def push_to_peers(src: torch.Tensor, destinations: list[torch.Tensor], n_ctas: int = 32) -> None:

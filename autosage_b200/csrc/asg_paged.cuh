@@ -1,0 +1,116 @@
+// What the kernels of the paged cache share: element types, where a token's row lies, argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "asg_common.cuh"
+
+namespace asg {
+namespace paged {
+
+constexpr int kMaxDim = 256;
+
+inline bool is_wide(int type) { return type == ASG_TYPE_F32 || type == ASG_TYPE_BF16 || type == ASG_TYPE_F16; }
+inline bool is_coded(int type) { return type == ASG_TYPE_E4M3 || type == ASG_TYPE_INT8; }
+inline int type_bytes(int type) { return type == ASG_TYPE_F32 ? 4 : is_coded(type) ? 1 : 2; }
+
+// Whether every row of a pool, or of token rows, starts on a multiple of `bytes`.
+inline bool rows_aligned(const asg_page_pool& p, int item, int bytes) {
+  return ((reinterpret_cast<uintptr_t>(p.data) | static_cast<uintptr_t>(p.page_stride * item) |
+           static_cast<uintptr_t>(p.token_stride * item) | static_cast<uintptr_t>(p.head_stride * item)) &
+          (bytes - 1)) == 0;
+}
+inline bool rows_aligned(const asg_token_rows& r, int item, int bytes) {
+  return ((reinterpret_cast<uintptr_t>(r.data) | static_cast<uintptr_t>(r.token_stride * item) |
+           static_cast<uintptr_t>(r.head_stride * item)) & (bytes - 1)) == 0;
+}
+
+// The checks that the three entry points share (host).
+inline int check_pools(const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
+                       int64_t page_size, int n_heads, int head_dim, int wide_type, int cache_type) {
+  ASG_REQUIRE(is_wide(wide_type), ASG_EINVAL, "the type of the tokens must be float32, bfloat16 or float16");
+  ASG_REQUIRE(is_wide(cache_type) || is_coded(cache_type), ASG_EINVAL, "unknown type of the pages");
+  ASG_REQUIRE(n_pages >= 0 && page_size >= 1 && n_heads >= 1 && head_dim >= 1, ASG_EINVAL,
+              "n_pages must be non-negative, page_size, heads and head_dim positive");
+  ASG_REQUIRE(head_dim <= kMaxDim, ASG_ERANGE, "the paged kernels hold at most 256 features per head");
+  ASG_REQUIRE(n_pages <= 2147483647ll && page_size < (1ll << 30) && n_heads <= 65535, ASG_ERANGE,
+              "n_pages, page_size or n_heads exceeds the kernel index range");
+  ASG_REQUIRE(key_pool != nullptr && value_pool != nullptr, ASG_EINVAL, "key_pool and value_pool must not be null");
+  ASG_REQUIRE(n_pages == 0 || (key_pool->data != nullptr && value_pool->data != nullptr), ASG_EINVAL,
+              "the pages must not be null");
+  if (is_coded(cache_type))
+    ASG_REQUIRE(n_pages == 0 || (key_pool->scales != nullptr && value_pool->scales != nullptr), ASG_EINVAL,
+                "8-bit pages need scales");
+  return ASG_OK;
+}
+
+#ifdef __CUDACC__
+
+// Storage types and their float32 values.
+using F32 = float;
+using BF16 = __nv_bfloat16;
+using F16 = __half;
+struct E4M3 { uint8_t code; };
+struct INT8 { int8_t code; };
+
+template <typename T> struct TypeOf;
+template <> struct TypeOf<F32> { static constexpr int id = ASG_TYPE_F32; static constexpr bool coded = false; };
+template <> struct TypeOf<BF16> { static constexpr int id = ASG_TYPE_BF16; static constexpr bool coded = false; };
+template <> struct TypeOf<F16> { static constexpr int id = ASG_TYPE_F16; static constexpr bool coded = false; };
+template <> struct TypeOf<E4M3> { static constexpr int id = ASG_TYPE_E4M3; static constexpr bool coded = true; };
+template <> struct TypeOf<INT8> { static constexpr int id = ASG_TYPE_INT8; static constexpr bool coded = true; };
+
+__device__ __forceinline__ float to_float(F32 v) { return v; }
+__device__ __forceinline__ float to_float(BF16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(F16 v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(E4M3 v) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v.code, __NV_E4M3)));
+}
+__device__ __forceinline__ float to_float(INT8 v) { return static_cast<float>(v.code); }
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ F32 from_float<F32>(float v) { return v; }
+template <> __device__ __forceinline__ BF16 from_float<BF16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ F16 from_float<F16>(float v) { return __float2half_rn(v); }
+
+// N consecutive elements, moved in vectors of up to 16 bytes (the address is a multiple of that).
+template <typename T, int N>
+struct Pack {
+  static constexpr int kBytes = N * static_cast<int>(sizeof(T));
+  static constexpr int kVec = kBytes < 16 ? kBytes : 16;
+  alignas(kVec) T v[N];
+  __device__ __forceinline__ void load(const T* p) { move(v, p); }
+  __device__ __forceinline__ void store(T* p) const { move(p, v); }
+  static __device__ __forceinline__ void move(T* to, const T* from) {
+    if constexpr (kVec == 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
+    } else if constexpr (kVec == 8) {
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
+    } else if constexpr (kVec == 4) {
+      *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+    } else {
+      static_assert(kVec == 2, "no such vector");
+      *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+    }
+  }
+};
+
+// page and place of a slot; most caches have fewer than 2^32 slots, and a 64-bit division is long
+__device__ __forceinline__ void split_slot(long long slot, int page_size, long long& page, int& place) {
+  if (static_cast<unsigned long long>(slot) >> 32 == 0) {
+    const unsigned s = static_cast<unsigned>(slot), q = s / static_cast<unsigned>(page_size);
+    page = q;
+    place = static_cast<int>(s - q * static_cast<unsigned>(page_size));
+  } else {
+    page = slot / page_size;
+    place = static_cast<int>(slot - page * page_size);
+  }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace paged
+}  // namespace asg

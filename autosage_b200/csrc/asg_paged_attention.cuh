@@ -1,0 +1,286 @@
+// Attention of one new token per sequence over a paged cache: what its kernels share.
+//
+// The work is a flat list of units: a unit is kUnit consecutive tokens of one item, an item is one row
+// (sequence) with the query heads of one group (up to GT heads that share a key head).  The list runs over
+// rows, inside a row over items, inside an item over tokens; CTA c of G takes the units [c S, (c + 1) S),
+// S = ceil(total / G), so every CTA streams the same number of cache bytes whatever the lengths are, one
+// long row fills the GPU, and an item is cut only where a CTA's share ends.  A piece that is a whole item
+// is normalised and stored at once; the others leave (max, sum, accumulator) in the workspace, at most two
+// per CTA (the piece it begins with and the piece it ends with), and join_kernel puts them together in the
+// order of the tokens, so results do not depend on timing.  Nothing waits on another CTA.
+//
+// Softmax: scores are kept in units of log2 (scale * log2(e) is folded into q), each warp keeps a running
+// maximum m, sum l and accumulator o of its tokens:
+//   m' = max(m, s),  o' = o 2^(m - m') + 2^(s - m') v,  l' = l 2^(m - m') + 2^(s - m').
+// With 8-bit pages the key scale multiplies the score and the value scale the weight; codes are never
+// multiplied out in memory.
+#pragma once
+
+#include <math_constants.h>
+
+#include "asg_paged.cuh"
+
+namespace asg {
+namespace paged {
+
+constexpr int kWarps = 4;                  // warps of a CTA; each takes every fourth tile of a piece
+constexpr int kUnit = 64;                  // tokens per unit: one 16-token tile for each warp
+constexpr int kTile = kUnit / kWarps;
+constexpr int kMaxCtasPerSm = 4;           // bounds the workspace; no kernel is launched with more
+
+struct AttentionArgs {
+  const int64_t* crow;
+  const int64_t* col;
+  const int64_t* lengths;
+  const void* q;
+  void* out;
+  float* lse;
+  asg_page_pool key, value;
+  long long q_token_stride, q_head_stride;
+  long long n_cols, n_pages, window;
+  int n_rows, page_size, n_heads, n_kv_heads, dim;
+  int group;        // query heads per key head
+  int subgroups;    // items per key head: ceil(group / GT)
+  int type;         // of q and out
+  float scale_log2; // scale * log2(e)
+  float* partial;   // [G][2][GT][dim] accumulators of unfinished pieces
+  float2* stats;    // [G][2][GT] their (m, l)
+  int4* pieces;     // [G] (row, item, starts an item it does not finish, 0 / 1 / 2: see below)
+};
+// pieces[c].w: how CTA c's first piece continues an earlier CTA's item: 0 it does not, 1 it ends it,
+// 2 the item goes on into CTA c + 1.
+
+size_t workspace_bytes_for(int ctas, int gt, int dim);
+
+#ifdef __CUDACC__
+
+// Tokens [first, last) of a row that are seen, and where its pages start in col.  Whatever the arrays hold,
+// nothing outside them is addressed: crow is cut to [0, n_cols], lengths to what the pages hold.
+struct RowSpan {
+  long long first, last, pages_begin;
+  __device__ __forceinline__ long long units() const { return (last - first + kUnit - 1) / kUnit; }
+};
+__device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
+  const long long n_cols = a.n_cols;
+  const long long lo = a.crow[row], hi = a.crow[row + 1], n = a.lengths[row];
+  RowSpan s;
+  s.pages_begin = lo < 0 ? 0 : (lo > n_cols ? n_cols : lo);
+  const long long end = hi < s.pages_begin ? s.pages_begin : (hi > n_cols ? n_cols : hi);
+  const long long held = (end - s.pages_begin) * a.page_size;
+  s.last = n < 0 ? 0 : (n > held ? held : n);
+  s.first = a.window > 0 && s.last > a.window ? s.last - a.window : 0;
+  return s;
+}
+
+// Where a CTA's share begins.
+struct Share {
+  long long pos, end;   // in units, flat
+  long long row_begin;  // flat index of the row's first unit
+  int row;
+};
+
+// Every thread sums the units of its rows, a block scan finds the row that holds the first unit.
+__device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
+  __shared__ long long warp_total[kWarps];
+  __shared__ long long found_begin;
+  __shared__ int found_row;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per_thread = (a.n_rows + kWarps * 32 - 1) / (kWarps * 32);
+  const long long r0 = static_cast<long long>(tid) * per_thread;
+  long long mine = 0;
+  for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) mine += row_span(a, static_cast<int>(r)).units();
+  long long scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long other = __shfl_up_sync(kFull, scan, o);
+    if (lane >= o) scan += other;
+  }
+  if (lane == 31) warp_total[warp] = scan;
+  if (tid == 0) found_row = -1;
+  __syncthreads();
+  long long before = scan - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_total[w];
+    total += warp_total[w];
+  }
+  total *= items_per_row;
+  const long long per_cta = (total + gridDim.x - 1) / gridDim.x;
+  Share s;
+  s.pos = per_cta * blockIdx.x;
+  s.end = s.pos + per_cta < total ? s.pos + per_cta : total;
+  if (s.pos < s.end) {
+    long long at = before * items_per_row;
+    if (s.pos >= at && s.pos < at + mine * items_per_row) {  // exactly one thread
+      long long r = r0;
+      for (; r + 1 < a.n_rows; ++r) {
+        const long long here = row_span(a, static_cast<int>(r)).units() * items_per_row;
+        if (s.pos < at + here) break;
+        at += here;
+      }
+      found_row = static_cast<int>(r);
+      found_begin = at;
+    }
+  }
+  __syncthreads();
+  s.row = found_row;
+  s.row_begin = found_begin;
+  return s;
+}
+
+// First row after `row` that has units (there is one), looked for by all lanes together.
+__device__ __forceinline__ int next_row(const AttentionArgs& a, int row) {
+  for (int base = row + 1; base < a.n_rows; base += 32) {
+    const int r = base + lane_id();
+    const bool some = r < a.n_rows && row_span(a, r).units() > 0;
+    const unsigned who = __ballot_sync(kFull, some);
+    if (who != 0) return base + __ffs(who) - 1;
+  }
+  return a.n_rows;
+}
+
+__device__ __forceinline__ float load_wide(const void* p, long long i, int type) {
+  if (type == ASG_TYPE_F32) return static_cast<const float*>(p)[i];
+  if (type == ASG_TYPE_BF16) return __bfloat162float(static_cast<const BF16*>(p)[i]);
+  return __half2float(static_cast<const F16*>(p)[i]);
+}
+__device__ __forceinline__ void store_wide(void* p, long long i, int type, float v) {
+  if (type == ASG_TYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (type == ASG_TYPE_BF16) static_cast<BF16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<F16*>(p)[i] = __float2half_rn(v);
+}
+
+// 2^(m - top) as the factor of a part with maximum m and sum l; a part without tokens counts nothing,
+// one that holds a NaN keeps it.
+__device__ __forceinline__ float part_factor(float m, float l, float top) {
+  return m == -CUDART_INF_F && l == 0.f ? 0.f : exp2f(m - top);
+}
+__device__ __forceinline__ float log_sum(float top, float sum) {
+  return sum == 0.f ? -CUDART_INF_F : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// The warps' parts of one piece lie in shared memory: o[kWarps][GT][pitch], ml[kWarps][GT] = (m, l).  Puts them
+// together and stores the result (whole item) or a partial record.  All threads call it between barriers.
+template <int GT>
+__device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot,
+                                            const float* o, int pitch, const float2* ml) {
+  const int first_head = kv_head * a.group + sub * GT;
+  const int heads = min(GT, a.group - sub * GT);
+  for (int i = threadIdx.x; i < heads * a.dim; i += blockDim.x) {
+    const int g = i / a.dim, d = i - g * a.dim;
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * GT + g].x);
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 s = ml[w * GT + g];
+      const float f = part_factor(s.x, s.y, top);
+      sum += f * s.y;
+      acc += f * o[(w * GT + g) * pitch + d];
+    }
+    if (slot < 0) {
+      const long long head = static_cast<long long>(row) * a.n_heads + first_head + g;
+      store_wide(a.out, head * a.dim + d, a.type, sum == 0.f ? 0.f : acc / sum);
+      if (a.lse != nullptr && d == 0) a.lse[head] = log_sum(top, sum);
+    } else {
+      const long long record = (static_cast<long long>(blockIdx.x) * 2 + slot) * GT + g;
+      a.partial[record * a.dim + d] = acc;
+      if (d == 0) a.stats[record] = make_float2(top, sum);
+    }
+  }
+}
+
+// Rows that see nothing: every CTA clears its share of them.
+__device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a) {
+  for (long long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+    if (row_span(a, static_cast<int>(r)).units() > 0) continue;
+    for (int i = threadIdx.x; i < a.n_heads * a.dim; i += blockDim.x)
+      store_wide(a.out, r * a.n_heads * a.dim + i, a.type, 0.f);
+    if (a.lse != nullptr)
+      for (int h = threadIdx.x; h < a.n_heads; h += blockDim.x) a.lse[r * a.n_heads + h] = -CUDART_INF_F;
+  }
+}
+
+// The kernel around an Engine, which computes one warp's part of a piece:
+//   Engine(smem)                                  once
+//   begin(a, row, first head, heads)              when the item changes
+//   run(a, span, kv_head, first, last)            the warp's tiles of tokens [first, last) of the row
+//   publish(o, pitch, ml)                         its part into shared memory
+template <typename Engine>
+__global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
+  constexpr int GT = Engine::kHeads;
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_release_dependents();
+  const int items_per_row = a.n_kv_heads * a.subgroups;
+  Share s = locate_share(a, items_per_row);
+  int4 piece = make_int4(0, 0, 0, 0);
+  if (s.pos < s.end) {
+    Engine engine(smem);
+    float* o = Engine::merge_buffer(smem);
+    float2* ml = reinterpret_cast<float2*>(o + kWarps * GT * Engine::kPitch);
+    RowSpan span = row_span(a, s.row);
+    long long units = span.units();
+    int item = static_cast<int>((s.pos - s.row_begin) / units);
+    long long u0 = (s.pos - s.row_begin) - item * units;
+    for (;;) {
+      const long long left = s.end - s.pos;
+      const long long u1 = units - u0 <= left ? units : u0 + left;
+      const int kv_head = item / a.subgroups, sub = item - kv_head * a.subgroups;
+      engine.begin(a, s.row, kv_head * a.group + sub * GT, min(GT, a.group - sub * GT));
+      const long long first = span.first + u0 * kUnit;
+      const long long last = u1 == units ? span.last : span.first + u1 * kUnit;
+      engine.run(a, span, kv_head, first, last);
+      engine.publish(o, ml);
+      __syncthreads();
+      int slot = -1;  // a whole item
+      if (u0 > 0) {
+        slot = 0;
+        piece.w = u1 == units ? 1 : 2;
+      } else if (u1 < units) {
+        slot = 1;
+        piece.x = s.row;
+        piece.y = item;
+        piece.z = 1;
+      }
+      store_piece<GT>(a, s.row, kv_head, sub, slot, o, Engine::kPitch, ml);
+      __syncthreads();  // the buffers are free again
+      s.pos += u1 - u0;
+      if (s.pos >= s.end) break;
+      u0 = 0;
+      if (++item == items_per_row) {
+        item = 0;
+        s.row = next_row(a, s.row);
+        if (s.row >= a.n_rows) break;
+        span = row_span(a, s.row);
+        units = span.units();
+      }
+    }
+  }
+  if (threadIdx.x == 0) a.pieces[blockIdx.x] = piece;
+  clear_empty_rows(a);
+}
+
+// Host: attributes and launch of one instance, at most `most_ctas` CTAs.
+template <typename Engine>
+int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
+  auto kernel = attention_kernel<Engine>;
+  if (Engine::kSmem > 48 * 1024)
+    ASG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Engine::kSmem));
+  kernel<<<ctas, kWarps * 32, Engine::kSmem, stream>>>(args);
+  ASG_CUDA(cudaGetLastError());
+  return ASG_OK;
+}
+
+#endif  // __CUDACC__
+
+// What a family of engines would launch for given sizes; `launch` null: the family does not take them.
+struct Choice {
+  int gt = 0;          // query heads per item
+  int ctas_per_sm = 0;
+  int (*launch)(const AttentionArgs&, int ctas, cudaStream_t) = nullptr;
+};
+Choice choose_general(const AttentionArgs& a, int cache_type);  // asg_paged_general.cu
+
+}  // namespace paged
+}  // namespace asg

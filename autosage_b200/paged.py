@@ -1,0 +1,216 @@
+"""Attention of new tokens over a paged cache of keys and values, and the cache itself.
+
+``csr_attention_forward`` computes all rows of an attention pattern at once.  A model that answers token by
+token has one new query a sequence and keeps the keys and values of the tokens before it; here they lie in
+pages of a fixed number of tokens, and the page table is a CSR pattern of its own: row = sequence, column =
+page id, in the order of the tokens.
+
+    paged_cache_write     keys and values of new tokens into their slots, quantised on the way if the pages are 8-bit
+    paged_cache_read      tokens out of their slots again
+    csr_paged_attention   one new token of every sequence attends to the tokens of its pages
+
+Pages are ``[n_pages, page_size, n_kv_heads, head_dim]`` tensors, one for keys and one for values, in float32,
+bfloat16, float16, ``float8_e4m3fn`` or int8, with any strides whose features are contiguous.  The two 8-bit types
+go with float32 scales ``[n_pages, n_kv_heads, page_size]``, one for each row of ``head_dim`` features: value =
+code * scale.  A slot is ``page * page_size + place in the page``.
+
+These are operators of inference: there is no backward, and a call that would need one is refused.  The reference
+has no counterpart (its attention, ``autosage/_auto.py:762-780``, is the whole-pattern form).
+"""
+from __future__ import annotations
+
+import os
+from typing import Optional
+
+import torch
+
+from . import _native, ops
+
+_WIDE = (torch.float32, torch.bfloat16, torch.float16)
+_CODED = (torch.float8_e4m3fn, torch.int8)
+_INDEX_DTYPES = (torch.int32, torch.int64)
+MAX_HEAD_DIM = 256
+
+
+def _index(name: str, tensor: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if tensor.dtype not in _INDEX_DTYPES:
+        raise TypeError(f"{name} must use integer indices")
+    if tensor.ndim != 1:
+        raise ValueError(f"{name} must be one-dimensional")
+    if tensor.device != device:
+        raise ValueError(f"{name} must be on the device of the pages")
+    return tensor.to(torch.long).contiguous()
+
+
+def _check_pages(key_pages, value_pages, key_scales, value_scales) -> None:
+    if key_pages.ndim != 4 or key_pages.shape != value_pages.shape:
+        raise ValueError("key_pages and value_pages must have the same [n_pages, page_size, n_kv_heads, head_dim] shape")
+    _, page_size, heads, dim = key_pages.shape
+    if min(page_size, heads, dim) < 1:
+        raise ValueError("page_size, n_kv_heads and head_dim must be positive")
+    if dim > MAX_HEAD_DIM:
+        raise ValueError(f"head_dim is at most {MAX_HEAD_DIM}")
+    if key_pages.dtype != value_pages.dtype or key_pages.dtype not in _WIDE + _CODED:
+        raise TypeError("the pages must both be float32, bfloat16, float16, float8_e4m3fn or int8")
+    if dim > 1 and (key_pages.stride(3) != 1 or value_pages.stride(3) != 1):
+        raise ValueError("the features of a page row must be contiguous")
+    device = key_pages.device
+    if value_pages.device != device:
+        raise ValueError("key_pages and value_pages must be on the same device")
+    if key_pages.dtype in _CODED:
+        for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
+            if scales is None:
+                raise ValueError(f"8-bit pages need {name}")
+            if scales.dtype != torch.float32:
+                raise TypeError(f"{name} must be float32")
+            if scales.shape != (key_pages.size(0), heads, page_size):
+                raise ValueError(f"{name} must have shape [n_pages, n_kv_heads, page_size]")
+            if scales.device != device:
+                raise ValueError(f"{name} must be on the device of the pages")
+    elif key_scales is not None or value_scales is not None:
+        raise ValueError("scales go with 8-bit pages only")
+
+
+def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    if device.type != "cuda":
+        raise RuntimeError("the paged cache needs CUDA tensors")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
+    if not ops.load_native():
+        detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
+        raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")
+
+
+def _contiguous_features(rows: torch.Tensor) -> torch.Tensor:
+    return rows if rows.size(-1) <= 1 or rows.stride(-1) == 1 else rows.contiguous()
+
+
+def _checking() -> bool:
+    return os.getenv("AUTOSAGE_CHECK_INDICES") == "1"
+
+
+def _check_writable(name: str, tensor: Optional[torch.Tensor]) -> None:
+    if tensor is not None and any(step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
+        raise ValueError(f"{name} is written and must not repeat memory (it has a stride of 0)")
+
+
+def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
+                      value_pages: torch.Tensor, *, key_scales: Optional[torch.Tensor] = None,
+                      value_scales: Optional[torch.Tensor] = None) -> None:
+    """Writes token t of ``key`` and ``value`` (``[T, n_kv_heads, head_dim]``) to slot ``slots[t]`` of the pages, in place.
+
+    Pages have the type of the tokens, or an 8-bit type: then ``scale = max|x| / 448`` (e4m3) or ``/ 127`` (int8) over
+    the features of a row, and each code is the nearest to ``x / scale``, ties to even.  A row with an infinity or a
+    NaN reads back as NaN.
+
+    A slot outside the pages (-1, say) is skipped: padding.  The others must differ from one another: of two tokens
+    with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call)."""
+    _check_pages(key_pages, value_pages, key_scales, value_scales)
+    if key.ndim != 3 or key.shape != value.shape or key.shape[1:] != key_pages.shape[2:]:
+        raise ValueError("key and value must have the same [tokens, n_kv_heads, head_dim] shape, as wide as the pages")
+    if key.dtype != value.dtype or key.dtype not in _WIDE:
+        raise TypeError("key and value must both be float32, bfloat16 or float16")
+    if key_pages.dtype not in _CODED and key_pages.dtype != key.dtype:
+        raise TypeError("the pages must have the type of key and value, or an 8-bit type")
+    device = key_pages.device
+    if key.device != device or value.device != device:
+        raise ValueError("key and value must be on the device of the pages")
+    slots = _index("slots", slots, device)
+    if slots.numel() != key.size(0):
+        raise ValueError("slots must contain one slot per token")
+    for name, tensor in (("key_pages", key_pages), ("value_pages", value_pages), ("key_scales", key_scales),
+                         ("value_scales", value_scales)):
+        _check_writable(name, tensor)
+    _require_native(device, key, value, key_pages, value_pages)
+    if slots.numel() == 0 or key_pages.size(0) == 0:
+        return
+    if _checking():
+        kept = slots[(slots >= 0) & (slots < key_pages.size(0) * key_pages.size(1))]
+        if kept.unique().numel() != kept.numel():
+            raise RuntimeError("two tokens have the same slot")
+    _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
+                              key_scales, value_scales)
+
+
+def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, *,
+                     key_scales: Optional[torch.Tensor] = None, value_scales: Optional[torch.Tensor] = None,
+                     dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values in the slots ``slots``, as two ``[T, n_kv_heads, head_dim]`` tensors of type ``dtype`` (that
+    of the pages, or float32 for 8-bit pages).  Slots may repeat; one outside the pages reads as zeros."""
+    _check_pages(key_pages, value_pages, key_scales, value_scales)
+    if dtype is None:
+        dtype = torch.float32 if key_pages.dtype in _CODED else key_pages.dtype
+    if dtype not in _WIDE:
+        raise TypeError("dtype must be float32, bfloat16 or float16")
+    device = key_pages.device
+    slots = _index("slots", slots, device)
+    _require_native(device, key_pages, value_pages, key_scales, value_scales)
+    shape = (slots.numel(), key_pages.size(2), key_pages.size(3))
+    key, value = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    if slots.numel():
+        _native.paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales)
+    return key, value
+
+
+def _debug_check_table(crow, col, lengths, n_pages: int, page_size: int) -> None:
+    """AUTOSAGE_CHECK_INDICES=1: verify the page table before the launch (synchronises)."""
+    if not _checking():
+        return
+    if int(crow[0].item()) != 0 or int(crow[-1].item()) != col.numel():
+        raise RuntimeError("crow must run from 0 to the number of columns")
+    pages = crow[1:] - crow[:-1]
+    if bool((pages < 0).any().item()):
+        raise RuntimeError("crow must be non-decreasing")
+    if bool(((lengths < 0) | (lengths > pages * page_size)).any().item()):
+        raise RuntimeError("lengths must lie between 0 and what the pages of the row hold")
+    if col.numel() and int(col.max().item()) >= n_pages:
+        raise RuntimeError(f"page ids must lie below {n_pages}")
+
+
+def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Tensor, query: torch.Tensor,
+                        key_pages: torch.Tensor, value_pages: torch.Tensor, *,
+                        key_scales: Optional[torch.Tensor] = None, value_scales: Optional[torch.Tensor] = None,
+                        scale: Optional[float] = None, window: Optional[int] = None, return_lse: bool = False):
+    """``softmax_t(scale * <query, k_t>) v_t`` for one new token of every sequence.
+
+    ``crow`` ``[B + 1]`` and ``col`` are the page table in CSR form (row r owns the pages ``col[crow[r]:crow[r + 1]]``, in
+    the order of its tokens) and ``lengths`` ``[B]`` the number of tokens of each row, at most what its pages hold.  ``query``
+    is ``[B, n_heads, head_dim]`` with ``n_heads`` a multiple of the pages' ``n_kv_heads``: neighbouring query heads
+    share a key head.  Pages have the type of the query, or an 8-bit type.  ``scale=None`` leaves the scores unscaled, as in
+    ``csr_attention_forward``; ``window=w`` lets a token see the last w tokens of its row only.
+
+    Returns ``[B, n_heads, head_dim]`` in the type of the query and, with ``return_lse=True``, the natural
+    logarithm of each softmax's denominator as float32 ``[B, n_heads]`` (parts computed over different pages can be
+    joined with it).  A row that sees nothing gives 0 and ``-inf``.  A page id outside the pages is a hole whose
+    tokens are not seen; whatever lies behind a row's length in its last pages is not read."""
+    _check_pages(key_pages, value_pages, key_scales, value_scales)
+    device = key_pages.device
+    if query.ndim != 3 or query.size(2) != key_pages.size(3):
+        raise ValueError("query must have shape [rows, n_heads, head_dim] with the pages' head_dim")
+    if query.size(1) < 1 or query.size(1) % key_pages.size(2) != 0:
+        raise ValueError("n_heads must be a positive multiple of n_kv_heads")
+    if query.dtype not in _WIDE:
+        raise TypeError("query must be float32, bfloat16 or float16")
+    if key_pages.dtype not in _CODED and key_pages.dtype != query.dtype:
+        raise TypeError("the pages must have the type of the query, or an 8-bit type")
+    if query.device != device:
+        raise ValueError("query must be on the device of the pages")
+    crow, col, lengths = _index("crow", crow, device), _index("col", col, device), _index("lengths", lengths, device)
+    rows = query.size(0)
+    if crow.numel() != rows + 1:
+        raise ValueError("crow must contain one entry per row and one more")
+    if lengths.numel() != rows:
+        raise ValueError("lengths must contain one entry per row")
+    if window is not None and window < 1:
+        raise ValueError("window must be positive")
+    _require_native(device, query, key_pages, value_pages, key_scales, value_scales)
+    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    if rows:
+        _debug_check_table(crow, col, lengths, key_pages.size(0), key_pages.size(1))
+        _native.paged_attention(crow, col, lengths, _contiguous_features(query), out, lse, key_pages, value_pages, key_scales,
+                                value_scales, scale=1.0 if scale is None else float(scale), window=int(window or 0))
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["csr_paged_attention", "paged_cache_read", "paged_cache_write"]

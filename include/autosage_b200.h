@@ -334,6 +334,84 @@ int64_t asg_static_max_rows(void);
  */
 int asg_static_status(const void* device_pointer, int32_t* host_status, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Paged cache and its attention (no counterpart in the reference, whose attention sees all queries of
+ * a graph at once).  A cache keeps the keys and values of past tokens in pages of page_size tokens; a
+ * page table in CSR form lists the pages of every sequence (row = sequence, column = page id), and one
+ * new token of every sequence attends to the tokens of its pages.
+ */
+#define ASG_TYPE_F32 0
+#define ASG_TYPE_BF16 1
+#define ASG_TYPE_F16 2
+#define ASG_TYPE_E4M3 3 /* 8-bit float, largest value 448 */
+#define ASG_TYPE_INT8 4 /* codes -127 ... 127 */
+
+/* Key or value pages: element (page, token, head, d) lies at data + page * page_stride + token *
+ * token_stride + head * head_stride + d, strides in elements, features contiguous.  The two 8-bit types
+ * carry one float32 scale for each (page, head, token): value = code * scale. */
+typedef struct asg_page_pool {
+  void* data;
+  float* scales; /* NULL for the wider types */
+  int64_t page_stride, token_stride, head_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+} asg_page_pool;
+
+/* Rows of new tokens: element (token, head, d) at data + token * token_stride + head * head_stride + d. */
+typedef struct asg_token_rows {
+  void* data;
+  int64_t token_stride, head_stride;
+} asg_token_rows;
+
+/*
+ * Writes the keys and values of n_tokens new tokens into the cache: token t goes to slot slots[t] =
+ * page * page_size + place in the page.  A slot below 0 or not below n_pages * page_size is skipped (a
+ * padded batch).  The other slots of one call must differ from one another.
+ * cache_type is in_type, or one of the 8-bit types: then scale = max|x| / 448 or / 127 over the
+ * features of the row, held in float32, and code = x / scale rounded to the nearest code (ties to
+ * even; the quotient is not rounded first).  A row with an infinity or a NaN reads back as NaN.
+ * head_dim at most 256.
+ */
+int asg_paged_cache_write(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key,
+                          const asg_token_rows* value, const asg_page_pool* key_pool,
+                          const asg_page_pool* value_pool, int64_t n_pages, int64_t page_size, int n_heads,
+                          int head_dim, int in_type, int cache_type, void* stream);
+
+/*
+ * Reads tokens back: row t of key and value (type out_type, any of the three wider ones) becomes the
+ * token in slot slots[t], code * scale (a float32 product) for the 8-bit types; zeros where the slot
+ * lies outside the cache.
+ */
+int asg_paged_cache_read(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key,
+                         const asg_token_rows* value, const asg_page_pool* key_pool,
+                         const asg_page_pool* value_pool, int64_t n_pages, int64_t page_size, int n_heads,
+                         int head_dim, int out_type, int cache_type, void* stream);
+
+/* Bytes of workspace of asg_paged_attention (the partial results of rows that several CTAs share). */
+size_t asg_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+
+/*
+ * out[r, h, :] = softmax_t(scale * <q[r, h, :], k_t>) v_t over the tokens t of row r, for one query
+ * token a row; lse[r, h] = log sum_t exp(scale * <q, k_t>) when lse is not NULL (natural logarithm).
+ *   crow[n_rows + 1], col[n_cols]  the page table: row r owns the pages col[crow[r] ... crow[r + 1])
+ *   lengths[n_rows]   tokens of the row, the one in place i of the row's page j being token
+ *                     j * page_size + i; cut to what the row's pages hold
+ *   window            > 0: only the last `window` tokens of a row are seen; 0: all
+ *   n_heads           query heads, a multiple of n_kv_heads; query head h uses key head
+ *                     h / (n_heads / n_kv_heads)
+ *   type, cache_type  of q and out, and of the pages: equal, or cache_type one of the 8-bit types
+ * q takes the layout of asg_token_rows, out is [n_rows, n_heads, head_dim] and lse [n_rows, n_heads],
+ * both contiguous.  A page id outside [0, n_pages) is a hole: its tokens are not seen.  A row that sees
+ * nothing gets out = 0, lse = -inf.  The tokens behind a row's length are never read.  Scores, softmax
+ * and sums are held in float32.  head_dim at most 256.  The workspace is 256-byte aligned; its content
+ * need not be kept or cleared between calls.
+ */
+int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* lengths, int64_t n_rows,
+                        int64_t n_cols, const asg_token_rows* q, void* out, float* lse,
+                        const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
+                        int64_t page_size, int n_heads, int n_kv_heads, int head_dim, float scale,
+                        int64_t window, int type, int cache_type, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
