@@ -139,7 +139,10 @@ int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* 
   a.group = n_heads / n_kv_heads;
   a.type = type;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const Choice choice = choose_general(a, cache_type);
+  // 16-bit queries run on the tensor cores wherever 16-byte copies can fetch the rows; float32 queries, whose
+  // products have to keep 24 bits, and everything else on the FMA pipe
+  Choice choice = is_coded(cache_type) ? choose_tensor8(a, cache_type) : choose_tensor16(a, cache_type);
+  if (choice.launch == nullptr) choice = choose_general(a, cache_type);
   a.subgroups = (a.group + choice.gt - 1) / choice.gt;
   // no more CTAs than units there can be (every row may end in a partly filled one)
   const int64_t items = static_cast<int64_t>(n_kv_heads) * a.subgroups;

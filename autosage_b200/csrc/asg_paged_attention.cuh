@@ -159,11 +159,12 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
   return sum == 0.f ? -CUDART_INF_F : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
-// The warps' parts of one piece lie in shared memory: o[kWarps][GT][pitch], ml[kWarps][GT] = (m, l).  Puts them
-// together and stores the result (whole item) or a partial record.  All threads call it between barriers.
+// The warps' parts of one piece lie in shared memory: warp w's accumulators o[w * warp_stride + g * pitch + d] and
+// ml[w * GT + g] = (m, l).  Puts them together and stores the result (whole item) or a partial record.  All threads
+// call it between barriers.
 template <int GT>
 __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot,
-                                            const float* o, int pitch, const float2* ml) {
+                                            const float* o, int warp_stride, int pitch, const float2* ml) {
   const int first_head = kv_head * a.group + sub * GT;
   const int heads = min(GT, a.group - sub * GT);
   for (int i = threadIdx.x; i < heads * a.dim; i += blockDim.x) {
@@ -177,7 +178,7 @@ __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int
       const float2 s = ml[w * GT + g];
       const float f = part_factor(s.x, s.y, top);
       sum += f * s.y;
-      acc += f * o[(w * GT + g) * pitch + d];
+      acc += f * o[w * warp_stride + g * pitch + d];
     }
     if (slot < 0) {
       const long long head = static_cast<long long>(row) * a.n_heads + first_head + g;
@@ -206,7 +207,9 @@ __device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a) {
 //   Engine(smem)                                  once
 //   begin(a, row, first head, heads)              when the item changes
 //   run(a, span, kv_head, first, last)            the warp's tiles of tokens [first, last) of the row
-//   publish(o, pitch, ml)                         its part into shared memory
+//   publish(smem, ml)                             its part into shared memory: float o[kHeads][kPitch] at
+//                                                 smem + warp * kWarpBytes (its own region, which run() may use too)
+// kWarpBytes * kWarps bytes of shared memory belong to the engine, the (m, l) pairs lie behind them.
 template <typename Engine>
 __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
   constexpr int GT = Engine::kHeads;
@@ -217,8 +220,8 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
   int4 piece = make_int4(0, 0, 0, 0);
   if (s.pos < s.end) {
     Engine engine(smem);
-    float* o = Engine::merge_buffer(smem);
-    float2* ml = reinterpret_cast<float2*>(o + kWarps * GT * Engine::kPitch);
+    const float* o = reinterpret_cast<const float*>(smem);
+    float2* ml = reinterpret_cast<float2*>(smem + kWarps * Engine::kWarpBytes);
     RowSpan span = row_span(a, s.row);
     long long units = span.units();
     int item = static_cast<int>((s.pos - s.row_begin) / units);
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
       const long long first = span.first + u0 * kUnit;
       const long long last = u1 == units ? span.last : span.first + u1 * kUnit;
       engine.run(a, span, kv_head, first, last);
-      engine.publish(o, ml);
+      engine.publish(smem, ml);
       __syncthreads();
       int slot = -1;  // a whole item
       if (u0 > 0) {
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
         piece.y = item;
         piece.z = 1;
       }
-      store_piece<GT>(a, s.row, kv_head, sub, slot, o, Engine::kPitch, ml);
+      store_piece<GT>(a, s.row, kv_head, sub, slot, o, Engine::kWarpBytes / 4, Engine::kPitch, ml);
       __syncthreads();  // the buffers are free again
       s.pos += u1 - u0;
       if (s.pos >= s.end) break;
@@ -261,13 +264,16 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
   clear_empty_rows(a);
 }
 
-// Host: attributes and launch of one instance, at most `most_ctas` CTAs.
+// Host: launch of one instance.
 template <typename Engine>
 int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
+  constexpr int smem = kWarps * (Engine::kWarpBytes + Engine::kHeads * static_cast<int>(sizeof(float2)));
+  static_assert(Engine::kWarpBytes >= Engine::kHeads * Engine::kPitch * 4 && Engine::kWarpBytes % 128 == 0, "warp region");
+  static_assert(Engine::kCtasPerSm <= kMaxCtasPerSm && Engine::kCtasPerSm * (smem + 1024) <= 228 * 1024, "shared memory");
   auto kernel = attention_kernel<Engine>;
-  if (Engine::kSmem > 48 * 1024)
-    ASG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Engine::kSmem));
-  kernel<<<ctas, kWarps * 32, Engine::kSmem, stream>>>(args);
+  if (smem > 48 * 1024)
+    ASG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<ctas, kWarps * 32, smem, stream>>>(args);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }
@@ -281,6 +287,17 @@ struct Choice {
   int (*launch)(const AttentionArgs&, int ctas, cudaStream_t) = nullptr;
 };
 Choice choose_general(const AttentionArgs& a, int cache_type);  // asg_paged_general.cu
+Choice choose_tensor16(const AttentionArgs& a, int cache_type); // asg_paged_tensor16.cu
+Choice choose_tensor8(const AttentionArgs& a, int cache_type);  // asg_paged_tensor8.cu
+
+template <typename Engine>
+inline Choice made() {
+  Choice c;
+  c.gt = Engine::kHeads;
+  c.ctas_per_sm = Engine::kCtasPerSm;
+  c.launch = launch_engine<Engine>;
+  return c;
+}
 
 }  // namespace paged
 }  // namespace asg

@@ -18,9 +18,8 @@ struct General {
   static constexpr int TB = E == 8 ? 4 : (GT == 8 ? 4 : 8);  // tokens per batch: K and V rows of a batch are in registers
   static constexpr int N = TB * GT;                          // scores per batch: 4 ... 32
   static constexpr int kShift = N == 32 ? 0 : N == 16 ? 1 : N == 8 ? 2 : 3;
-  static constexpr int kSmem = kWarps * GT * (kPitch * 4 + 8);
+  static constexpr int kWarpBytes = GT * kPitch * 4;
   static_assert(N == 32 || N == 16 || N == 8 || N == 4, "reduce-scatter sizes");
-  static __device__ __forceinline__ float* merge_buffer(unsigned char* smem) { return reinterpret_cast<float*>(smem); }
 
   float q[GT][E], o[GT][E];
   float m, l;  // of the head that this lane owns scores of: head (lane >> kShift) % GT
@@ -166,7 +165,8 @@ struct General {
     }
   }
 
-  __device__ __forceinline__ void publish(float* buffer, float2* ml) {
+  __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
+    float* buffer = reinterpret_cast<float*>(smem) + warp * GT * kPitch;
     // the sum of a head is spread over the lanes that own its scores of different tokens
 #pragma unroll
     for (int step = 16; step >= GT << kShift; step >>= 1) l += __shfl_xor_sync(kFull, l, step);
@@ -175,18 +175,9 @@ struct General {
 #pragma unroll
     for (int g = 0; g < GT; ++g)
 #pragma unroll
-      for (int e = 0; e < E; ++e) buffer[(warp * GT + g) * kPitch + feature(lane, e)] = o[g][e];
+      for (int e = 0; e < E; ++e) buffer[g * kPitch + feature(lane, e)] = o[g][e];
   }
 };
-
-template <typename Engine>
-static Choice made() {
-  Choice c;
-  c.gt = Engine::kHeads;
-  c.ctas_per_sm = Engine::kCtasPerSm;
-  c.launch = launch_engine<Engine>;
-  return c;
-}
 
 // Heads per item: the group if it is small; a group of more takes several items, whose second reading of
 // the keys and values comes from L2.  Features wider than 128 leave room for four heads in registers.

@@ -1,0 +1,496 @@
+// Paged attention on the tensor cores: 16-bit queries, 16-bit or 8-bit pages.
+//
+// A decoding step multiplies each key with the few query heads of its group, so it is bound by the bytes of
+// the cache; what the kernel has to do is keep enough of them in flight and stay out of their way.  The
+// tiles are far too thin for tcgen05 (its smallest tile is 64 or 128 rows on a side that here holds 1 to 16
+// query heads, or 8 columns against 128 tokens whose rows would have to be gathered into one swizzled operand), so
+// the products use the warp-level instruction m16n8k16 with the TOKENS as its 16 rows and the query heads as
+// its 8 columns: half the instructions of the other orientation for groups of up to 8.
+//
+//   S^T[16 tokens x 8 heads] = K Q^T      A = K rows (ldmatrix), B = Q^T in registers for the whole item
+//   O^T[16 d x 8 heads]     += V^T P^T    A = V columns (ldmatrix.trans), B = the weights: S^T's registers
+//                                         packed to 16 bits and transposed by movmatrix, no trip to memory
+// The weights enter as two 16-bit pieces (p = hi + lo, 2^-17 of p lost at most), so that the result is as
+// good as one with float32 weights: the second product costs nothing while the kernel waits for memory.
+//
+// Each warp works alone: 16-token tiles, a ring of kStages tiles of its own in shared memory filled by
+// cp.async 16 bytes at a time (rows padded by 16 bytes, so ldmatrix is free of bank conflicts), page ids
+// fetched one tile ahead of the copies that need them.  The warps of a CTA meet only at the end of a piece.
+//
+// 8-bit pages.  Codes stay codes in shared memory and become f16 numbers in registers, exactly:
+//   int8   0x6400 | (c + 128) is the number 1024 + c + 128; subtract 1152
+//   e4m3   the hardware's conversion of two at a time
+// A byte-wise ldmatrix hands a lane four neighbouring features of a token (K) or two features of two tokens
+// (V, transposed in 16-bit units); the order of features inside a k-step or of output rows inside a block
+// is free, so Q and O are simply laid out to match.  f16 holds codes whole but not every scale, so
+//   - a query head is multiplied by the power of two that brings its largest feature into [1, 2) (features
+//     below 2^-14 of that lose what lies below 2^-24 of it), undone in the factor of its scores;
+//   - the accumulator has a running reference of its own: with value scales c_t it holds
+//     sum_t 2^(s_t + log2 |c_t| - r) sign(c_t) code_t, r the largest s_t + log2 |c_t| so far, so its weights are
+//     at most 1 whatever the scales are, and 2^(r - m) brings it to the common maximum m in the end.
+#pragma once
+
+#include "asg_paged_attention.cuh"
+
+namespace asg {
+namespace paged {
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename H>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<BF16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<F16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// bytes of global memory into shared memory, zeros if !ok (nothing is read then)
+__device__ __forceinline__ void copy_async16(uint32_t to, const void* from, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t to, const void* from, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Two floats as two 16-bit numbers (first in the low half), and what they lose.
+template <typename H> __device__ __forceinline__ uint32_t pack2(float a, float b, float& rest_a, float& rest_b);
+template <>
+__device__ __forceinline__ uint32_t pack2<BF16>(float a, float b, float& rest_a, float& rest_b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const float2 f = __bfloat1622float2(h);
+  rest_a = a - f.x;
+  rest_b = b - f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<F16>(float a, float b, float& rest_a, float& rest_b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  rest_a = a - f.x;
+  rest_b = b - f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Bytes I and J of x, codes of type T, as two f16 numbers.
+constexpr uint32_t byte_selector(uint32_t i, uint32_t j) { return i | (4u << 4) | (j << 8) | (5u << 12); }
+template <int I, int J>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t x, INT8) {
+  const uint32_t biased = __byte_perm(x ^ 0x80808080u, 0x64646464u, byte_selector(I, J));
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int I, int J>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t x, E4M3) {
+  const uint32_t two = I == 0 && J == 1 ? x : I == 2 && J == 3 ? x >> 16 : __byte_perm(x, 0u, I | (J << 4) | 0x4400u);
+  const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(v.x) | (static_cast<uint32_t>(v.y) << 16);
+}
+
+// T: type of the pages; DP: features, padded; NT: groups of 8 heads.
+template <typename T, int DP, int NT, int STAGES, int CTAS>
+struct Tensor {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kCtasPerSm = CTAS;
+  static constexpr int kStages = STAGES;
+  static constexpr bool kCoded = TypeOf<T>::coded;
+  static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+  static constexpr int kRowPitch = kRowBytes + 16;
+  static constexpr int kChunks = kRowBytes / 16;                    // 16-byte pieces of a row
+  static constexpr int kValues = kTile * kRowPitch;                 // offset of the V tile in a stage
+  static constexpr int kExtras = 2 * kTile * kRowPitch;             // then the scales (key, value), then the mask of seen tokens
+  static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * kTile * 4 : 0) + 4 + 15) / 16 * 16;
+  static constexpr int kPitch = DP + 4;                             // of the published accumulators: no bank conflicts
+  static constexpr int kNeed = kStages * kStageBytes > kHeads * kPitch * 4 ? kStages * kStageBytes : kHeads * kPitch * 4;
+  static constexpr int kWarpBytes = (kNeed + 127) / 128 * 128;
+  static constexpr int kSteps = DP / 16;
+  using H = typename std::conditional<kCoded, F16, T>::type;        // type of the products
+  // f16 weights are held 2^14 above their value: the pieces of small weights stay clear of f16's smallest step
+  static constexpr float kLift = std::is_same<H, F16>::value ? 14.f : 0.f;
+
+  uint32_t q[NT][kSteps][2];
+  float o[NT][kSteps][4];
+  float m[NT][2], l[NT][2];  // of heads 8 nt + 2 (lane % 4) + {0, 1}
+  float ref[NT][2];          // 8-bit pages: the accumulator's own reference, and what undoes the query's power of two
+  float unit[NT][2];
+  int lane, warp, dim_bytes;
+  uint32_t ring;             // shared address of the warp's region
+
+  __device__ __forceinline__ explicit Tensor(unsigned char* smem)
+      : lane(threadIdx.x & 31), warp(threadIdx.x >> 5), ring(smem_u32(smem) + warp * kWarpBytes) {}
+
+  // Feature that a lane's register holds in step `step`: entry 0 or 1 of the pair `half`.
+  static __device__ __forceinline__ int query_feature(int step, int lane, int half, int entry) {
+    return kCoded ? 16 * step + 4 * (lane & 3) + 2 * half + entry : 16 * step + 8 * half + 2 * (lane & 3) + entry;
+  }
+  static __device__ __forceinline__ int output_feature(int step, int lane, int half) {
+    return kCoded ? 16 * step + 2 * (lane >> 2) + half : 16 * step + 8 * half + (lane >> 2);
+  }
+
+  __device__ __forceinline__ void begin(const AttentionArgs& a, int row, int head, int heads) {
+    const long long base = row * a.q_token_stride + head * a.q_head_stride;
+    dim_bytes = a.dim * static_cast<int>(sizeof(T));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = 8 * nt + (lane >> 2);
+      const long long from = base + h * a.q_head_stride;
+      if constexpr (!kCoded) {
+        const uint16_t* bits = static_cast<const uint16_t*>(a.q) + from;
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t pair = 0;
+#pragma unroll
+            for (int entry = 0; entry < 2; ++entry) {
+              const int d = query_feature(step, lane, half, entry);
+              if (h < heads && d < a.dim) pair |= static_cast<uint32_t>(bits[d]) << (16 * entry);
+            }
+            q[nt][step][half] = pair;
+          }
+      } else {
+        float top = 0.f;
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = query_feature(step, lane, i >> 1, i & 1);
+            if (h < heads && d < a.dim) top = fmaxf(top, fabsf(load_wide(a.q, from + d, a.type)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+        int power = (__float_as_int(top) >> 23) - 127;  // top in [2^power, 2^(power + 1)); 0 and infinity: as they are
+        power = power < -126 || power > 126 ? 0 : power;
+        const float down = __int_as_float((127 - power) << 23), up = __int_as_float((127 + power) << 23);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x[2];
+#pragma unroll
+            for (int entry = 0; entry < 2; ++entry) {
+              const int d = query_feature(step, lane, half, entry);
+              x[entry] = h < heads && d < a.dim ? load_wide(a.q, from + d, a.type) * down : 0.f;
+            }
+            float none0, none1;
+            q[nt][step][half] = pack2<F16>(x[0], x[1], none0, none1);
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unit[nt][i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
+          ref[nt][i] = -CUDART_INF_F;
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][step][i] = 0.f;
+      m[nt][0] = m[nt][1] = -CUDART_INF_F;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+    if (dim_bytes < kRowBytes) {  // features past the head's end are never copied: they are zeros
+      const int first = dim_bytes / 16, missing = kChunks - first;
+      for (int i = lane; i < kStages * 2 * kTile * missing; i += 32) {
+        const int r = i / missing, chunk = first + i - r * missing;
+        const int stage = r / (2 * kTile), line = r - stage * 2 * kTile;
+        const uint32_t at = ring + stage * kStageBytes + line * kRowPitch + chunk * 16;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+      }
+      __syncwarp();
+    }
+  }
+
+  // Where the copies of a piece come from.
+  struct Source {
+    const char* keys;
+    const char* values;
+    const int64_t* ids;  // of the page that holds the piece's first token
+    int place0, count;
+    int kv_head;
+  };
+  // page (or -1) and place of token (lane % 16) of the tile that starts at `tile`
+  __device__ __forceinline__ void find(const AttentionArgs& a, const Source& s, int tile, long long& id, int& place) const {
+    id = -1;
+    place = 0;
+    const int token = tile + (lane & (kTile - 1));
+    if (token < s.count) {
+      const unsigned at = static_cast<unsigned>(s.place0) + static_cast<unsigned>(token);
+      const unsigned nth = at / static_cast<unsigned>(a.page_size);
+      place = static_cast<int>(at - nth * static_cast<unsigned>(a.page_size));
+      id = s.ids[nth];
+    }
+  }
+  __device__ __forceinline__ void issue(const AttentionArgs& a, const Source& s, int stage, long long id, int place) const {
+    const bool held = id >= 0 && id < a.n_pages;
+    const int page = held ? static_cast<int>(id) : -1;
+    const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
+    const uint32_t base = ring + stage * kStageBytes;
+#pragma unroll
+    for (int n = 0; n < kTile * kChunks / 32; ++n) {
+      const int index = n * 32 + lane, line = index / kChunks, chunk = index % kChunks;
+      const int p = __shfl_sync(kFull, page, line), in = __shfl_sync(kFull, place, line);
+      if (chunk * 16 < dim_bytes) {
+        const long long kp = p < 0 ? 0 : p * a.key.page_stride + in * a.key.token_stride;
+        const long long vp = p < 0 ? 0 : p * a.value.page_stride + in * a.value.token_stride;
+        const uint32_t to = base + line * kRowPitch + chunk * 16;
+        copy_async16(to, s.keys + kp * static_cast<int>(sizeof(T)) + chunk * 16, p >= 0);
+        copy_async16(to + kValues, s.values + vp * static_cast<int>(sizeof(T)) + chunk * 16, p >= 0);
+      }
+    }
+    if constexpr (kCoded) {
+      const asg_page_pool& pool = lane < kTile ? a.key : a.value;
+      const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
+      if (held) from += id * pool.scale_page_stride + place * pool.scale_token_stride;
+      copy_async4(base + kExtras + lane * 4, from, held);
+    }
+    if (lane == 0)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + kStageBytes - 4), "r"(seen) : "memory");
+  }
+
+  __device__ __forceinline__ void run(const AttentionArgs& a, const RowSpan& span, int kv_head, long long first, long long last) {
+    Source s;
+    s.keys = static_cast<const char*>(a.key.data) + kv_head * a.key.head_stride * static_cast<int>(sizeof(T));
+    s.values = static_cast<const char*>(a.value.data) + kv_head * a.value.head_stride * static_cast<int>(sizeof(T));
+    const long long page0 = first / a.page_size;  // page arithmetic in 32 bits from here on
+    s.place0 = static_cast<int>(first - page0 * a.page_size);
+    s.ids = a.col + span.pages_begin + page0;
+    s.count = static_cast<int>(last - first);
+    s.kv_head = kv_head;
+
+    int tile = warp * kTile;  // next tile to copy
+    long long id;
+    int place;
+    find(a, s, tile, id, place);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (tile < s.count) issue(a, s, i, id, place);
+      copy_commit();
+      tile += kUnit;
+      find(a, s, tile, id, place);
+    }
+    int stage = 0, fill = kStages - 1;
+    for (int now = warp * kTile; now < s.count; now += kUnit) {
+      copy_wait<kStages - 2>();
+      __syncwarp();  // the tile has arrived for all lanes, and all have left the stage that is filled next
+      if (tile < s.count) issue(a, s, fill, id, place);
+      copy_commit();
+      tile += kUnit;
+      find(a, s, tile, id, place);
+      compute(a, ring + stage * kStageBytes);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      fill = fill + 1 == kStages ? 0 : fill + 1;
+    }
+    copy_wait<0>();
+    __syncwarp();
+  }
+
+  // Largest score of one head in the tile (the lanes of equal lane % 4 hold its tokens), and the one before.
+  static __device__ __forceinline__ float largest_of_tile(float x0, float x1, float before) {
+    float top = fmaxf(x0, x1);
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 16));
+    return fmaxf(top, before);
+  }
+
+  __device__ __forceinline__ void compute(const AttentionArgs& a, uint32_t base) {
+    const uint32_t line16 = base + (lane & 15) * kRowPitch + (lane >> 4) * 16;
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+    if constexpr (!kCoded) {
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        uint32_t k[4];
+        ldmatrix_x4(k, line16 + step * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<H>(s[nt], k, q[nt][step][0], q[nt][step][1]);
+      }
+    } else {
+#pragma unroll
+      for (int step = 0; step < kSteps; step += 2) {  // 32 bytes: two steps of 16 features
+        uint32_t c[4];
+        ldmatrix_x4(c, line16 + step * 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t k[4] = {decode_pair<0, 1>(c[2 * i], T{}), decode_pair<0, 1>(c[2 * i + 1], T{}),
+                                 decode_pair<2, 3>(c[2 * i], T{}), decode_pair<2, 3>(c[2 * i + 1], T{})};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<H>(s[nt], k, q[nt][step + i][0], q[nt][step + i][1]);
+        }
+      }
+    }
+    // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 8 nt + 2 (lane % 4) + {0, 1}
+    unsigned seen;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(base + kStageBytes - 4));
+    float key_scale[2], value_log[2], value_sign[2];
+    bool in[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int token = (lane >> 2) + 8 * t;
+      in[t] = (seen >> token & 1u) != 0;
+      if constexpr (kCoded) {
+        float scale;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale[t]) : "r"(base + kExtras + token * 4));
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(base + kExtras + (kTile + token) * 4));
+        value_log[t] = log2f(fabsf(scale));
+        value_sign[t] = copysignf(1.f, scale);
+      }
+    }
+    float shrink[NT][2];  // of the accumulator
+    bool moved = false;
+    uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[2][2];  // [token][head]
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if constexpr (kCoded) x[t] = in[t] ? s[nt][2 * t + h] * (key_scale[t] * unit[nt][h]) : -CUDART_INF_F;
+          else x[t] = in[t] ? s[nt][2 * t + h] * a.scale_log2 : -CUDART_INF_F;
+        }
+        const float top = largest_of_tile(x[0], x[1], m[nt][h]);
+        const float at = top == -CUDART_INF_F ? 0.f : top;
+        const float fade = exp2f(m[nt][h] - at);
+        m[nt][h] = top;
+        const float lifted = at - kLift;
+        w[0][h] = exp2f(x[0] - lifted);
+        w[1][h] = exp2f(x[1] - lifted);
+        l[nt][h] = l[nt][h] * fade + (w[0][h] + w[1][h]);
+        shrink[nt][h] = fade;
+        if constexpr (kCoded) {
+          x[0] = in[0] ? x[0] + value_log[0] : -CUDART_INF_F;  // (a scale of 0 weighs nothing)
+          x[1] = in[1] ? x[1] + value_log[1] : -CUDART_INF_F;
+          const float new_ref = largest_of_tile(x[0], x[1], ref[nt][h]);
+          const float from = new_ref == -CUDART_INF_F ? 0.f : new_ref;
+          shrink[nt][h] = exp2f(ref[nt][h] - from);
+          ref[nt][h] = new_ref;
+          w[0][h] = value_sign[0] * exp2f(x[0] - (from - kLift));
+          w[1][h] = value_sign[1] * exp2f(x[1] - (from - kLift));
+        }
+        moved = moved || shrink[nt][h] != 1.f;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float rest0, rest1, none0, none1;
+        high[nt][t] = transpose_8x8(pack2<H>(w[t][0], w[t][1], rest0, rest1));
+        low[nt][t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));
+      }
+    }
+    if (__any_sync(kFull, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          o[nt][step][0] *= shrink[nt][0];
+          o[nt][step][1] *= shrink[nt][1];
+          o[nt][step][2] *= shrink[nt][0];
+          o[nt][step][3] *= shrink[nt][1];
+        }
+    }
+    if constexpr (!kCoded) {
+      const uint32_t line_v = base + kValues + ((lane & 7) + ((lane >> 4) << 3)) * kRowPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        uint32_t v[4];
+        ldmatrix_x4_trans(v, line_v + step * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<H>(o[nt][step], v, high[nt][0], high[nt][1]);
+          mma16816<H>(o[nt][step], v, low[nt][0], low[nt][1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int step = 0; step < kSteps; step += 2) {
+        uint32_t c[4];
+        ldmatrix_x4_trans(c, line16 + kValues + step * 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t v[4] = {decode_pair<0, 2>(c[2 * i], T{}), decode_pair<1, 3>(c[2 * i], T{}),
+                                 decode_pair<0, 2>(c[2 * i + 1], T{}), decode_pair<1, 3>(c[2 * i + 1], T{})};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<H>(o[nt][step + i], v, high[nt][0], high[nt][1]);
+            mma16816<H>(o[nt][step + i], v, low[nt][0], low[nt][1]);
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
+    float* to = reinterpret_cast<float*>(smem + warp * kWarpBytes);
+    constexpr float undo = kLift == 0.f ? 1.f : 1.f / 16384.f;
+    static_assert(kLift == 0.f || kLift == 14.f, "2^-kLift");
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int head = 8 * nt + 2 * (lane & 3) + h;
+        float sum = l[nt][h];
+        sum += __shfl_xor_sync(kFull, sum, 4);
+        sum += __shfl_xor_sync(kFull, sum, 8);
+        sum += __shfl_xor_sync(kFull, sum, 16);
+        if (lane < 4) ml[warp * kHeads + head] = make_float2(m[nt][h], sum * undo);
+        float back = undo;  // of the accumulator, to the maximum m
+        if (kCoded && ref[nt][h] != -CUDART_INF_F) back *= exp2f(ref[nt][h] - m[nt][h]);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            to[head * kPitch + output_feature(step, lane, half)] = o[nt][step][2 * half + h] * back;
+      }
+    }
+  }
+};
+
+// Stages of a warp's ring and CTAs per SM.  About 100 KB of the cache in flight per SM cover the latency of
+// HBM at full rate; the rest of the 227 KB decides how many warps share the arithmetic.
+template <typename T, int NT>
+inline Choice choose_padded(const AttentionArgs& a) {
+  if constexpr (sizeof(T) == 1) {
+    if (a.dim <= 64) return made<Tensor<T, 64, NT, 4, 4>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 3>>();
+    return made<Tensor<T, 256, NT, 3, 2>>();
+  } else {
+    if (a.dim <= 64) return made<Tensor<T, 64, NT, 3, 3>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 2>>();
+    return made<Tensor<T, 256, NT, 3, 1>>();
+  }
+}
+template <typename T>
+inline Choice choose_tensor(const AttentionArgs& a) {
+  const int item = static_cast<int>(sizeof(T));
+  if (a.dim * item % 16 != 0 || !rows_aligned(a.key, item, 16) || !rows_aligned(a.value, item, 16)) return Choice{};
+  return a.group <= 8 ? choose_padded<T, 1>(a) : choose_padded<T, 2>(a);
+}
+
+#endif  // __CUDACC__
+
+}  // namespace paged
+}  // namespace asg

@@ -62,7 +62,8 @@ def attention(crow, col, lengths, query, key, value, page_size, scale, window):
         # score: dim products added in float32, the tensor core truncating each sum (two half steps), and the
         # factors scale * log2(e), the key scale and the running maximum: eight more roundings of |s| or less
         size = torch.einsum("hgd,thd->hgt", q.abs(), k.abs()).amax(-1) * abs(scale)
-        score = (2 * dim + 8) * eps * size
+        # (8-bit pages: the query is held to 2^-24 of its largest feature, rounded to half of that)
+        score = (2 * dim + 8) * eps * size + eps / 2 * (q.abs().amax(-1, keepdim=True) * k.abs().sum(-1).t().unsqueeze(1)).amax(-1) * abs(scale)
         # weight: twice the score error (it and the sum), the exponential, the running factors of the sums
         count = ids.numel()
         relative = 2 * score + (2 * count + 32) * eps
