@@ -6,23 +6,26 @@ namespace paged {
 
 size_t workspace_bytes_for(int ctas, int gt, int dim) {
   const size_t records = static_cast<size_t>(ctas) * 2 * gt;
-  return align256(static_cast<size_t>(ctas) * sizeof(int4)) + align256(records * sizeof(float2)) + align256(records * dim * sizeof(float));
+  return align256(static_cast<size_t>(ctas) * sizeof(int4)) + align256(records * sizeof(float2)) + align256(records * ((dim + 3) / 4 * 4) * sizeof(float));
 }
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 
-// Block (c, g): if CTA c's last piece starts an item that it does not finish, puts head g of that item together
-// from CTA c's piece and the first pieces of the CTAs after it, in order.
+// Block (c, y): if CTA c's last piece starts an item that it does not finish, puts the heads y, y + gridDim.y, ... of
+// that item together from CTA c's piece and the first pieces of the CTAs after it.  The threads of a block share
+// a head's features, four a thread, and where some are left over the pieces too; their sums are added in a fixed order.
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs a, int ctas, int gt) {
   extern __shared__ float factor[];  // [ctas]
   __shared__ float s_part[kJoinThreads / 32];
+  __shared__ float4 s_sum[kJoinThreads];
   __shared__ int s_last;
+  const int c = blockIdx.x, tid = threadIdx.x;
+  if (blockIdx.y == 0) clear_empty_rows(a, c, ctas);
   pdl_wait_for_primary();
-  const int c = blockIdx.x, g = blockIdx.y, tid = threadIdx.x;
   const int4 piece = a.pieces[c];
   if (piece.z == 0) return;
   const int kv_head = piece.y / a.subgroups, sub = piece.y - kv_head * a.subgroups;
-  if (sub * gt + g >= a.group) return;
+  const int heads = min(gt, a.group - sub * gt);
   // the CTA that ends the item: the first after c whose first piece does not go on
   if (tid == 0) s_last = ctas - 1;
   __syncthreads();
@@ -32,41 +35,71 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
     if (__syncthreads_or(ends)) break;
   }
   const int n = s_last - c + 1;
-  auto record = [&](int i) { return (static_cast<long long>(c + i) * 2 + (i == 0 ? 1 : 0)) * gt + g; };
-  float top = -CUDART_INF_F;
-  for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, a.stats[record(i)].x);
-  top = warp_max(top);
-  if ((tid & 31) == 0) s_part[tid >> 5] = top;
-  __syncthreads();
-  top = s_part[0];
+  const int fours = (a.dim + 3) / 4;
+  int slices = 1;  // threads that share four features, a power of two
+  while (slices * 2 * fours <= kJoinThreads) slices *= 2;
+  const int slice = tid / fours, column = tid - slice * fours;
+  for (int g = blockIdx.y; g < heads; g += gridDim.y) {
+    auto record = [&](int i) { return (static_cast<long long>(c + i) * 2 + (i == 0 ? 1 : 0)) * gt + g; };
+    __syncthreads();  // factor, s_part and s_sum of the head before have been read
+    float top = -CUDART_INF_F;
+    for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, a.stats[record(i)].x);
+    top = warp_max(top);
+    if ((tid & 31) == 0) s_part[tid >> 5] = top;
+    __syncthreads();
+    top = s_part[0];
 #pragma unroll
-  for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_part[w]);
-  float sum = 0.f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float2 s = a.stats[record(i)];
-    factor[i] = part_factor(s.x, s.y, top);
-    sum += factor[i] * s.y;
-  }
-  sum = warp_sum(sum);
-  __syncthreads();  // s_part has been read
-  if ((tid & 31) == 0) s_part[tid >> 5] = sum;
-  __syncthreads();
-  sum = 0.f;
+    for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_part[w]);
+    __syncthreads();
+    float sum = 0.f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+      const float2 s = a.stats[record(i)];
+      factor[i] = part_factor(s.x, s.y, top);
+      sum += factor[i] * s.y;
+    }
+    sum = warp_sum(sum);
+    if ((tid & 31) == 0) s_part[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_part[w];
-  const long long head = static_cast<long long>(piece.x) * a.n_heads + kv_head * a.group + sub * gt + g;
-  for (int d = tid; d < a.dim; d += kJoinThreads) {
-    float acc = 0.f;
+    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_part[w];
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (slice < slices) {
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) acc += factor[i] * a.partial[record(i) * a.dim + d];
-    store_wide(a.out, head * a.dim + d, a.type, sum == 0.f ? 0.f : acc / sum);
+      for (int i = slice; i < n; i += slices) {
+        const float4 x = *reinterpret_cast<const float4*>(a.partial + record(i) * a.partial_pitch + column * 4);
+        const float f = factor[i];
+        acc.x += f * x.x;
+        acc.y += f * x.y;
+        acc.z += f * x.z;
+        acc.w += f * x.w;
+      }
+      s_sum[tid] = acc;
+    }
+    __syncthreads();
+    const long long row = static_cast<long long>(piece.x) * a.n_heads + kv_head * a.group + sub * gt + g;
+    if (slice == 0) {
+      for (int i = 1; i < slices; ++i) {
+        const float4 x = s_sum[i * fours + column];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+      }
+      const float scale = sum == 0.f ? 0.f : 1.f / sum;
+      store_four(a, row, column * 4, make_float4(acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale));
+    }
+    if (a.lse != nullptr && tid == 0) a.lse[row] = log_sum(top, sum);
   }
-  if (a.lse != nullptr && tid == 0) a.lse[head] = log_sum(top, sum);
 }
 
-static int launch_join(const AttentionArgs& args, int ctas, int gt, cudaStream_t stream) {
+static int launch_join(const AttentionArgs& args, int ctas, int gt, int64_t items, cudaStream_t stream) {
+  // an item cut into many pieces is worth a block per head (there are few such items, so few blocks find work);
+  // where items are cut once, one block goes through the heads
+  const int heads = args.group < gt ? args.group : gt;
+  const bool many = items * 4 < ctas;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(gt));
+  config.gridDim = dim3(static_cast<unsigned>(ctas), many ? static_cast<unsigned>(heads) : 1u);
   config.blockDim = dim3(kJoinThreads);
   config.dynamicSmemBytes = sizeof(float) * static_cast<size_t>(ctas);
   config.stream = stream;
@@ -78,7 +111,6 @@ static int launch_join(const AttentionArgs& args, int ctas, int gt, cudaStream_t
   ASG_CUDA(cudaLaunchKernelEx(&config, join_kernel, args, ctas, gt));
   return ASG_OK;
 }
-
 
 }  // namespace paged
 }  // namespace asg
@@ -139,6 +171,9 @@ int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* 
   a.group = n_heads / n_kv_heads;
   a.type = type;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.q_pairs = rows_aligned(*q, type_bytes(type), 8);
+  a.out_vector = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  a.partial_pitch = (head_dim + 3) / 4 * 4;
   // 16-bit queries run on the tensor cores wherever 16-byte copies can fetch the rows; float32 queries, whose
   // products have to keep 24 bits, and everything else on the FMA pipe
   Choice choice = is_coded(cache_type) ? choose_tensor8(a, cache_type) : choose_tensor16(a, cache_type);
@@ -160,7 +195,7 @@ int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* 
   a.partial = reinterpret_cast<float*>(at);
   if (int rc = choice.launch(a, ctas, stream)) return rc;
   if (ctas == 1) return ASG_OK;  // nothing is shared
-  return launch_join(a, ctas, choice.gt, stream);
+  return launch_join(a, ctas, choice.gt, items * n_rows, stream);
 }
 
 }  // extern "C"

@@ -43,7 +43,10 @@ struct AttentionArgs {
   int subgroups;    // items per key head: ceil(group / GT)
   int type;         // of q and out
   float scale_log2; // scale * log2(e)
-  float* partial;   // [G][2][GT][dim] accumulators of unfinished pieces
+  bool q_pairs;     // the query's rows start on 8 bytes
+  bool out_vector;  // four neighbours of out can be stored at once
+  int partial_pitch;
+  float* partial;   // [G][2][GT][partial_pitch] accumulators of unfinished pieces
   float2* stats;    // [G][2][GT] their (m, l)
   int4* pieces;     // [G] (row, item, starts an item it does not finish, 0 / 1 / 2: see below)
 };
@@ -53,6 +56,13 @@ struct AttentionArgs {
 size_t workspace_bytes_for(int ctas, int gt, int dim);
 
 #ifdef __CUDACC__
+
+// 64-bit quotients that mostly have 32-bit operands (a 64-bit division is some hundred instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if ((static_cast<unsigned long long>(a) | static_cast<unsigned long long>(b)) >> 32 == 0)
+    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
 
 // Tokens [first, last) of a row that are seen, and where its pages start in col.  Whatever the arrays hold,
 // nothing outside them is addressed: crow is cut to [0, n_cols], lengths to what the pages hold.
@@ -105,7 +115,7 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
     total += warp_total[w];
   }
   total *= items_per_row;
-  const long long per_cta = (total + gridDim.x - 1) / gridDim.x;
+  const long long per_cta = quotient(total + gridDim.x - 1, gridDim.x);
   Share s;
   s.pos = per_cta * blockIdx.x;
   s.end = s.pos + per_cta < total ? s.pos + per_cta : total;
@@ -159,42 +169,84 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
   return sum == 0.f ? -CUDART_INF_F : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
-// The warps' parts of one piece lie in shared memory: warp w's accumulators o[w * warp_stride + g * pitch + d] and
+// Four neighbours, or what is left of them, of a result row.
+__device__ __forceinline__ void store_four(const AttentionArgs& a, long long row, int d, float4 v) {
+  const long long at = row * a.dim + d;
+  if (a.out_vector) {
+    if (a.type == ASG_TYPE_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+    } else {
+      uint2 two;
+      if (a.type == ASG_TYPE_BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+        two = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      } else {
+        const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+        two = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = two;
+    }
+    return;
+  }
+  const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (d + i < a.dim) store_wide(a.out, at + i, a.type, x[i]);
+}
+
+// The warps' parts of one piece lie in shared memory: warp w's accumulators o[w * warp_stride + g * PITCH + d] and
 // ml[w * GT + g] = (m, l).  Puts them together and stores the result (whole item) or a partial record.  All threads
 // call it between barriers.
-template <int GT>
+template <int GT, int DIM, int PITCH>
 __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot,
-                                            const float* o, int warp_stride, int pitch, const float2* ml) {
-  const int first_head = kv_head * a.group + sub * GT;
+                                            const float* o, int warp_stride, const float2* ml) {
+  __shared__ float4 factors[GT];
+  static_assert(kWarps == 4, "one float4 of factors per head");
   const int heads = min(GT, a.group - sub * GT);
-  for (int i = threadIdx.x; i < heads * a.dim; i += blockDim.x) {
-    const int g = i / a.dim, d = i - g * a.dim;
-    float top = -CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * GT + g].x);
-    float sum = 0.f, acc = 0.f;
+  const long long first_row = static_cast<long long>(row) * a.n_heads + kv_head * a.group + sub * GT;
+  const long long first_record = (static_cast<long long>(blockIdx.x) * 2 + slot) * GT;
+  const int tid = threadIdx.x;
+  if (tid < heads) {
+    float2 part[kWarps];
+    float top = -CUDART_INF_F, sum = 0.f, f[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float2 s = ml[w * GT + g];
-      const float f = part_factor(s.x, s.y, top);
-      sum += f * s.y;
-      acc += f * o[w * warp_stride + g * pitch + d];
+      part[w] = ml[w * GT + tid];
+      top = fmaxf(top, part[w].x);
     }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      f[w] = part_factor(part[w].x, part[w].y, top);
+      sum += f[w] * part[w].y;
+    }
+    float scale = 1.f;
     if (slot < 0) {
-      const long long head = static_cast<long long>(row) * a.n_heads + first_head + g;
-      store_wide(a.out, head * a.dim + d, a.type, sum == 0.f ? 0.f : acc / sum);
-      if (a.lse != nullptr && d == 0) a.lse[head] = log_sum(top, sum);
+      scale = sum == 0.f ? 0.f : 1.f / sum;
+      if (a.lse != nullptr) a.lse[first_row + tid] = log_sum(top, sum);
     } else {
-      const long long record = (static_cast<long long>(blockIdx.x) * 2 + slot) * GT + g;
-      a.partial[record * a.dim + d] = acc;
-      if (d == 0) a.stats[record] = make_float2(top, sum);
+      a.stats[first_record + tid] = make_float2(top, sum);
     }
+    factors[tid] = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
+  }
+  __syncthreads();
+  constexpr int kFours = DIM / 4;
+  for (int i = tid; i < heads * kFours; i += kWarps * 32) {
+    const int g = i / kFours, d = i % kFours * 4;
+    if (d >= a.dim) continue;
+    const float4 f = factors[g];
+    const float* at = o + g * PITCH + d;
+    const float4 x0 = *reinterpret_cast<const float4*>(at), x1 = *reinterpret_cast<const float4*>(at + warp_stride),
+                 x2 = *reinterpret_cast<const float4*>(at + 2 * warp_stride), x3 = *reinterpret_cast<const float4*>(at + 3 * warp_stride);
+    const float4 v = make_float4(f.x * x0.x + f.y * x1.x + f.z * x2.x + f.w * x3.x, f.x * x0.y + f.y * x1.y + f.z * x2.y + f.w * x3.y,
+                                 f.x * x0.z + f.y * x1.z + f.z * x2.z + f.w * x3.z, f.x * x0.w + f.y * x1.w + f.z * x2.w + f.w * x3.w);
+    if (slot < 0) store_four(a, first_row + g, d, v);
+    else *reinterpret_cast<float4*>(a.partial + (first_record + g) * a.partial_pitch + d) = v;
   }
 }
 
-// Rows that see nothing: every CTA clears its share of them.
-__device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a) {
-  for (long long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+// Rows that see nothing: block `block` of `blocks` clears its share of them.
+__device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a, int block, int blocks) {
+  for (long long r = block; r < a.n_rows; r += blocks) {
     if (row_span(a, static_cast<int>(r)).units() > 0) continue;
     for (int i = threadIdx.x; i < a.n_heads * a.dim; i += blockDim.x)
       store_wide(a.out, r * a.n_heads * a.dim + i, a.type, 0.f);
@@ -224,7 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
     float2* ml = reinterpret_cast<float2*>(smem + kWarps * Engine::kWarpBytes);
     RowSpan span = row_span(a, s.row);
     long long units = span.units();
-    int item = static_cast<int>((s.pos - s.row_begin) / units);
+    int item = static_cast<int>(quotient(s.pos - s.row_begin, units));
     long long u0 = (s.pos - s.row_begin) - item * units;
     for (;;) {
       const long long left = s.end - s.pos;
@@ -246,7 +298,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
         piece.y = item;
         piece.z = 1;
       }
-      store_piece<GT>(a, s.row, kv_head, sub, slot, o, Engine::kWarpBytes / 4, Engine::kPitch, ml);
+      store_piece<GT, Engine::kDim, Engine::kPitch>(a, s.row, kv_head, sub, slot, o, Engine::kWarpBytes / 4, ml);
       __syncthreads();  // the buffers are free again
       s.pos += u1 - u0;
       if (s.pos >= s.end) break;
@@ -261,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
     }
   }
   if (threadIdx.x == 0) a.pieces[blockIdx.x] = piece;
-  clear_empty_rows(a);
+  if (gridDim.x == 1) clear_empty_rows(a, 0, 1);  // otherwise the join kernel does, while this one runs
 }
 
 // Host: launch of one instance.

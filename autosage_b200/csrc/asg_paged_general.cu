@@ -13,7 +13,8 @@ namespace paged {
 template <typename T, int E, int GT, bool VEC>
 struct General {
   static constexpr int kHeads = GT;
-  static constexpr int kPitch = 32 * E;
+  static constexpr int kDim = 32 * E;
+  static constexpr int kPitch = kDim;
   static constexpr int kCtasPerSm = GT * E >= 32 ? 3 : 4;     // registers: q and o take 2 GT E, a batch 2 TB E
   static constexpr int TB = E == 8 ? 4 : (GT == 8 ? 4 : 8);  // tokens per batch: K and V rows of a batch are in registers
   static constexpr int N = TB * GT;                          // scores per batch: 4 ... 32
@@ -65,7 +66,7 @@ struct General {
     const T* keys = static_cast<const T*>(a.key.data) + kv_head * a.key.head_stride;
     const T* values = static_cast<const T*>(a.value.data) + kv_head * a.value.head_stride;
     // page arithmetic in 32 bits, from the page that holds the piece's first token
-    const long long page0 = first / a.page_size;
+    const long long page0 = quotient(first, a.page_size);
     const int place0 = static_cast<int>(first - page0 * a.page_size);
     const long long pages = span.pages_begin + page0;
     const int count = static_cast<int>(last - first);

@@ -69,6 +69,17 @@ __device__ __forceinline__ void copy_async16(uint32_t to, const void* from, bool
 __device__ __forceinline__ void copy_async4(uint32_t to, const void* from, bool ok) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(ok ? 4 : 0) : "memory");
 }
+// 2^x and log2(x) of the hardware (results and arguments below the normal range count as 0)
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -120,6 +131,7 @@ struct Tensor {
   static constexpr int kValues = kTile * kRowPitch;                 // offset of the V tile in a stage
   static constexpr int kExtras = 2 * kTile * kRowPitch;             // then the scales (key, value), then the mask of seen tokens
   static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * kTile * 4 : 0) + 4 + 15) / 16 * 16;
+  static constexpr int kDim = DP;
   static constexpr int kPitch = DP + 4;                             // of the published accumulators: no bank conflicts
   static constexpr int kNeed = kStages * kStageBytes > kHeads * kPitch * 4 ? kStages * kStageBytes : kHeads * kPitch * 4;
   static constexpr int kWarpBytes = (kNeed + 127) / 128 * 128;
@@ -147,35 +159,49 @@ struct Tensor {
     return kCoded ? 16 * step + 2 * (lane >> 2) + half : 16 * step + 8 * half + (lane >> 2);
   }
 
+  // The four query features that a lane holds in a step, as they lie in memory (16 bits each; 8-bit pages: four
+  // neighbours, 16-bit pages: two pairs of neighbours).
+  static __device__ __forceinline__ uint2 load_query(const AttentionArgs& a, const uint16_t* row, bool ok, int step, int lane) {
+    const int d0 = query_feature(step, lane, 0, 0), d1 = query_feature(step, lane, 1, 0);
+    uint2 x = make_uint2(0u, 0u);
+    if (a.q_pairs) {  // whole pairs lie inside or outside the head
+      if constexpr (kCoded) {
+        if (ok && d0 < a.dim) x = *reinterpret_cast<const uint2*>(row + d0);
+      } else {
+        if (ok && d0 < a.dim) x.x = *reinterpret_cast<const uint32_t*>(row + d0);
+        if (ok && d1 < a.dim) x.y = *reinterpret_cast<const uint32_t*>(row + d1);
+      }
+    } else if (ok) {
+      if (d0 < a.dim) x.x = row[d0] | static_cast<uint32_t>(row[d0 + 1]) << 16;
+      if (d1 < a.dim) x.y = row[d1] | static_cast<uint32_t>(row[d1 + 1]) << 16;
+    }
+    return x;
+  }
+  static __device__ __forceinline__ float2 widen(uint32_t pair, bool bf16) {
+    return bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair)) : __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  }
+
   __device__ __forceinline__ void begin(const AttentionArgs& a, int row, int head, int heads) {
-    const long long base = row * a.q_token_stride + head * a.q_head_stride;
     dim_bytes = a.dim * static_cast<int>(sizeof(T));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = 8 * nt + (lane >> 2);
-      const long long from = base + h * a.q_head_stride;
-      if constexpr (!kCoded) {
-        const uint16_t* bits = static_cast<const uint16_t*>(a.q) + from;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) + row * a.q_token_stride + (head + h) * a.q_head_stride;
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t pair = 0;
-#pragma unroll
-            for (int entry = 0; entry < 2; ++entry) {
-              const int d = query_feature(step, lane, half, entry);
-              if (h < heads && d < a.dim) pair |= static_cast<uint32_t>(bits[d]) << (16 * entry);
-            }
-            q[nt][step][half] = pair;
-          }
-      } else {
+      for (int step = 0; step < kSteps; ++step) {
+        const uint2 x = load_query(a, from, h < heads, step, lane);
+        q[nt][step][0] = x.x;
+        q[nt][step][1] = x.y;
+      }
+      if constexpr (kCoded) {
+        const bool bf16 = a.type == ASG_TYPE_BF16;
         float top = 0.f;
 #pragma unroll
         for (int step = 0; step < kSteps; ++step)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = query_feature(step, lane, i >> 1, i & 1);
-            if (h < heads && d < a.dim) top = fmaxf(top, fabsf(load_wide(a.q, from + d, a.type)));
+          for (int half = 0; half < 2; ++half) {
+            const float2 x = widen(q[nt][step][half], bf16);
+            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
           }
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
@@ -186,14 +212,9 @@ struct Tensor {
         for (int step = 0; step < kSteps; ++step)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float x[2];
-#pragma unroll
-            for (int entry = 0; entry < 2; ++entry) {
-              const int d = query_feature(step, lane, half, entry);
-              x[entry] = h < heads && d < a.dim ? load_wide(a.q, from + d, a.type) * down : 0.f;
-            }
+            const float2 x = widen(q[nt][step][half], bf16);
             float none0, none1;
-            q[nt][step][half] = pack2<F16>(x[0], x[1], none0, none1);
+            q[nt][step][half] = pack2<F16>(x.x * down, x.y * down, none0, none1);
           }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -220,82 +241,89 @@ struct Tensor {
     }
   }
 
-  // Where the copies of a piece come from.
+  // Where the copies of a piece come from, and how far they are.  Lane l looks after token l % 16 of the next tile:
+  // the page of the table it lies in, its place there, and the page's id, loaded one tile ahead.
   struct Source {
     const char* keys;
     const char* values;
     const int64_t* ids;  // of the page that holds the piece's first token
-    int place0, count;
-    int kv_head;
+    long long page_bytes, token_bytes;
+    int kv_head, count, tile;
+    int nth, place;
+    int step_pages, step_place;  // kUnit tokens on
+    long long id;
   };
-  // page (or -1) and place of token (lane % 16) of the tile that starts at `tile`
-  __device__ __forceinline__ void find(const AttentionArgs& a, const Source& s, int tile, long long& id, int& place) const {
-    id = -1;
-    place = 0;
-    const int token = tile + (lane & (kTile - 1));
-    if (token < s.count) {
-      const unsigned at = static_cast<unsigned>(s.place0) + static_cast<unsigned>(token);
-      const unsigned nth = at / static_cast<unsigned>(a.page_size);
-      place = static_cast<int>(at - nth * static_cast<unsigned>(a.page_size));
-      id = s.ids[nth];
-    }
+  __device__ __forceinline__ void look_up(Source& s) const {
+    s.id = s.tile + (lane & (kTile - 1)) < s.count ? s.ids[s.nth] : -1;
   }
-  __device__ __forceinline__ void issue(const AttentionArgs& a, const Source& s, int stage, long long id, int place) const {
-    const bool held = id >= 0 && id < a.n_pages;
-    const int page = held ? static_cast<int>(id) : -1;
-    const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
-    const uint32_t base = ring + stage * kStageBytes;
+  __device__ __forceinline__ void issue(const AttentionArgs& a, Source& s, int stage) const {
+    if (s.tile < s.count) {
+      const bool held = s.id >= 0 && s.id < a.n_pages;
+      const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
+      const long long offset = held ? s.id * s.page_bytes + s.place * s.token_bytes : 0;
+      const int offset_low = static_cast<int>(offset), offset_high = static_cast<int>(offset >> 32);
+      const uint32_t base = ring + stage * kStageBytes;
+      constexpr int kLines = 32 / kChunks;  // rows that one copy of all lanes covers
+      const int chunk = lane % kChunks * 16, line0 = lane / kChunks;
+      const uint32_t to = base + line0 * kRowPitch + chunk;
+      const bool inside = chunk < dim_bytes;
 #pragma unroll
-    for (int n = 0; n < kTile * kChunks / 32; ++n) {
-      const int index = n * 32 + lane, line = index / kChunks, chunk = index % kChunks;
-      const int p = __shfl_sync(kFull, page, line), in = __shfl_sync(kFull, place, line);
-      if (chunk * 16 < dim_bytes) {
-        const long long kp = p < 0 ? 0 : p * a.key.page_stride + in * a.key.token_stride;
-        const long long vp = p < 0 ? 0 : p * a.value.page_stride + in * a.value.token_stride;
-        const uint32_t to = base + line * kRowPitch + chunk * 16;
-        copy_async16(to, s.keys + kp * static_cast<int>(sizeof(T)) + chunk * 16, p >= 0);
-        copy_async16(to + kValues, s.values + vp * static_cast<int>(sizeof(T)) + chunk * 16, p >= 0);
+      for (int n = 0; n < kTile / kLines; ++n) {
+        const int line = n * kLines + line0;
+        const unsigned low = static_cast<unsigned>(__shfl_sync(kFull, offset_low, line));
+        const int high = __shfl_sync(kFull, offset_high, line);
+        const long long from = (static_cast<long long>(high) << 32 | low) + chunk;
+        const bool ok = (seen >> line & 1u) != 0;
+        if (inside) {
+          copy_async16(to + n * kLines * kRowPitch, s.keys + from, ok);
+          copy_async16(to + n * kLines * kRowPitch + kValues, s.values + from, ok);
+        }
       }
+      if constexpr (kCoded) {
+        const asg_page_pool& pool = lane < kTile ? a.key : a.value;
+        const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
+        if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
+        copy_async4(base + kExtras + lane * 4, from, held);
+      }
+      if (lane == 0)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + kStageBytes - 4), "r"(seen) : "memory");
     }
-    if constexpr (kCoded) {
-      const asg_page_pool& pool = lane < kTile ? a.key : a.value;
-      const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
-      if (held) from += id * pool.scale_page_stride + place * pool.scale_token_stride;
-      copy_async4(base + kExtras + lane * 4, from, held);
+    copy_commit();
+    s.tile += kUnit;
+    s.nth += s.step_pages;
+    s.place += s.step_place;
+    if (s.place >= a.page_size) {
+      s.place -= a.page_size;
+      ++s.nth;
     }
-    if (lane == 0)
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + kStageBytes - 4), "r"(seen) : "memory");
+    look_up(s);
   }
 
   __device__ __forceinline__ void run(const AttentionArgs& a, const RowSpan& span, int kv_head, long long first, long long last) {
     Source s;
     s.keys = static_cast<const char*>(a.key.data) + kv_head * a.key.head_stride * static_cast<int>(sizeof(T));
     s.values = static_cast<const char*>(a.value.data) + kv_head * a.value.head_stride * static_cast<int>(sizeof(T));
-    const long long page0 = first / a.page_size;  // page arithmetic in 32 bits from here on
-    s.place0 = static_cast<int>(first - page0 * a.page_size);
+    s.page_bytes = a.key.page_stride * static_cast<int>(sizeof(T));
+    s.token_bytes = a.key.token_stride * static_cast<int>(sizeof(T));
+    s.kv_head = kv_head;
+    const unsigned page_size = static_cast<unsigned>(a.page_size);
+    const long long page0 = quotient(first, a.page_size);  // page arithmetic in 32 bits from here on
     s.ids = a.col + span.pages_begin + page0;
     s.count = static_cast<int>(last - first);
-    s.kv_head = kv_head;
-
-    int tile = warp * kTile;  // next tile to copy
-    long long id;
-    int place;
-    find(a, s, tile, id, place);
+    s.tile = warp * kTile;
+    const unsigned at = static_cast<unsigned>(first - page0 * a.page_size) + s.tile + (lane & (kTile - 1));
+    s.nth = static_cast<int>(at / page_size);
+    s.place = static_cast<int>(at % page_size);
+    s.step_pages = static_cast<int>(kUnit / page_size);
+    s.step_place = static_cast<int>(kUnit % page_size);
+    look_up(s);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (tile < s.count) issue(a, s, i, id, place);
-      copy_commit();
-      tile += kUnit;
-      find(a, s, tile, id, place);
-    }
+    for (int i = 0; i < kStages - 1; ++i) issue(a, s, i);
     int stage = 0, fill = kStages - 1;
     for (int now = warp * kTile; now < s.count; now += kUnit) {
       copy_wait<kStages - 2>();
       __syncwarp();  // the tile has arrived for all lanes, and all have left the stage that is filled next
-      if (tile < s.count) issue(a, s, fill, id, place);
-      copy_commit();
-      tile += kUnit;
-      find(a, s, tile, id, place);
+      issue(a, s, fill);
       compute(a, ring + stage * kStageBytes);
       stage = stage + 1 == kStages ? 0 : stage + 1;
       fill = fill + 1 == kStages ? 0 : fill + 1;
@@ -355,7 +383,7 @@ struct Tensor {
         float scale;
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale[t]) : "r"(base + kExtras + token * 4));
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(base + kExtras + (kTile + token) * 4));
-        value_log[t] = log2f(fabsf(scale));
+        value_log[t] = fast_log2(fabsf(scale));
         value_sign[t] = copysignf(1.f, scale);
       }
     }
@@ -375,11 +403,11 @@ struct Tensor {
         }
         const float top = largest_of_tile(x[0], x[1], m[nt][h]);
         const float at = top == -CUDART_INF_F ? 0.f : top;
-        const float fade = exp2f(m[nt][h] - at);
+        const float fade = fast_exp2(m[nt][h] - at);
         m[nt][h] = top;
         const float lifted = at - kLift;
-        w[0][h] = exp2f(x[0] - lifted);
-        w[1][h] = exp2f(x[1] - lifted);
+        w[0][h] = fast_exp2(x[0] - lifted);
+        w[1][h] = fast_exp2(x[1] - lifted);
         l[nt][h] = l[nt][h] * fade + (w[0][h] + w[1][h]);
         shrink[nt][h] = fade;
         if constexpr (kCoded) {
@@ -387,10 +415,10 @@ struct Tensor {
           x[1] = in[1] ? x[1] + value_log[1] : -CUDART_INF_F;
           const float new_ref = largest_of_tile(x[0], x[1], ref[nt][h]);
           const float from = new_ref == -CUDART_INF_F ? 0.f : new_ref;
-          shrink[nt][h] = exp2f(ref[nt][h] - from);
+          shrink[nt][h] = fast_exp2(ref[nt][h] - from);
           ref[nt][h] = new_ref;
-          w[0][h] = value_sign[0] * exp2f(x[0] - (from - kLift));
-          w[1][h] = value_sign[1] * exp2f(x[1] - (from - kLift));
+          w[0][h] = value_sign[0] * fast_exp2(x[0] - (from - kLift));
+          w[1][h] = value_sign[1] * fast_exp2(x[1] - (from - kLift));
         }
         moved = moved || shrink[nt][h] != 1.f;
       }
@@ -487,6 +515,8 @@ template <typename T>
 inline Choice choose_tensor(const AttentionArgs& a) {
   const int item = static_cast<int>(sizeof(T));
   if (a.dim * item % 16 != 0 || !rows_aligned(a.key, item, 16) || !rows_aligned(a.value, item, 16)) return Choice{};
+  // one offset serves a token's key and value
+  if (a.key.page_stride != a.value.page_stride || a.key.token_stride != a.value.token_stride) return Choice{};
   return a.group <= 8 ? choose_padded<T, 1>(a) : choose_padded<T, 2>(a);
 }
 
