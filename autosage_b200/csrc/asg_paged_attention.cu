@@ -11,13 +11,14 @@ size_t workspace_bytes_for(int ctas, int gt, int dim) {
 
 constexpr int kJoinThreads = 256;
 
-// Block (c, y): if CTA c's last piece starts an item that it does not finish, puts the heads y, y + gridDim.y, ... of
-// that item together from CTA c's piece and the first pieces of the CTAs after it.  The threads of a block share
-// a head's features, four a thread, and where some are left over the pieces too; their sums are added in a fixed order.
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs a, int ctas, int gt) {
-  extern __shared__ float factor[];  // [ctas]
-  __shared__ float s_part[kJoinThreads / 32];
-  __shared__ float4 s_sum[kJoinThreads];
+// Block (c, y): if CTA c's last piece starts an item that it does not finish, puts that item together from CTA c's
+// piece and the first pieces of the CTAs after it.  A thread owns four features of a head and walks through the
+// pieces with a running maximum, like the warps through the tokens.  Usually an item has a few pieces, and a
+// thread takes them all; where items are so few that each has many (`sliced`), block y is a head of its own, groups of
+// threads take every slices-th piece, and their parts are added in a fixed order.
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs a, int ctas, int gt, bool sliced) {
+  __shared__ float4 s_acc[kJoinThreads];
+  __shared__ float2 s_stat[kJoinThreads];
   __shared__ int s_last;
   const int c = blockIdx.x, tid = threadIdx.x;
   if (blockIdx.y == 0) clear_empty_rows(a, c, ctas);
@@ -36,79 +37,62 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
   }
   const int n = s_last - c + 1;
   const int fours = (a.dim + 3) / 4;
-  int slices = 1;  // threads that share four features, a power of two
-  while (slices * 2 * fours <= kJoinThreads) slices *= 2;
-  const int slice = tid / fours, column = tid - slice * fours;
-  for (int g = blockIdx.y; g < heads; g += gridDim.y) {
-    auto record = [&](int i) { return (static_cast<long long>(c + i) * 2 + (i == 0 ? 1 : 0)) * gt + g; };
-    __syncthreads();  // factor, s_part and s_sum of the head before have been read
-    float top = -CUDART_INF_F;
-    for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, a.stats[record(i)].x);
-    top = warp_max(top);
-    if ((tid & 31) == 0) s_part[tid >> 5] = top;
-    __syncthreads();
-    top = s_part[0];
-#pragma unroll
-    for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_part[w]);
-    __syncthreads();
-    float sum = 0.f;
-    for (int i = tid; i < n; i += kJoinThreads) {
-      const float2 s = a.stats[record(i)];
-      factor[i] = part_factor(s.x, s.y, top);
-      sum += factor[i] * s.y;
+  int slices = 1;  // a power of two
+  while (sliced && slices * 2 * fours <= kJoinThreads) slices *= 2;
+  const int columns = sliced ? fours : heads * fours;
+  const int slice = sliced ? tid / fours : 0;
+  const int column = sliced ? tid - slice * fours : static_cast<int>(blockIdx.y) * kJoinThreads + tid;
+  const int g = sliced ? static_cast<int>(blockIdx.y) : column / fours;
+  const int d = (column - (sliced ? 0 : g * fours)) * 4;
+  const bool active = slice < slices && column < columns && g < heads;
+  float top = -CUDART_INF_F, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float2 s, float4 x) {
+    const float m = fmaxf(top, s.x);
+    const float keep = part_factor(top, sum, m), f = part_factor(s.x, s.y, m);
+    top = m;
+    sum = sum * keep + s.y * f;
+    acc.x = acc.x * keep + x.x * f;
+    acc.y = acc.y * keep + x.y * f;
+    acc.z = acc.z * keep + x.z * f;
+    acc.w = acc.w * keep + x.w * f;
+  };
+  if (active) {
+#pragma unroll 4
+    for (int i = slice; i < n; i += slices) {
+      const long long record = (static_cast<long long>(c + i) * 2 + (i == 0 ? 1 : 0)) * gt + g;
+      add(a.stats[record], *reinterpret_cast<const float4*>(a.partial + record * a.partial_pitch + d));
     }
-    sum = warp_sum(sum);
-    if ((tid & 31) == 0) s_part[tid >> 5] = sum;
+  }
+  if (sliced) {  // uniform
+    s_stat[tid] = make_float2(top, sum);
+    s_acc[tid] = acc;
     __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_part[w];
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (slice < slices) {
-#pragma unroll 8
-      for (int i = slice; i < n; i += slices) {
-        const float4 x = *reinterpret_cast<const float4*>(a.partial + record(i) * a.partial_pitch + column * 4);
-        const float f = factor[i];
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
-      }
-      s_sum[tid] = acc;
-    }
-    __syncthreads();
+    if (active && slice == 0)
+      for (int i = 1; i < slices; ++i) add(s_stat[i * fours + column], s_acc[i * fours + column]);
+  }
+  if (active && slice == 0) {
     const long long row = static_cast<long long>(piece.x) * a.n_heads + kv_head * a.group + sub * gt + g;
-    if (slice == 0) {
-      for (int i = 1; i < slices; ++i) {
-        const float4 x = s_sum[i * fours + column];
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-      }
-      const float scale = sum == 0.f ? 0.f : 1.f / sum;
-      store_four(a, row, column * 4, make_float4(acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale));
-    }
-    if (a.lse != nullptr && tid == 0) a.lse[row] = log_sum(top, sum);
+    const float scale = sum == 0.f ? 0.f : 1.f / sum;
+    store_four(a, row, d, make_float4(acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale));
+    if (a.lse != nullptr && d == 0) a.lse[row] = log_sum(top, sum);
   }
 }
 
 static int launch_join(const AttentionArgs& args, int ctas, int gt, int64_t items, cudaStream_t stream) {
-  // an item cut into many pieces is worth a block per head (there are few such items, so few blocks find work);
-  // where items are cut once, one block goes through the heads
   const int heads = args.group < gt ? args.group : gt;
-  const bool many = items * 4 < ctas;
+  const bool sliced = items * 8 < ctas;
+  const int blocks = sliced ? heads : (heads * ((args.dim + 3) / 4) + kJoinThreads - 1) / kJoinThreads;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(ctas), many ? static_cast<unsigned>(heads) : 1u);
+  config.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(blocks));
   config.blockDim = dim3(kJoinThreads);
-  config.dynamicSmemBytes = sizeof(float) * static_cast<size_t>(ctas);
   config.stream = stream;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  ASG_CUDA(cudaLaunchKernelEx(&config, join_kernel, args, ctas, gt));
+  ASG_CUDA(cudaLaunchKernelEx(&config, join_kernel, args, ctas, gt, sliced));
   return ASG_OK;
 }
 

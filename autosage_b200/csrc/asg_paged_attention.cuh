@@ -2,9 +2,10 @@
 //
 // The work is a flat list of units: a unit is kUnit consecutive tokens of one item, an item is one row
 // (sequence) with the query heads of one group (up to GT heads that share a key head).  The list runs over
-// rows, inside a row over items, inside an item over tokens; CTA c of G takes the units [c S, (c + 1) S),
-// S = ceil(total / G), so every CTA streams the same number of cache bytes whatever the lengths are, one
-// long row fills the GPU, and an item is cut only where a CTA's share ends.  A piece that is a whole item
+// rows, inside a row over items, inside an item over tokens, and each item is preceded by kStart empty units
+// that stand for the cost of starting one (its query, its first pages, its result).  CTA c of G takes the
+// entries [c S, (c + 1) S), S = ceil(total / G), so every CTA does the same work whatever the lengths are,
+// one long row fills the GPU, and an item is cut only where a CTA's share ends.  A piece that is a whole item
 // is normalised and stored at once; the others leave (max, sum, accumulator) in the workspace, at most two
 // per CTA (the piece it begins with and the piece it ends with), and join_kernel puts them together in the
 // order of the tokens, so results do not depend on timing.  Nothing waits on another CTA.
@@ -26,6 +27,7 @@ namespace paged {
 constexpr int kWarps = 4;                  // warps of a CTA; each takes every fourth tile of a piece
 constexpr int kUnit = 64;                  // tokens per unit: one 16-token tile for each warp
 constexpr int kTile = kUnit / kWarps;
+constexpr int kStart = 2;                  // cost of starting an item, in units (where the GPU has more than a unit a CTA)
 constexpr int kMaxCtasPerSm = 4;           // bounds the workspace; no kernel is launched with more
 
 struct AttentionArgs {
@@ -84,53 +86,68 @@ __device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
 
 // Where a CTA's share begins.
 struct Share {
-  long long pos, end;   // in units, flat
-  long long row_begin;  // flat index of the row's first unit
+  long long pos, end;   // entries of the list, flat
+  long long row_begin;  // entry at which the row begins
   int row;
+  int start;            // empty units before each item
 };
 
-// Every thread sums the units of its rows, a block scan finds the row that holds the first unit.
+// Every thread sums the units of its rows, a block scan finds the row that holds the share's first entry.
 __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
-  __shared__ long long warp_total[kWarps];
+  __shared__ long long warp_units[kWarps], warp_rows[kWarps];
   __shared__ long long found_begin;
   __shared__ int found_row;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_thread = (a.n_rows + kWarps * 32 - 1) / (kWarps * 32);
   const long long r0 = static_cast<long long>(tid) * per_thread;
-  long long mine = 0;
-  for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) mine += row_span(a, static_cast<int>(r)).units();
-  long long scan = mine;
+  long long units = 0, rows = 0;
+  for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) {
+    const long long here = row_span(a, static_cast<int>(r)).units();
+    units += here;
+    rows += here > 0;
+  }
+  long long units_scan = units, rows_scan = rows;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long other = __shfl_up_sync(kFull, scan, o);
-    if (lane >= o) scan += other;
+    const long long u = __shfl_up_sync(kFull, units_scan, o), r = __shfl_up_sync(kFull, rows_scan, o);
+    if (lane >= o) {
+      units_scan += u;
+      rows_scan += r;
+    }
   }
-  if (lane == 31) warp_total[warp] = scan;
+  if (lane == 31) {
+    warp_units[warp] = units_scan;
+    warp_rows[warp] = rows_scan;
+  }
   if (tid == 0) found_row = -1;
   __syncthreads();
-  long long before = scan - mine, total = 0;
+  long long units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += warp_total[w];
-    total += warp_total[w];
+    if (w < warp) {
+      units_before += warp_units[w];
+      rows_before += warp_rows[w];
+    }
+    all_units += warp_units[w];
+    all_rows += warp_rows[w];
   }
-  total *= items_per_row;
-  const long long per_cta = quotient(total + gridDim.x - 1, gridDim.x);
   Share s;
+  s.start = all_units * items_per_row > gridDim.x ? kStart : 0;
+  const long long total = (all_units + s.start * all_rows) * items_per_row;
+  const long long per_cta = quotient(total + gridDim.x - 1, gridDim.x);
   s.pos = per_cta * blockIdx.x;
   s.end = s.pos + per_cta < total ? s.pos + per_cta : total;
-  if (s.pos < s.end) {
-    long long at = before * items_per_row;
-    if (s.pos >= at && s.pos < at + mine * items_per_row) {  // exactly one thread
-      long long r = r0;
-      for (; r + 1 < a.n_rows; ++r) {
-        const long long here = row_span(a, static_cast<int>(r)).units() * items_per_row;
-        if (s.pos < at + here) break;
-        at += here;
-      }
-      found_row = static_cast<int>(r);
-      found_begin = at;
+  long long at = (units_before + s.start * rows_before) * items_per_row;
+  if (s.pos < s.end && s.pos >= at && s.pos < at + (units + s.start * rows) * items_per_row) {  // exactly one thread
+    long long r = r0;
+    for (; r + 1 < a.n_rows; ++r) {
+      const long long n = row_span(a, static_cast<int>(r)).units();
+      const long long here = n > 0 ? (n + s.start) * items_per_row : 0;
+      if (s.pos < at + here) break;
+      at += here;
     }
+    found_row = static_cast<int>(r);
+    found_begin = at;
   }
   __syncthreads();
   s.row = found_row;
@@ -255,64 +272,104 @@ __device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a, int blo
   }
 }
 
+// One piece of a CTA's share.
+struct Piece {
+  RowSpan span;
+  int row, item, kv_head, sub;
+  long long units, u0, u1;  // of the item; the piece's
+  __device__ __forceinline__ long long first() const { return span.first + u0 * kUnit; }
+  __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + u1 * kUnit; }
+};
+
+// Walks through a share.
+struct Walk {
+  Share s;
+  RowSpan span;
+  long long units, at;  // of the row's items; entry inside the item
+  int item, items_per_row;
+  __device__ __forceinline__ Walk(const AttentionArgs& a, int items) : s(locate_share(a, items)), items_per_row(items) {
+    if (s.pos >= s.end) return;
+    span = row_span(a, s.row);
+    units = span.units();
+    item = static_cast<int>(quotient(s.pos - s.row_begin, units + s.start));
+    at = s.pos - s.row_begin - item * (units + s.start);
+  }
+  // The next piece that has tokens; all threads of the block get the same.
+  __device__ __forceinline__ bool next(const AttentionArgs& a, Piece& p) {
+    while (s.pos < s.end) {
+      const long long entries = units + s.start, left = s.end - s.pos;
+      const long long to = entries - at <= left ? entries : at + left;
+      p.span = span;
+      p.row = s.row;
+      p.item = item;
+      p.units = units;
+      p.u0 = at > s.start ? at - s.start : 0;
+      p.u1 = to > s.start ? to - s.start : 0;
+      s.pos += to - at;
+      at = 0;
+      if (s.pos < s.end && ++item == items_per_row) {
+        item = 0;
+        s.row = next_row(a, s.row);
+        if (s.row >= a.n_rows) s.pos = s.end;
+        else span = row_span(a, s.row);
+        units = span.units();
+      }
+      if (p.u0 < p.u1) {
+        p.kv_head = p.item / a.subgroups;
+        p.sub = p.item - p.kv_head * a.subgroups;
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
 // The kernel around an Engine, which computes one warp's part of a piece:
-//   Engine(smem)                                  once
-//   begin(a, row, first head, heads)              when the item changes
-//   run(a, span, kv_head, first, last)            the warp's tiles of tokens [first, last) of the row
-//   publish(smem, ml)                             its part into shared memory: float o[kHeads][kPitch] at
-//                                                 smem + warp * kWarpBytes (its own region, which run() may use too)
+//   Engine(smem)                      once
+//   start(a, piece)                   begins to fetch the piece's tokens; the part of the piece before is still unpublished
+//   query(a, piece)                   takes the query and clears the accumulators
+//   run(a)                            the warp's tiles
+//   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + warp * kWarpBytes +
+//                                     kPublish, which no copy of a started piece writes before run()
 // kWarpBytes * kWarps bytes of shared memory belong to the engine, the (m, l) pairs lie behind them.
 template <typename Engine>
 __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
   constexpr int GT = Engine::kHeads;
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_release_dependents();
-  const int items_per_row = a.n_kv_heads * a.subgroups;
-  Share s = locate_share(a, items_per_row);
-  int4 piece = make_int4(0, 0, 0, 0);
-  if (s.pos < s.end) {
+  Walk walk(a, a.n_kv_heads * a.subgroups);
+  int4 left_over = make_int4(0, 0, 0, 0);
+  Piece now;
+  if (walk.next(a, now)) {
     Engine engine(smem);
-    const float* o = reinterpret_cast<const float*>(smem);
+    const float* o = reinterpret_cast<const float*>(smem + Engine::kPublish);
     float2* ml = reinterpret_cast<float2*>(smem + kWarps * Engine::kWarpBytes);
-    RowSpan span = row_span(a, s.row);
-    long long units = span.units();
-    int item = static_cast<int>(quotient(s.pos - s.row_begin, units));
-    long long u0 = (s.pos - s.row_begin) - item * units;
-    for (;;) {
-      const long long left = s.end - s.pos;
-      const long long u1 = units - u0 <= left ? units : u0 + left;
-      const int kv_head = item / a.subgroups, sub = item - kv_head * a.subgroups;
-      engine.begin(a, s.row, kv_head * a.group + sub * GT, min(GT, a.group - sub * GT));
-      const long long first = span.first + u0 * kUnit;
-      const long long last = u1 == units ? span.last : span.first + u1 * kUnit;
-      engine.run(a, span, kv_head, first, last);
+    engine.start(a, now);
+    engine.query(a, now);
+    for (bool more = true; more;) {
+      engine.run(a);
+      Piece next;
+      more = walk.next(a, next);
+      if (more) engine.start(a, next);
       engine.publish(smem, ml);
+      if (more) engine.query(a, next);
       __syncthreads();
       int slot = -1;  // a whole item
-      if (u0 > 0) {
+      if (now.u0 > 0) {
         slot = 0;
-        piece.w = u1 == units ? 1 : 2;
-      } else if (u1 < units) {
+        left_over.w = now.u1 == now.units ? 1 : 2;
+      } else if (now.u1 < now.units) {
         slot = 1;
-        piece.x = s.row;
-        piece.y = item;
-        piece.z = 1;
+        left_over.x = now.row;
+        left_over.y = now.item;
+        left_over.z = 1;
       }
-      store_piece<GT, Engine::kDim, Engine::kPitch>(a, s.row, kv_head, sub, slot, o, Engine::kWarpBytes / 4, ml);
+      store_piece<GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o, Engine::kWarpBytes / 4, ml);
       __syncthreads();  // the buffers are free again
-      s.pos += u1 - u0;
-      if (s.pos >= s.end) break;
-      u0 = 0;
-      if (++item == items_per_row) {
-        item = 0;
-        s.row = next_row(a, s.row);
-        if (s.row >= a.n_rows) break;
-        span = row_span(a, s.row);
-        units = span.units();
-      }
+      now = next;
     }
   }
-  if (threadIdx.x == 0) a.pieces[blockIdx.x] = piece;
+  if (threadIdx.x == 0) a.pieces[blockIdx.x] = left_over;
   if (gridDim.x == 1) clear_empty_rows(a, 0, 1);  // otherwise the join kernel does, while this one runs
 }
 
@@ -320,7 +377,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
 template <typename Engine>
 int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
   constexpr int smem = kWarps * (Engine::kWarpBytes + Engine::kHeads * static_cast<int>(sizeof(float2)));
-  static_assert(Engine::kWarpBytes >= Engine::kHeads * Engine::kPitch * 4 && Engine::kWarpBytes % 128 == 0, "warp region");
+  static_assert(Engine::kWarpBytes >= Engine::kPublish + Engine::kHeads * Engine::kPitch * 4 && Engine::kWarpBytes % 128 == 0, "warp region");
   static_assert(Engine::kCtasPerSm <= kMaxCtasPerSm && Engine::kCtasPerSm * (smem + 1024) <= 228 * 1024, "shared memory");
   auto kernel = attention_kernel<Engine>;
   if (smem > 48 * 1024)

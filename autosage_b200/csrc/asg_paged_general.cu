@@ -20,6 +20,7 @@ struct General {
   static constexpr int N = TB * GT;                          // scores per batch: 4 ... 32
   static constexpr int kShift = N == 32 ? 0 : N == 16 ? 1 : N == 8 ? 2 : 3;
   static constexpr int kWarpBytes = GT * kPitch * 4;
+  static constexpr int kPublish = 0;
   static_assert(N == 32 || N == 16 || N == 8 || N == 4, "reduce-scatter sizes");
 
   float q[GT][E], o[GT][E];
@@ -30,14 +31,30 @@ struct General {
 
   static __device__ __forceinline__ int feature(int lane, int e) { return VEC ? lane * E + e : e * 32 + lane; }
 
-  __device__ __forceinline__ void begin(const AttentionArgs& a, int row, int head, int heads) {
+  const T* keys;
+  const T* values;
+  const int64_t* ids;  // of the page that holds the piece's first token
+  int kv_head, place0, count;
+
+  __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
+    kv_head = p.kv_head;
+    keys = static_cast<const T*>(a.key.data) + kv_head * a.key.head_stride;
+    values = static_cast<const T*>(a.value.data) + kv_head * a.value.head_stride;
+    const long long first = p.first(), page0 = quotient(first, a.page_size);  // page arithmetic in 32 bits from here on
+    place0 = static_cast<int>(first - page0 * a.page_size);
+    ids = a.col + p.span.pages_begin + page0;
+    count = static_cast<int>(p.last() - first);
+  }
+
+  __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
+    const int head = p.kv_head * a.group + p.sub * GT, heads = min(GT, a.group - p.sub * GT);
 #pragma unroll
     for (int g = 0; g < GT; ++g)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int d = feature(lane, e);
         q[g][e] = g < heads && d < a.dim
-                      ? load_wide(a.q, row * a.q_token_stride + (head + g) * a.q_head_stride + d, a.type) * a.scale_log2
+                      ? load_wide(a.q, p.row * a.q_token_stride + (head + g) * a.q_head_stride + d, a.type) * a.scale_log2
                       : 0.f;
         o[g][e] = 0.f;
       }
@@ -62,14 +79,7 @@ struct General {
     }
   }
 
-  __device__ __forceinline__ void run(const AttentionArgs& a, const RowSpan& span, int kv_head, long long first, long long last) {
-    const T* keys = static_cast<const T*>(a.key.data) + kv_head * a.key.head_stride;
-    const T* values = static_cast<const T*>(a.value.data) + kv_head * a.value.head_stride;
-    // page arithmetic in 32 bits, from the page that holds the piece's first token
-    const long long page0 = quotient(first, a.page_size);
-    const int place0 = static_cast<int>(first - page0 * a.page_size);
-    const long long pages = span.pages_begin + page0;
-    const int count = static_cast<int>(last - first);
+  __device__ __forceinline__ void run(const AttentionArgs& a) {
     for (int tile = warp * kTile; tile < count; tile += kUnit) {
       // lane t < kTile finds token tile + t
       int page = -1, place = 0;
@@ -77,7 +87,7 @@ struct General {
       if (lane < kTile && tile + lane < count) {
         const unsigned at = static_cast<unsigned>(place0) + static_cast<unsigned>(tile + lane);
         const unsigned nth = at / static_cast<unsigned>(a.page_size);
-        const long long id = a.col[pages + nth];
+        const long long id = ids[nth];
         place = static_cast<int>(at - nth * static_cast<unsigned>(a.page_size));
         if (id >= 0 && id < a.n_pages) page = static_cast<int>(id);
         if (TypeOf<T>::coded && page >= 0) {

@@ -133,7 +133,8 @@ struct Tensor {
   static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * kTile * 4 : 0) + 4 + 15) / 16 * 16;
   static constexpr int kDim = DP;
   static constexpr int kPitch = DP + 4;                             // of the published accumulators: no bank conflicts
-  static constexpr int kNeed = kStages * kStageBytes > kHeads * kPitch * 4 ? kStages * kStageBytes : kHeads * kPitch * 4;
+  static constexpr int kPublish = (kStages - 1) * kStageBytes;      // the next piece's first copies go to the stages before it
+  static constexpr int kNeed = kPublish + (kStageBytes > kHeads * kPitch * 4 ? kStageBytes : kHeads * kPitch * 4);
   static constexpr int kWarpBytes = (kNeed + 127) / 128 * 128;
   static constexpr int kSteps = DP / 16;
   using H = typename std::conditional<kCoded, F16, T>::type;        // type of the products
@@ -181,12 +182,12 @@ struct Tensor {
     return bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair)) : __half22float2(*reinterpret_cast<const __half2*>(&pair));
   }
 
-  __device__ __forceinline__ void begin(const AttentionArgs& a, int row, int head, int heads) {
-    dim_bytes = a.dim * static_cast<int>(sizeof(T));
+  __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
+    const int head = p.kv_head * a.group + p.sub * kHeads, heads = min(kHeads, a.group - p.sub * kHeads);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = 8 * nt + (lane >> 2);
-      const uint16_t* from = static_cast<const uint16_t*>(a.q) + row * a.q_token_stride + (head + h) * a.q_head_stride;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) + p.row * a.q_token_stride + (head + h) * a.q_head_stride;
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         const uint2 x = load_query(a, from, h < heads, step, lane);
@@ -229,16 +230,6 @@ struct Tensor {
       m[nt][0] = m[nt][1] = -CUDART_INF_F;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    if (dim_bytes < kRowBytes) {  // features past the head's end are never copied: they are zeros
-      const int first = dim_bytes / 16, missing = kChunks - first;
-      for (int i = lane; i < kStages * 2 * kTile * missing; i += 32) {
-        const int r = i / missing, chunk = first + i - r * missing;
-        const int stage = r / (2 * kTile), line = r - stage * 2 * kTile;
-        const uint32_t at = ring + stage * kStageBytes + line * kRowPitch + chunk * 16;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-      }
-      __syncwarp();
-    }
   }
 
   // Where the copies of a piece come from, and how far they are.  Lane l looks after token l % 16 of the next tile:
@@ -253,10 +244,11 @@ struct Tensor {
     int step_pages, step_place;  // kUnit tokens on
     long long id;
   };
-  __device__ __forceinline__ void look_up(Source& s) const {
+  Source s;
+  __device__ __forceinline__ void look_up() {
     s.id = s.tile + (lane & (kTile - 1)) < s.count ? s.ids[s.nth] : -1;
   }
-  __device__ __forceinline__ void issue(const AttentionArgs& a, Source& s, int stage) const {
+  __device__ __forceinline__ void issue(const AttentionArgs& a, int stage) {
     if (s.tile < s.count) {
       const bool held = s.id >= 0 && s.id < a.n_pages;
       const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
@@ -274,10 +266,9 @@ struct Tensor {
         const int high = __shfl_sync(kFull, offset_high, line);
         const long long from = (static_cast<long long>(high) << 32 | low) + chunk;
         const bool ok = (seen >> line & 1u) != 0;
-        if (inside) {
-          copy_async16(to + n * kLines * kRowPitch, s.keys + from, ok);
-          copy_async16(to + n * kLines * kRowPitch + kValues, s.values + from, ok);
-        }
+        // zeros for a token that is not seen and for features past the head's end
+        copy_async16(to + n * kLines * kRowPitch, s.keys + from, ok && inside);
+        copy_async16(to + n * kLines * kRowPitch + kValues, s.values + from, ok && inside);
       }
       if constexpr (kCoded) {
         const asg_page_pool& pool = lane < kTile ? a.key : a.value;
@@ -296,11 +287,14 @@ struct Tensor {
       s.place -= a.page_size;
       ++s.nth;
     }
-    look_up(s);
+    look_up();
   }
 
-  __device__ __forceinline__ void run(const AttentionArgs& a, const RowSpan& span, int kv_head, long long first, long long last) {
-    Source s;
+  __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
+    __syncwarp();  // all lanes have left the stages
+    dim_bytes = a.dim * static_cast<int>(sizeof(T));
+    const int kv_head = p.kv_head;
+    const long long first = p.first(), last = p.last();
     s.keys = static_cast<const char*>(a.key.data) + kv_head * a.key.head_stride * static_cast<int>(sizeof(T));
     s.values = static_cast<const char*>(a.value.data) + kv_head * a.value.head_stride * static_cast<int>(sizeof(T));
     s.page_bytes = a.key.page_stride * static_cast<int>(sizeof(T));
@@ -308,7 +302,7 @@ struct Tensor {
     s.kv_head = kv_head;
     const unsigned page_size = static_cast<unsigned>(a.page_size);
     const long long page0 = quotient(first, a.page_size);  // page arithmetic in 32 bits from here on
-    s.ids = a.col + span.pages_begin + page0;
+    s.ids = a.col + p.span.pages_begin + page0;
     s.count = static_cast<int>(last - first);
     s.tile = warp * kTile;
     const unsigned at = static_cast<unsigned>(first - page0 * a.page_size) + s.tile + (lane & (kTile - 1));
@@ -316,14 +310,18 @@ struct Tensor {
     s.place = static_cast<int>(at % page_size);
     s.step_pages = static_cast<int>(kUnit / page_size);
     s.step_place = static_cast<int>(kUnit % page_size);
-    look_up(s);
+    look_up();
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(a, s, i);
+    for (int i = 0; i < kStages - 1; ++i) issue(a, i);
+  }
+
+  __device__ __forceinline__ void run(const AttentionArgs& a) {
+    const int tiles = s.count <= warp * kTile ? 0 : (s.count - warp * kTile + kUnit - 1) / kUnit;
     int stage = 0, fill = kStages - 1;
-    for (int now = warp * kTile; now < s.count; now += kUnit) {
+    for (int i = 0; i < tiles; ++i) {
       copy_wait<kStages - 2>();
       __syncwarp();  // the tile has arrived for all lanes, and all have left the stage that is filled next
-      issue(a, s, fill);
+      issue(a, fill);
       compute(a, ring + stage * kStageBytes);
       stage = stage + 1 == kStages ? 0 : stage + 1;
       fill = fill + 1 == kStages ? 0 : fill + 1;
@@ -343,18 +341,18 @@ struct Tensor {
 
   __device__ __forceinline__ void compute(const AttentionArgs& a, uint32_t base) {
     const uint32_t line16 = base + (lane & 15) * kRowPitch + (lane >> 4) * 16;
-    float s[NT][4];
+    float dots[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+      for (int i = 0; i < 4; ++i) dots[nt][i] = 0.f;
     if constexpr (!kCoded) {
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         uint32_t k[4];
         ldmatrix_x4(k, line16 + step * 32);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<H>(s[nt], k, q[nt][step][0], q[nt][step][1]);
+        for (int nt = 0; nt < NT; ++nt) mma16816<H>(dots[nt], k, q[nt][step][0], q[nt][step][1]);
       }
     } else {
 #pragma unroll
@@ -366,7 +364,7 @@ struct Tensor {
           const uint32_t k[4] = {decode_pair<0, 1>(c[2 * i], T{}), decode_pair<0, 1>(c[2 * i + 1], T{}),
                                  decode_pair<2, 3>(c[2 * i], T{}), decode_pair<2, 3>(c[2 * i + 1], T{})};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<H>(s[nt], k, q[nt][step + i][0], q[nt][step + i][1]);
+          for (int nt = 0; nt < NT; ++nt) mma16816<H>(dots[nt], k, q[nt][step + i][0], q[nt][step + i][1]);
         }
       }
     }
@@ -398,8 +396,8 @@ struct Tensor {
         float x[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if constexpr (kCoded) x[t] = in[t] ? s[nt][2 * t + h] * (key_scale[t] * unit[nt][h]) : -CUDART_INF_F;
-          else x[t] = in[t] ? s[nt][2 * t + h] * a.scale_log2 : -CUDART_INF_F;
+          if constexpr (kCoded) x[t] = in[t] ? dots[nt][2 * t + h] * (key_scale[t] * unit[nt][h]) : -CUDART_INF_F;
+          else x[t] = in[t] ? dots[nt][2 * t + h] * a.scale_log2 : -CUDART_INF_F;
         }
         const float top = largest_of_tile(x[0], x[1], m[nt][h]);
         const float at = top == -CUDART_INF_F ? 0.f : top;
@@ -472,7 +470,7 @@ struct Tensor {
   }
 
   __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
-    float* to = reinterpret_cast<float*>(smem + warp * kWarpBytes);
+    float* to = reinterpret_cast<float*>(smem + warp * kWarpBytes + kPublish);
     constexpr float undo = kLift == 0.f ? 1.f : 1.f / 16384.f;
     static_assert(kLift == 0.f || kLift == 14.f, "2^-kLift");
 #pragma unroll
@@ -504,7 +502,7 @@ inline Choice choose_padded(const AttentionArgs& a) {
   if constexpr (sizeof(T) == 1) {
     if (a.dim <= 64) return made<Tensor<T, 64, NT, 4, 4>>();
     if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 3>>();
-    return made<Tensor<T, 256, NT, 3, 2>>();
+    return made<Tensor<T, 256, NT, NT == 1 ? 3 : 2, 2>>();
   } else {
     if (a.dim <= 64) return made<Tensor<T, 64, NT, 3, 3>>();
     if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 2>>();
