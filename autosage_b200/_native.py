@@ -34,6 +34,22 @@ _U32 = ctypes.c_uint
 _SZ = ctypes.c_size_t
 _F32 = ctypes.c_float
 
+class PagePool(ctypes.Structure):
+    """``asg_page_pool`` of the header."""
+
+    _fields_ = [("data", _P), ("scales", _P), ("page_stride", _I64), ("token_stride", _I64), ("head_stride", _I64),
+                ("scale_page_stride", _I64), ("scale_head_stride", _I64), ("scale_token_stride", _I64)]
+
+
+class TokenRows(ctypes.Structure):
+    """``asg_token_rows`` of the header."""
+
+    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+_ROWS = ctypes.POINTER(TokenRows)
+_POOL = ctypes.POINTER(PagePool)
+
 # name -> (restype, argtypes); kept in the order of the header
 SIGNATURES = {
     "asg_version": (_INT, []),
@@ -71,25 +87,12 @@ SIGNATURES = {
     "asg_spmm_csr_split_noalloc": (_INT, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _I64, _P]),
     "asg_static_max_rows": (_I64, []),
     "asg_static_status": (_INT, [_P, _P, _P]),
-    "asg_paged_cache_write": (_INT, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
-    "asg_paged_cache_read": (_INT, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
+    "asg_paged_cache_write": (_INT, [_P, _I64, _ROWS, _ROWS, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
+    "asg_paged_cache_read": (_INT, [_P, _I64, _ROWS, _ROWS, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
     "asg_paged_attention_workspace_bytes": (_SZ, [_INT, _INT, _INT]),
-    "asg_paged_attention": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _INT, _INT, _INT, _F32, _I64,
+    "asg_paged_attention": (_INT, [_P, _P, _P, _I64, _I64, _ROWS, _P, _P, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _F32, _I64,
                                    _INT, _INT, _P, _SZ, _P]),
 }
-
-
-class PagePool(ctypes.Structure):
-    """``asg_page_pool`` of the header."""
-
-    _fields_ = [("data", _P), ("scales", _P), ("page_stride", _I64), ("token_stride", _I64), ("head_stride", _I64),
-                ("scale_page_stride", _I64), ("scale_head_stride", _I64), ("scale_token_stride", _I64)]
-
-
-class TokenRows(ctypes.Structure):
-    """``asg_token_rows`` of the header."""
-
-    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
 
 
 # ASG_TYPE_* of the header
@@ -177,12 +180,16 @@ def _capturing() -> bool:
 
 
 def scratch(device: torch.device, n_rows: int, extra_bytes: int = 0) -> torch.Tensor:
-    need = workspace_bytes(n_rows) + int(extra_bytes)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return _scratch_on(device, index, _stream(device), workspace_bytes(n_rows) + int(extra_bytes))
+
+
+def _scratch_on(device: torch.device, index: int, stream: int, need: int) -> torch.Tensor:
     if _capturing():
         # a captured launch keeps the raw pointer: the buffer has to come from the graph's own pool
         # (and so live as long as the graph), not from a cache that may replace it later
         return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
-    key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device))
+    key = (index, stream)
     buffer = _SCRATCH.get(key)
     if buffer is None or buffer.numel() < need:
         buffer = torch.empty(max(need, 1 << 16), dtype=torch.uint8, device=device)
@@ -455,31 +462,41 @@ def conv_fused(crow: torch.Tensor, col: torch.Tensor, val: Optional[torch.Tensor
 def _page_pool(pages: torch.Tensor, scales: Optional[torch.Tensor]) -> PagePool:
     page, token, head, _ = pages.stride()
     if scales is None:
-        return PagePool(pages.data_ptr(), None, page, token, head, 0, 0, 0)
+        return PagePool(pages.data_ptr(), None, page, token, head)
     return PagePool(pages.data_ptr(), scales.data_ptr(), page, token, head, *scales.stride())
 
 
 def _token_rows(rows: torch.Tensor) -> TokenRows:
-    return TokenRows(rows.data_ptr(), rows.stride(0), rows.stride(1))
+    token, head, _ = rows.stride()
+    return TokenRows(rows.data_ptr(), token, head)
 
 
-def _paged_cache(entry: str, slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
-    k, v = _token_rows(key), _token_rows(value)
-    kp, vp = _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales)
-    check(getattr(library(), entry)(slots.data_ptr(), slots.numel(), ctypes.byref(k), ctypes.byref(v), ctypes.byref(kp),
-                                    ctypes.byref(vp), key_pages.size(0), key_pages.size(1), key_pages.size(2),
-                                    key_pages.size(3), TYPES[key.dtype], TYPES[key_pages.dtype],
-                                    _stream(key_pages.device)))
+# One token is little work for the GPU, so the calls of the paged cache are made of little else than the call:
+# the stream's handle as torch's own extensions take it, no keyword arguments, no copies of what is at hand.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def paged_cache_write(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
     """Rows [T, heads, dim] into the slots of the pages, quantised where the pages are 8-bit."""
-    _paged_cache("asg_paged_cache_write", slots, key, value, key_pages, value_pages, key_scales, value_scales)
+    n_pages, page_size, heads, dim = key_pages.shape
+    code = library().asg_paged_cache_write(
+        slots.data_ptr(), slots.numel(), _token_rows(key), _token_rows(value), _page_pool(key_pages, key_scales),
+        _page_pool(value_pages, value_scales), n_pages, page_size, heads, dim, TYPES[key.dtype], TYPES[key_pages.dtype],
+        _raw_stream(key_pages.device.index))
+    if code:
+        check(code)
 
 
 def paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
     """The slots of the pages into the rows key and value."""
-    _paged_cache("asg_paged_cache_read", slots, key, value, key_pages, value_pages, key_scales, value_scales)
+    n_pages, page_size, heads, dim = key_pages.shape
+    code = library().asg_paged_cache_read(
+        slots.data_ptr(), slots.numel(), _token_rows(key), _token_rows(value), _page_pool(key_pages, key_scales),
+        _page_pool(value_pages, value_scales), n_pages, page_size, heads, dim, TYPES[key.dtype], TYPES[key_pages.dtype],
+        _raw_stream(key_pages.device.index))
+    if code:
+        check(code)
 
 
 @functools.lru_cache(maxsize=None)
@@ -487,19 +504,22 @@ def _paged_attention_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     return int(library().asg_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim))
 
 
-def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages, key_scales, value_scales, *,
-                    scale: float, window: int) -> None:
+def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages, key_scales, value_scales, scale: float,
+                    window: int) -> None:
     """out[r] = softmax(scale q_r K^T) V over the tokens of row r's pages (one query token a row)."""
     n_rows, n_heads, head_dim = query.shape
     n_pages, page_size, n_kv_heads, _ = key_pages.shape
-    workspace = scratch(query.device, 0, _paged_attention_bytes(n_heads, n_kv_heads, head_dim))
-    q = _token_rows(query)
-    kp, vp = _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales)
-    check(library().asg_paged_attention(crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(),
-                                        ctypes.byref(q), out.data_ptr(), _ptr(lse), ctypes.byref(kp), ctypes.byref(vp),
-                                        n_pages, page_size, n_heads, n_kv_heads, head_dim, scale, window,
-                                        TYPES[query.dtype], TYPES[key_pages.dtype], workspace.data_ptr(),
-                                        workspace.numel(), _stream(query.device)))
+    device = query.device
+    stream = _raw_stream(device.index)
+    need = _paged_attention_bytes(n_heads, n_kv_heads, head_dim)
+    workspace = _scratch_on(device, device.index, stream, need)
+    code = library().asg_paged_attention(
+        crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), _token_rows(query), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales),
+        n_pages, page_size, n_heads, n_kv_heads, head_dim, scale, window, TYPES[query.dtype], TYPES[key_pages.dtype],
+        workspace.data_ptr(), workspace.numel(), stream)
+    if code:
+        check(code)
 
 
 def push_to_peers(src: torch.Tensor, destinations: list[torch.Tensor], n_ctas: int = 32) -> None:

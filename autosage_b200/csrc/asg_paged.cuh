@@ -77,25 +77,47 @@ template <> __device__ __forceinline__ F32 from_float<F32>(float v) { return v; 
 template <> __device__ __forceinline__ BF16 from_float<BF16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ F16 from_float<F16>(float v) { return __float2half_rn(v); }
 
-// N consecutive elements, moved in vectors of up to 16 bytes (the address is a multiple of that).
+// N consecutive elements, moved in vectors of up to 32 bytes (the address is a multiple of their size).
 template <typename T, int N>
 struct Pack {
   static constexpr int kBytes = N * static_cast<int>(sizeof(T));
-  static constexpr int kVec = kBytes < 16 ? kBytes : 16;
+  static constexpr int kVec = kBytes < 32 ? kBytes : 32;
   alignas(kVec) T v[N];
-  __device__ __forceinline__ void load(const T* p) { move(v, p); }
-  __device__ __forceinline__ void store(T* p) const { move(p, v); }
-  static __device__ __forceinline__ void move(T* to, const T* from) {
-    if constexpr (kVec == 16) {
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kVec == 32) {
+      uint32_t* r = reinterpret_cast<uint32_t*>(v);
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
-    } else if constexpr (kVec == 8) {
-      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
-    } else if constexpr (kVec == 4) {
-      *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+      for (int i = 0; i < kBytes / 32; ++i)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[8 * i]), "=r"(r[8 * i + 1]), "=r"(r[8 * i + 2]), "=r"(r[8 * i + 3]), "=r"(r[8 * i + 4]),
+                       "=r"(r[8 * i + 5]), "=r"(r[8 * i + 6]), "=r"(r[8 * i + 7])
+                     : "l"(reinterpret_cast<const uint32_t*>(p) + 8 * i)
+                     : "memory");
     } else {
-      static_assert(kVec == 2, "no such vector");
-      *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+      move(v, p);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kVec == 32) {
+      const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+      for (int i = 0; i < kBytes / 32; ++i)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + 8 * i),
+                     "r"(r[8 * i]), "r"(r[8 * i + 1]), "r"(r[8 * i + 2]), "r"(r[8 * i + 3]), "r"(r[8 * i + 4]),
+                     "r"(r[8 * i + 5]), "r"(r[8 * i + 6]), "r"(r[8 * i + 7])
+                     : "memory");
+    } else {
+      move(p, v);
+    }
+  }
+  static __device__ __forceinline__ void move(T* to, const T* from) {
+    if constexpr (kVec == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+    else if constexpr (kVec == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
+    else if constexpr (kVec == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+    else if constexpr (kVec == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+    else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) to[i] = from[i];
     }
   }
 };

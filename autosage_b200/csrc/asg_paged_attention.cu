@@ -177,9 +177,10 @@ int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* 
   a.stats = reinterpret_cast<float2*>(at);
   at += align256(records * sizeof(float2));
   a.partial = reinterpret_cast<float*>(at);
+  // an item of at most one unit is never cut, and no row has more tokens than all pages of the table
+  a.join = ctas > 1 && n_cols * page_size > kUnit;
   if (int rc = choice.launch(a, ctas, stream)) return rc;
-  if (ctas == 1) return ASG_OK;  // nothing is shared
-  return launch_join(a, ctas, choice.gt, items * n_rows, stream);
+  return !a.join ? ASG_OK : launch_join(a, ctas, choice.gt, items * n_rows, stream);
 }
 
 }  // extern "C"

@@ -19,6 +19,8 @@
 
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "asg_paged.cuh"
 
 namespace asg {
@@ -46,6 +48,7 @@ struct AttentionArgs {
   int type;         // of q and out
   float scale_log2; // scale * log2(e)
   bool q_pairs;     // the query's rows start on 8 bytes
+  bool join;        // the join kernel follows
   bool out_vector;  // four neighbours of out can be stored at once
   int partial_pitch;
   float* partial;   // [G][2][GT][partial_pitch] accumulators of unfinished pieces
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
     }
   }
   if (threadIdx.x == 0) a.pieces[blockIdx.x] = left_over;
-  if (gridDim.x == 1) clear_empty_rows(a, 0, 1);  // otherwise the join kernel does, while this one runs
+  if (!a.join) clear_empty_rows(a, blockIdx.x, gridDim.x);  // otherwise the join kernel does, while this one runs
 }
 
 // Host: launch of one instance.
@@ -380,8 +383,16 @@ int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
   static_assert(Engine::kWarpBytes >= Engine::kPublish + Engine::kHeads * Engine::kPitch * 4 && Engine::kWarpBytes % 128 == 0, "warp region");
   static_assert(Engine::kCtasPerSm <= kMaxCtasPerSm && Engine::kCtasPerSm * (smem + 1024) <= 228 * 1024, "shared memory");
   auto kernel = attention_kernel<Engine>;
-  if (smem > 48 * 1024)
-    ASG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 48 * 1024) {  // once per device
+    static std::atomic<unsigned long long> known{0};
+    int device = 0;
+    ASG_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if ((known.load(std::memory_order_relaxed) & bit) == 0) {
+      ASG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
   kernel<<<ctas, kWarps * 32, smem, stream>>>(args);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;

@@ -5,16 +5,21 @@
 //   read    x[t, h, d] = round(code_d * s)
 //
 // Both move every byte once and are bound by memory: a group of lanes owns the key row AND the value row
-// of one (token, head), eight features a lane in 16-byte vectors, so two independent rows are in flight
-// per lane and consecutive groups touch consecutive heads of a token (contiguous in the usual layouts).
+// of one (token, head), 32 bytes of the wide type a lane where the rows allow it, so two independent rows are in
+// flight per lane and consecutive groups touch consecutive heads of a token (contiguous in the usual layouts).
 //
-// Rounding.  A quotient rounded to float32 first would often land exactly between two codes that the true
-// quotient is not between (16-bit inputs share few mantissa bits, so near-ties are common), and the tie
-// rule would then pick the wrong one.  The quotient is therefore rounded "to odd": correctly rounded by
-// one multiply with 1/s and two fused multiply-adds, then its last bit is set towards the sign of the exact
-// remainder x - q s.  Borders between codes have an even last bit, so rounding that value to a code gives
-// the code nearest to the true quotient, for about nine instructions a value; dividing in float64 instead
-// is kept for scales so small or large that 1/s or the remainder would leave float32's range.
+// Rounding.  The quotient x / s is not rounded before the code is chosen: rounded to float32 it would often
+// land exactly between two codes that the true quotient is not between, and the tie rule would then pick the wrong one.
+//   16-bit x.  With t = max|x| the quotient is x Q / t times t / (Q s), which is 1 + e, |e| <= 2^-24, the same for
+//     the whole row.  x Q / t is a quotient of short numbers: unless it lies ON a border b between codes it is
+//     further than 2^-19 b away from it (x Q and b t are integers below 2^19 times a power of two).  So one
+//     product x w with w = (1 / s) (1 + 2^-21 sign(e)) decides every code: its own error, below 2^-22, moves
+//     nothing across a border, and what lies on a border goes where e sends it.  For e = 0 the quotient is
+//     corrected by its remainder instead, which gives a quotient on a border exactly, and the tie rule holds.
+//   float32 x.  The quotient is rounded "to odd": correctly rounded by one multiply with 1/s and two fused
+//     multiply-adds, then its last bit is set towards the sign of the exact remainder x - q s.  Borders have
+//     an even last bit, so rounding that value to a code gives the code nearest to the true quotient.
+//   Scales so small or large that 1/s or a remainder would leave float32's range: division in float64.
 #include "asg_paged.cuh"
 
 namespace asg {
@@ -29,12 +34,11 @@ struct CacheArgs {
 };
 
 constexpr int kThreads = 256;
-constexpr int kPerLane = 8;  // features of a lane: 32 lanes cover kMaxDim
 
 __device__ __forceinline__ float largest_code(E4M3) { return 448.f; }
 __device__ __forceinline__ float largest_code(INT8) { return 127.f; }
 
-// x / s, rounded to odd in float32 (see above); inv = 1 / s, s in [2^-90, 2^90].
+// x / s, rounded to odd in float32; inv = 1 / s, s in [2^-90, 2^90].
 __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
   const float q0 = x * inv;
   const float q = fmaf(fmaf(-q0, s, x), inv, q0);
@@ -43,105 +47,157 @@ __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
   const int step = ((__float_as_int(rest) ^ bits) < 0) ? -1 : 1;  // towards the remainder
   return __int_as_float(rest != 0.f && (bits & 1) == 0 ? bits + step : bits);
 }
-
-__device__ __forceinline__ E4M3 nearest_code(float q, E4M3) {
-  E4M3 c;
-  c.code = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-  return c;
+// The same by way of float64: a quotient of two 24-bit numbers is never nearer to a border between codes than
+// 2^-40 of itself without lying on it, so 53 bits decide; they are rounded to odd too.
+__device__ __noinline__ float quotient_by_double(float x, float s) {
+  const double wide = s == 0.f ? 0.0 : static_cast<double>(x) / static_cast<double>(s);
+  const float q = static_cast<float>(wide);
+  const double rest = wide - static_cast<double>(q);
+  const int bits = __float_as_int(q);
+  if (!(fabs(rest) > 0.0) || (bits & 1) != 0 || q == 0.f || isinf(q)) return q;
+  return __int_as_float(bits + ((rest < 0.0) == (q < 0.f) ? 1 : -1));
 }
-__device__ __forceinline__ INT8 nearest_code(float q, INT8) {
-  INT8 c;
-  c.code = static_cast<int8_t>(max(-127, min(127, __float2int_rn(q))));
-  return c;
+
+// Two quotients to their nearest codes (ties to even, cut to the largest), first in the low byte.
+__device__ __forceinline__ uint32_t nearest_codes(float a, float b, E4M3) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t nearest_codes(float a, float b, INT8) {
+  const int x = max(-127, min(127, __float2int_rn(a))), y = max(-127, min(127, __float2int_rn(b)));
+  return (x & 0xff) | (y & 0xff) << 8;
 }
 
-// Feature of entry i of a lane: eight neighbours (VEC), or one in 32 (any alignment, any head size).
-template <bool VEC>
-__device__ __forceinline__ int feature(int lane, int i) { return VEC ? lane * kPerLane + i : i * 32 + lane; }
+// P features a lane, next to one another (whole rows of such packs, aligned); P = 0: eight, one in 32 each, for any
+// alignment and head size.
+constexpr int lane_features(int p) { return p == 0 ? 8 : p; }
+template <int P>
+__device__ __forceinline__ int feature(int lane, int i) { return P == 0 ? i * 32 + lane : lane * P + i; }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void load_row(Pack<T, kPerLane>& x, const T* row, int lane, int dim) {
-  if constexpr (VEC) {
-    if (lane * kPerLane < dim) {
-      x.load(row + lane * kPerLane);
+template <int P, typename T>
+__device__ __forceinline__ void load_row(Pack<T, lane_features(P)>& x, const T* row, int lane, int dim) {
+  if constexpr (P > 0) {
+    if (lane * P < dim) {
+      x.load(row + lane * P);
       return;
     }
   }
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int d = feature<VEC>(lane, i);
+  for (int i = 0; i < lane_features(P); ++i) {
     x.v[i] = T{};
-    if (!VEC && d < dim) x.v[i] = row[d];
+    if (P == 0 && feature<P>(lane, i) < dim) x.v[i] = row[feature<P>(lane, i)];
   }
 }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void store_row(const Pack<T, kPerLane>& x, T* row, int lane, int dim) {
-  if constexpr (VEC) {
-    if (lane * kPerLane < dim) x.store(row + lane * kPerLane);
+template <int P, typename T>
+__device__ __forceinline__ void store_row(const Pack<T, lane_features(P)>& x, T* row, int lane, int dim) {
+  if constexpr (P > 0) {
+    if (lane * P < dim) x.store(row + lane * P);
   } else {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (feature<VEC>(lane, i) < dim) row[feature<VEC>(lane, i)] = x.v[i];
+    for (int i = 0; i < lane_features(P); ++i)
+      if (feature<P>(lane, i) < dim) row[feature<P>(lane, i)] = x.v[i];
   }
 }
 
-template <typename IN, typename CACHE, bool VEC>
+// The largest magnitude of a row, by its bits: a NaN is above everything and is not lost.
+template <typename IN, int N>
+__device__ __forceinline__ float largest_of_row(const Pack<IN, N>& x, int group, unsigned mask) {
+  if constexpr (sizeof(IN) == 2) {
+    const uint32_t* two = reinterpret_cast<const uint32_t*>(x.v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) top = __vmaxu2(top, two[i] & 0x7fff7fffu);
+    for (int o = group >> 1; o >= 1; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(mask, top, o));
+    const uint16_t one = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    return to_float(*reinterpret_cast<const IN*>(&one));
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x.v[i]) & 0x7fffffffu);
+    for (int o = group >> 1; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+    return __uint_as_float(top);
+  }
+}
+
+template <typename IN, typename CACHE, int N>
+__device__ __forceinline__ float quantise(const Pack<IN, N>& x, Pack<CACHE, N>& c, int group, unsigned mask) {
+  const float top = largest_of_row(x, group, mask), most = largest_code(CACHE{});
+  const float s = top / most;
+  uint32_t codes[N / 2];
+  if (s > 0x1p-90f && s < 0x1p90f) {
+    if constexpr (sizeof(IN) == 2) {
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within one unit in the last place
+      const float off = fmaf(-s, most, top);                   // exact; its sign is that of e
+      if (off != 0.f) {
+        const float w = inv * (off > 0.f ? 1.f + 0x1p-21f : 1.f - 0x1p-21f);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          codes[i] = nearest_codes(to_float(x.v[2 * i]) * w, to_float(x.v[2 * i + 1]) * w, CACHE{});
+      } else {
+        inv = fmaf(fmaf(-inv, s, 1.f), inv, inv);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float q[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float v = to_float(x.v[2 * i + j]), q0 = v * inv;
+            q[j] = fmaf(fmaf(-q0, s, v), inv, q0);
+          }
+          codes[i] = nearest_codes(q[0], q[1], CACHE{});
+        }
+      }
+    } else {
+      const float inv = 1.f / s;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        codes[i] = nearest_codes(quotient_to_odd(x.v[2 * i], s, inv), quotient_to_odd(x.v[2 * i + 1], s, inv), CACHE{});
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      codes[i] = nearest_codes(quotient_by_double(to_float(x.v[2 * i]), s), quotient_by_double(to_float(x.v[2 * i + 1]), s), CACHE{});
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint8_t code = static_cast<uint8_t>(codes[i / 2] >> (8 * (i & 1)));
+    c.v[i] = *reinterpret_cast<const CACHE*>(&code);
+  }
+  return s;
+}
+
+template <typename IN, typename CACHE, int P>
 __global__ void __launch_bounds__(kThreads) write_kernel(const CacheArgs a, int group) {
+  constexpr int N = lane_features(P);
   const int lane = threadIdx.x & (group - 1);
   const unsigned mask = group == 32 ? kFull : ((1u << group) - 1u) << ((threadIdx.x & 31) & ~(group - 1));
   const long long n_rows = a.n_tokens * a.n_heads;
-  const long long stride = static_cast<long long>(gridDim.x) * (kThreads / group);
-  for (long long r = static_cast<long long>(blockIdx.x) * (kThreads / group) + threadIdx.x / group; r < n_rows; r += stride) {
+  const int groups = kThreads / group;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  for (long long r = static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group; r < n_rows; r += stride) {
     long long token;
     int head;
     split_slot(r, a.n_heads, token, head);
     const long long slot = a.slots[token];
     if (slot < 0 || slot >= a.n_slots) continue;  // the whole group leaves together
+    Pack<IN, N> x[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      load_row<P>(x[w], static_cast<const IN*>(a.rows[w].data) + token * a.rows[w].token_stride +
+                            head * a.rows[w].head_stride, lane, a.dim);
     long long page;
     int place;
     split_slot(slot, a.page_size, page, place);
-    Pack<IN, kPerLane> x[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-      load_row<VEC>(x[w], static_cast<const IN*>(a.rows[w].data) + token * a.rows[w].token_stride +
-                              head * a.rows[w].head_stride, lane, a.dim);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const asg_page_pool& pool = a.pools[w];
       CACHE* to = static_cast<CACHE*>(pool.data) + page * pool.page_stride + place * pool.token_stride + head * pool.head_stride;
       if constexpr (!TypeOf<CACHE>::coded) {
-        store_row<VEC>(x[w], to, lane, a.dim);
+        store_row<P>(x[w], to, lane, a.dim);
       } else {
-        // the largest magnitude by its bits: a NaN is above everything and is not lost
-        unsigned top = 0;
-        float v[kPerLane];
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-          v[i] = to_float(x[w].v[i]);
-          top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-        }
-        for (int o = group >> 1; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-        const float s = __uint_as_float(top) / largest_code(CACHE{});
-        Pack<CACHE, kPerLane> c;
-        if (s > 0x1p-90f && s < 0x1p90f) {
-          const float inv = 1.f / s;
-#pragma unroll
-          for (int i = 0; i < kPerLane; ++i) c.v[i] = nearest_code(quotient_to_odd(v[i], s, inv), CACHE{});
-        } else {
-          // a quotient of two 24-bit numbers is never nearer to a border between codes than 2^-40 of itself
-          // without lying on it: the nearest float32 of the float64 quotient, moved off the border, decides
-#pragma unroll
-          for (int i = 0; i < kPerLane; ++i) {
-            const double wide = s == 0.f ? 0.0 : static_cast<double>(v[i]) / static_cast<double>(s);
-            float q = static_cast<float>(wide);
-            const double rest = wide - static_cast<double>(q);
-            if (rest != 0.0 && (__float_as_int(q) & 1) == 0 && q != 0.f && !isinf(q) && rest == rest)
-              q = __int_as_float(__float_as_int(q) + ((rest < 0.0) == (q < 0.f) ? 1 : -1));
-            c.v[i] = nearest_code(q, CACHE{});
-          }
-        }
-        store_row<VEC>(c, to, lane, a.dim);
+        Pack<CACHE, N> c;
+        const float s = quantise(x[w], c, group, mask);
+        store_row<P>(c, to, lane, a.dim);
         if (lane == 0)
           pool.scales[page * pool.scale_page_stride + head * pool.scale_head_stride + place * pool.scale_token_stride] = s;
       }
@@ -149,12 +205,25 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const CacheArgs a, int 
   }
 }
 
-template <typename CACHE, typename OUT, bool VEC>
+// Codes 2 i and 2 i + 1 of a pack as floats.
+template <int N>
+__device__ __forceinline__ float2 two_values(const Pack<E4M3, N>& c, int i) {
+  const uint16_t two = reinterpret_cast<const uint16_t*>(c.v)[i];
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+}
+template <typename T, int N>
+__device__ __forceinline__ float2 two_values(const Pack<T, N>& c, int i) {
+  return make_float2(to_float(c.v[2 * i]), to_float(c.v[2 * i + 1]));
+}
+
+template <typename CACHE, typename OUT, int P>
 __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int group) {
+  constexpr int N = lane_features(P);
   const int lane = threadIdx.x & (group - 1);
   const long long n_rows = a.n_tokens * a.n_heads;
-  const long long stride = static_cast<long long>(gridDim.x) * (kThreads / group);
-  for (long long r = static_cast<long long>(blockIdx.x) * (kThreads / group) + threadIdx.x / group; r < n_rows; r += stride) {
+  const int groups = kThreads / group;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  for (long long r = static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group; r < n_rows; r += stride) {
     long long token;
     int head;
     split_slot(r, a.n_heads, token, head);
@@ -163,43 +232,53 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int g
     long long page = 0;
     int place = 0;
     if (held) split_slot(slot, a.page_size, page, place);
-    Pack<CACHE, kPerLane> c[2];
+    Pack<CACHE, N> c[2];
     float s[2] = {1.f, 1.f};
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const asg_page_pool& pool = a.pools[w];
-      load_row<VEC>(c[w], static_cast<const CACHE*>(pool.data) + page * pool.page_stride + place * pool.token_stride +
-                              head * pool.head_stride, lane, held ? a.dim : 0);
+      load_row<P>(c[w], static_cast<const CACHE*>(pool.data) + page * pool.page_stride + place * pool.token_stride +
+                            head * pool.head_stride, lane, held ? a.dim : 0);
       if (TypeOf<CACHE>::coded && held)
         s[w] = pool.scales[page * pool.scale_page_stride + head * pool.scale_head_stride + place * pool.scale_token_stride];
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      Pack<OUT, kPerLane> x;
+      Pack<OUT, N> x;
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) x.v[i] = from_float<OUT>(TypeOf<CACHE>::coded ? to_float(c[w].v[i]) * s[w] : to_float(c[w].v[i]));
-      store_row<VEC>(x, static_cast<OUT*>(a.rows[w].data) + token * a.rows[w].token_stride + head * a.rows[w].head_stride,
-                     lane, a.dim);
+      for (int i = 0; i < N / 2; ++i) {
+        float2 v = two_values(c[w], i);
+        if (TypeOf<CACHE>::coded) v = make_float2(v.x * s[w], v.y * s[w]);
+        x.v[2 * i] = from_float<OUT>(v.x);
+        x.v[2 * i + 1] = from_float<OUT>(v.y);
+      }
+      store_row<P>(x, static_cast<OUT*>(a.rows[w].data) + token * a.rows[w].token_stride + head * a.rows[w].head_stride,
+                   lane, a.dim);
     }
   }
 }
 
-// Lanes per row and blocks.  The vector form needs rows of whole 8-feature groups that start on 16 bytes
-// (8 for codes); everything else takes a warp a row, one feature in 32 a lane.
+// Features a lane, lanes per row and blocks.  Rows made of whole 32-byte packs of the wide type are moved in those, rows
+// of whole 16-byte packs in those (32768 tokens of 8 x 128 bfloat16 to e4m3: LANE32 against LANE16 us); anything else
+// takes a warp a row, one feature in 32 a lane.
 struct Shape {
-  bool vec;
-  int group;
+  int features, group;
   unsigned blocks;
 };
 
 static Shape shape_of(const CacheArgs& a, int wide_type, int cache_type) {
+  const int wide = type_bytes(wide_type), item = type_bytes(cache_type);
   Shape s;
-  s.vec = a.dim % kPerLane == 0;
-  for (int w = 0; w < 2; ++w)
-    s.vec = s.vec && rows_aligned(a.rows[w], type_bytes(wide_type), 16) &&
-            rows_aligned(a.pools[w], type_bytes(cache_type), is_coded(cache_type) ? 8 : 16);
+  s.features = 0;
+  for (int bytes = 32; bytes >= 16 && s.features == 0; bytes /= 2) {
+    const int p = bytes / wide, packed = p * item;
+    bool fits = a.dim % p == 0 && a.dim <= 32 * p;
+    for (int w = 0; w < 2; ++w)
+      fits = fits && rows_aligned(a.rows[w], wide, bytes) && rows_aligned(a.pools[w], item, packed < 32 ? packed : 32);
+    if (fits) s.features = p;
+  }
   s.group = 32;
-  while (s.vec && s.group > 1 && s.group / 2 * kPerLane >= a.dim) s.group /= 2;
+  while (s.features > 0 && s.group > 1 && s.group / 2 * s.features >= a.dim) s.group /= 2;
   const long long rows_per_block = kThreads / s.group;
   const long long blocks = (a.n_tokens * a.n_heads + rows_per_block - 1) / rows_per_block;
   s.blocks = static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20));
@@ -208,9 +287,11 @@ static Shape shape_of(const CacheArgs& a, int wide_type, int cache_type) {
 
 template <typename IN, typename CACHE>
 static int launch_write(const CacheArgs& a, cudaStream_t stream) {
+  constexpr int most = 32 / static_cast<int>(sizeof(IN));
   const Shape s = shape_of(a, TypeOf<IN>::id, TypeOf<CACHE>::id);
-  if (s.vec) write_kernel<IN, CACHE, true><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else write_kernel<IN, CACHE, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  if (s.features == most) write_kernel<IN, CACHE, most><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else if (s.features > 0) write_kernel<IN, CACHE, most / 2><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else write_kernel<IN, CACHE, 0><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }
@@ -223,9 +304,11 @@ static int launch_write(const CacheArgs& a, int cache_type, cudaStream_t stream)
 
 template <typename CACHE, typename OUT>
 static int launch_read(const CacheArgs& a, cudaStream_t stream) {
+  constexpr int most = 32 / static_cast<int>(sizeof(OUT));
   const Shape s = shape_of(a, TypeOf<OUT>::id, TypeOf<CACHE>::id);
-  if (s.vec) read_kernel<CACHE, OUT, true><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else read_kernel<CACHE, OUT, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  if (s.features == most) read_kernel<CACHE, OUT, most><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else if (s.features > 0) read_kernel<CACHE, OUT, most / 2><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else read_kernel<CACHE, OUT, 0><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }

@@ -35,58 +35,66 @@ MAX_HEAD_DIM = 256
 def _index(name: str, tensor: torch.Tensor, device: torch.device) -> torch.Tensor:
     if tensor.dtype not in _INDEX_DTYPES:
         raise TypeError(f"{name} must use integer indices")
-    if tensor.ndim != 1:
+    if tensor.dim() != 1:
         raise ValueError(f"{name} must be one-dimensional")
     if tensor.device != device:
         raise ValueError(f"{name} must be on the device of the pages")
-    return tensor.to(torch.long).contiguous()
+    if tensor.dtype is not torch.int64:
+        tensor = tensor.to(torch.int64)
+    return tensor if tensor.is_contiguous() else tensor.contiguous()
 
 
-def _check_pages(key_pages, value_pages, key_scales, value_scales) -> None:
-    if key_pages.ndim != 4 or key_pages.shape != value_pages.shape:
+def _check_pages(key_pages, value_pages, key_scales, value_scales) -> tuple:
+    """Checks the pages and returns (n_pages, page_size, heads, dim)."""
+    shape = key_pages.shape
+    if len(shape) != 4 or shape != value_pages.shape:
         raise ValueError("key_pages and value_pages must have the same [n_pages, page_size, n_kv_heads, head_dim] shape")
-    _, page_size, heads, dim = key_pages.shape
-    if min(page_size, heads, dim) < 1:
+    n_pages, page_size, heads, dim = shape
+    if page_size < 1 or heads < 1 or dim < 1:
         raise ValueError("page_size, n_kv_heads and head_dim must be positive")
     if dim > MAX_HEAD_DIM:
         raise ValueError(f"head_dim is at most {MAX_HEAD_DIM}")
-    if key_pages.dtype != value_pages.dtype or key_pages.dtype not in _WIDE + _CODED:
+    dtype = key_pages.dtype
+    if dtype != value_pages.dtype or (dtype not in _WIDE and dtype not in _CODED):
         raise TypeError("the pages must both be float32, bfloat16, float16, float8_e4m3fn or int8")
     if dim > 1 and (key_pages.stride(3) != 1 or value_pages.stride(3) != 1):
         raise ValueError("the features of a page row must be contiguous")
     device = key_pages.device
     if value_pages.device != device:
         raise ValueError("key_pages and value_pages must be on the same device")
-    if key_pages.dtype in _CODED:
+    if dtype in _CODED:
         for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
             if scales is None:
                 raise ValueError(f"8-bit pages need {name}")
-            if scales.dtype != torch.float32:
+            if scales.dtype is not torch.float32:
                 raise TypeError(f"{name} must be float32")
-            if scales.shape != (key_pages.size(0), heads, page_size):
+            if scales.shape != (n_pages, heads, page_size):
                 raise ValueError(f"{name} must have shape [n_pages, n_kv_heads, page_size]")
             if scales.device != device:
                 raise ValueError(f"{name} must be on the device of the pages")
     elif key_scales is not None or value_scales is not None:
         raise ValueError("scales go with 8-bit pages only")
+    return n_pages, page_size, heads, dim
 
 
 def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
     if device.type != "cuda":
         raise RuntimeError("the paged cache needs CUDA tensors")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor is not None and tensor.requires_grad:
+                raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
     if not ops.load_native():
         detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")
 
 
 def _contiguous_features(rows: torch.Tensor) -> torch.Tensor:
-    return rows if rows.size(-1) <= 1 or rows.stride(-1) == 1 else rows.contiguous()
+    return rows if rows.stride(2) == 1 or rows.size(2) <= 1 else rows.contiguous()
 
 
 def _checking() -> bool:
-    return os.getenv("AUTOSAGE_CHECK_INDICES") == "1"
+    return os.environ.get("AUTOSAGE_CHECK_INDICES") == "1"
 
 
 def _check_writable(name: str, tensor: Optional[torch.Tensor]) -> None:
@@ -105,8 +113,9 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
 
     A slot outside the pages (-1, say) is skipped: padding.  The others must differ from one another: of two tokens
     with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call)."""
-    _check_pages(key_pages, value_pages, key_scales, value_scales)
-    if key.ndim != 3 or key.shape != value.shape or key.shape[1:] != key_pages.shape[2:]:
+    n_pages, page_size, heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
+    shape = key.shape
+    if len(shape) != 3 or shape != value.shape or shape[1] != heads or shape[2] != dim:
         raise ValueError("key and value must have the same [tokens, n_kv_heads, head_dim] shape, as wide as the pages")
     if key.dtype != value.dtype or key.dtype not in _WIDE:
         raise TypeError("key and value must both be float32, bfloat16 or float16")
@@ -116,16 +125,16 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     if key.device != device or value.device != device:
         raise ValueError("key and value must be on the device of the pages")
     slots = _index("slots", slots, device)
-    if slots.numel() != key.size(0):
+    if slots.numel() != shape[0]:
         raise ValueError("slots must contain one slot per token")
     for name, tensor in (("key_pages", key_pages), ("value_pages", value_pages), ("key_scales", key_scales),
                          ("value_scales", value_scales)):
         _check_writable(name, tensor)
     _require_native(device, key, value, key_pages, value_pages)
-    if slots.numel() == 0 or key_pages.size(0) == 0:
+    if slots.numel() == 0 or n_pages == 0:
         return
     if _checking():
-        kept = slots[(slots >= 0) & (slots < key_pages.size(0) * key_pages.size(1))]
+        kept = slots[(slots >= 0) & (slots < n_pages * page_size)]
         if kept.unique().numel() != kept.numel():
             raise RuntimeError("two tokens have the same slot")
     _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
@@ -137,7 +146,7 @@ def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: 
                      dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values in the slots ``slots``, as two ``[T, n_kv_heads, head_dim]`` tensors of type ``dtype`` (that
     of the pages, or float32 for 8-bit pages).  Slots may repeat; one outside the pages reads as zeros."""
-    _check_pages(key_pages, value_pages, key_scales, value_scales)
+    _, _, heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
     if dtype is None:
         dtype = torch.float32 if key_pages.dtype in _CODED else key_pages.dtype
     if dtype not in _WIDE:
@@ -145,17 +154,16 @@ def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: 
     device = key_pages.device
     slots = _index("slots", slots, device)
     _require_native(device, key_pages, value_pages, key_scales, value_scales)
-    shape = (slots.numel(), key_pages.size(2), key_pages.size(3))
-    key, value = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
-    if slots.numel():
+    tokens = slots.numel()
+    key = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    value = torch.empty_like(key)
+    if tokens:
         _native.paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales)
     return key, value
 
 
 def _debug_check_table(crow, col, lengths, n_pages: int, page_size: int) -> None:
     """AUTOSAGE_CHECK_INDICES=1: verify the page table before the launch (synchronises)."""
-    if not _checking():
-        return
     if int(crow[0].item()) != 0 or int(crow[-1].item()) != col.numel():
         raise RuntimeError("crow must run from 0 to the number of columns")
     pages = crow[1:] - crow[:-1]
@@ -183,11 +191,13 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
     logarithm of each softmax's denominator as float32 ``[B, n_heads]`` (parts computed over different pages can be
     joined with it).  A row that sees nothing gives 0 and ``-inf``.  A page id outside the pages is a hole whose
     tokens are not seen; whatever lies behind a row's length in its last pages is not read."""
-    _check_pages(key_pages, value_pages, key_scales, value_scales)
+    n_pages, page_size, kv_heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
     device = key_pages.device
-    if query.ndim != 3 or query.size(2) != key_pages.size(3):
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != dim:
         raise ValueError("query must have shape [rows, n_heads, head_dim] with the pages' head_dim")
-    if query.size(1) < 1 or query.size(1) % key_pages.size(2) != 0:
+    rows, heads, _ = shape
+    if heads < 1 or heads % kv_heads != 0:
         raise ValueError("n_heads must be a positive multiple of n_kv_heads")
     if query.dtype not in _WIDE:
         raise TypeError("query must be float32, bfloat16 or float16")
@@ -196,7 +206,6 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
     if query.device != device:
         raise ValueError("query must be on the device of the pages")
     crow, col, lengths = _index("crow", crow, device), _index("col", col, device), _index("lengths", lengths, device)
-    rows = query.size(0)
     if crow.numel() != rows + 1:
         raise ValueError("crow must contain one entry per row and one more")
     if lengths.numel() != rows:
@@ -204,12 +213,13 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
     if window is not None and window < 1:
         raise ValueError("window must be positive")
     _require_native(device, query, key_pages, value_pages, key_scales, value_scales)
-    out = torch.empty(query.shape, dtype=query.dtype, device=device)
-    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
     if rows:
-        _debug_check_table(crow, col, lengths, key_pages.size(0), key_pages.size(1))
+        if _checking():
+            _debug_check_table(crow, col, lengths, n_pages, page_size)
         _native.paged_attention(crow, col, lengths, _contiguous_features(query), out, lse, key_pages, value_pages, key_scales,
-                                value_scales, scale=1.0 if scale is None else float(scale), window=int(window or 0))
+                                value_scales, 1.0 if scale is None else float(scale), 0 if window is None else int(window))
     return (out, lse) if return_lse else out
 
 
