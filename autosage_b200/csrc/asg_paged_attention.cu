@@ -156,6 +156,7 @@ int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* 
   a.type = type;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.q_pairs = rows_aligned(*q, type_bytes(type), 8);
+  a.same_strides = a.key.page_stride == a.value.page_stride && a.key.token_stride == a.value.token_stride;
   a.out_vector = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   a.partial_pitch = (head_dim + 3) / 4 * 4;
   // 16-bit queries run on the tensor cores wherever 16-byte copies can fetch the rows; float32 queries, whose

@@ -13,6 +13,8 @@
 // Softmax: scores are kept in units of log2 (scale * log2(e) is folded into q), each warp keeps a running
 // maximum m, sum l and accumulator o of its tokens:
 //   m' = max(m, s),  o' = o 2^(m - m') + 2^(s - m') v,  l' = l 2^(m - m') + 2^(s - m').
+// m moves only when a score exceeds it by more than kSlack: weights up to 2^kSlack do no harm in float32, and most
+// tiles then need neither the maximum over their lanes nor the rescaling (each of them a third of a tile's work).
 // With 8-bit pages the key scale multiplies the score and the value scale the weight; codes are never
 // multiplied out in memory.
 #pragma once
@@ -26,10 +28,12 @@
 namespace asg {
 namespace paged {
 
-constexpr int kWarps = 4;                  // warps of a CTA; each takes every fourth tile of a piece
-constexpr int kUnit = 64;                  // tokens per unit: one 16-token tile for each warp
-constexpr int kTile = kUnit / kWarps;
+constexpr int kRings = 4;                  // warps, or groups of warps, of a CTA; each takes every fourth tile of a piece
+constexpr int kUnit = 64;                  // tokens per unit: one 16-token tile for each ring
+constexpr int kTile = kUnit / kRings;
 constexpr int kStart = 2;                  // cost of starting an item, in units (where the GPU has more than a unit a CTA)
+constexpr float kSlack = 6.f;
+constexpr float kNoScore = -3.402823466e38f; // m before the first score: every finite score is above it
 constexpr int kMaxCtasPerSm = 4;           // bounds the workspace; no kernel is launched with more
 
 struct AttentionArgs {
@@ -49,6 +53,7 @@ struct AttentionArgs {
   float scale_log2; // scale * log2(e)
   bool q_pairs;     // the query's rows start on 8 bytes
   bool join;        // the join kernel follows
+  bool same_strides;  // of the pages of keys and values: one offset serves both
   bool out_vector;  // four neighbours of out can be stored at once
   int partial_pitch;
   float* partial;   // [G][2][GT][partial_pitch] accumulators of unfinished pieces
@@ -96,12 +101,13 @@ struct Share {
 };
 
 // Every thread sums the units of its rows, a block scan finds the row that holds the share's first entry.
+template <int WARPS>
 __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
-  __shared__ long long warp_units[kWarps], warp_rows[kWarps];
+  __shared__ long long warp_units[WARPS], warp_rows[WARPS];
   __shared__ long long found_begin;
   __shared__ int found_row;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per_thread = (a.n_rows + kWarps * 32 - 1) / (kWarps * 32);
+  const int per_thread = (a.n_rows + WARPS * 32 - 1) / (WARPS * 32);
   const long long r0 = static_cast<long long>(tid) * per_thread;
   long long units = 0, rows = 0;
   for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) {
@@ -126,7 +132,7 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
   __syncthreads();
   long long units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) {
       units_before += warp_units[w];
       rows_before += warp_rows[w];
@@ -214,28 +220,28 @@ __device__ __forceinline__ void store_four(const AttentionArgs& a, long long row
     if (d + i < a.dim) store_wide(a.out, at + i, a.type, x[i]);
 }
 
-// The warps' parts of one piece lie in shared memory: warp w's accumulators o[w * warp_stride + g * PITCH + d] and
+// The rings' parts of one piece lie in shared memory: ring w's accumulators o[w * ring_stride + g * PITCH + d] and
 // ml[w * GT + g] = (m, l).  Puts them together and stores the result (whole item) or a partial record.  All threads
 // call it between barriers.
-template <int GT, int DIM, int PITCH>
+template <int THREADS, int GT, int DIM, int PITCH>
 __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot,
-                                            const float* o, int warp_stride, const float2* ml) {
+                                            const float* o, int ring_stride, const float2* ml) {
   __shared__ float4 factors[GT];
-  static_assert(kWarps == 4, "one float4 of factors per head");
+  static_assert(kRings == 4, "one float4 of factors per head");
   const int heads = min(GT, a.group - sub * GT);
   const long long first_row = static_cast<long long>(row) * a.n_heads + kv_head * a.group + sub * GT;
   const long long first_record = (static_cast<long long>(blockIdx.x) * 2 + slot) * GT;
   const int tid = threadIdx.x;
   if (tid < heads) {
-    float2 part[kWarps];
-    float top = -CUDART_INF_F, sum = 0.f, f[kWarps];
+    float2 part[kRings];
+    float top = -CUDART_INF_F, sum = 0.f, f[kRings];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kRings; ++w) {
       part[w] = ml[w * GT + tid];
       top = fmaxf(top, part[w].x);
     }
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kRings; ++w) {
       f[w] = part_factor(part[w].x, part[w].y, top);
       sum += f[w] * part[w].y;
     }
@@ -250,13 +256,13 @@ __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int
   }
   __syncthreads();
   constexpr int kFours = DIM / 4;
-  for (int i = tid; i < heads * kFours; i += kWarps * 32) {
+  for (int i = tid; i < heads * kFours; i += THREADS) {
     const int g = i / kFours, d = i % kFours * 4;
     if (d >= a.dim) continue;
     const float4 f = factors[g];
     const float* at = o + g * PITCH + d;
-    const float4 x0 = *reinterpret_cast<const float4*>(at), x1 = *reinterpret_cast<const float4*>(at + warp_stride),
-                 x2 = *reinterpret_cast<const float4*>(at + 2 * warp_stride), x3 = *reinterpret_cast<const float4*>(at + 3 * warp_stride);
+    const float4 x0 = *reinterpret_cast<const float4*>(at), x1 = *reinterpret_cast<const float4*>(at + ring_stride),
+                 x2 = *reinterpret_cast<const float4*>(at + 2 * ring_stride), x3 = *reinterpret_cast<const float4*>(at + 3 * ring_stride);
     const float4 v = make_float4(f.x * x0.x + f.y * x1.x + f.z * x2.x + f.w * x3.x, f.x * x0.y + f.y * x1.y + f.z * x2.y + f.w * x3.y,
                                  f.x * x0.z + f.y * x1.z + f.z * x2.z + f.w * x3.z, f.x * x0.w + f.y * x1.w + f.z * x2.w + f.w * x3.w);
     if (slot < 0) store_four(a, first_row + g, d, v);
@@ -290,7 +296,7 @@ struct Walk {
   RowSpan span;
   long long units, at;  // of the row's items; entry inside the item
   int item, items_per_row;
-  __device__ __forceinline__ Walk(const AttentionArgs& a, int items) : s(locate_share(a, items)), items_per_row(items) {
+  __device__ __forceinline__ Walk(const AttentionArgs& a, int items, const Share& share) : s(share), items_per_row(items) {
     if (s.pos >= s.end) return;
     span = row_span(a, s.row);
     units = span.units();
@@ -327,26 +333,98 @@ struct Walk {
   }
 };
 
-// The kernel around an Engine, which computes one warp's part of a piece:
+// The copies of a ring: where they come from and how far they are.  Lane l looks after token l % 16 of the next
+// tile: the page of the table it lies in, its place there, and the page's id, loaded one tile ahead.
+struct Source {
+  const char* keys;
+  const char* values;
+  const int64_t* ids;                 // of the page that holds the piece's first token
+  long long page_bytes, token_bytes;  // of the keys' pages
+  int kv_head, count, tile;
+  int nth, place;
+  int step_pages, step_place;         // kUnit tokens on
+  long long id;
+
+  __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p, int ring, int item_bytes) {
+    keys = static_cast<const char*>(a.key.data) + p.kv_head * a.key.head_stride * item_bytes;
+    values = static_cast<const char*>(a.value.data) + p.kv_head * a.value.head_stride * item_bytes;
+    page_bytes = a.key.page_stride * item_bytes;
+    token_bytes = a.key.token_stride * item_bytes;
+    kv_head = p.kv_head;
+    const unsigned page_size = static_cast<unsigned>(a.page_size);
+    const long long first = p.first(), page0 = quotient(first, a.page_size);  // 32-bit page arithmetic from here on
+    ids = a.col + p.span.pages_begin + page0;
+    count = static_cast<int>(p.last() - first);
+    tile = ring * kTile;
+    const unsigned at = static_cast<unsigned>(first - page0 * a.page_size) + tile + (lane_id() & (kTile - 1));
+    nth = static_cast<int>(at / page_size);
+    place = static_cast<int>(at % page_size);
+    step_pages = static_cast<int>(kUnit / page_size);
+    step_place = static_cast<int>(kUnit % page_size);
+    look_up();
+  }
+  __device__ __forceinline__ void look_up() { id = tile + (lane_id() & (kTile - 1)) < count ? ids[nth] : -1; }
+  __device__ __forceinline__ bool held(const AttentionArgs& a) const { return id >= 0 && id < a.n_pages; }
+  __device__ __forceinline__ void advance(const AttentionArgs& a) {
+    tile += kUnit;
+    nth += step_pages;
+    place += step_place;
+    if (place >= a.page_size) {
+      place -= a.page_size;
+      ++nth;
+    }
+    look_up();
+  }
+};
+
+// bytes of global memory into shared memory, zeros if !ok (nothing is read then)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool ok) {
+  static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "sizes of cp.async");
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 2^x and log2(x) of the hardware (results and arguments below the normal range count as 0)
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// A part's maximum as the joins know it: minus infinity where no score has been.
+__device__ __forceinline__ float published_max(float m) { return m == kNoScore ? -CUDART_INF_F : m; }
+
+// The kernel around an Engine, which computes one ring's part of a piece:
 //   Engine(smem)                      once
 //   start(a, piece)                   begins to fetch the piece's tokens; the part of the piece before is still unpublished
 //   query(a, piece)                   takes the query and clears the accumulators
-//   run(a)                            the warp's tiles
-//   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + warp * kWarpBytes +
+//   run(a)                            the ring's tiles
+//   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + ring * kRingBytes +
 //                                     kPublish, which no copy of a started piece writes before run()
-// kWarpBytes * kWarps bytes of shared memory belong to the engine, the (m, l) pairs lie behind them.
+// kRingBytes * kRings bytes of shared memory belong to the engine, the (m, l) pairs lie behind them.
 template <typename Engine>
-__global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
   constexpr int GT = Engine::kHeads;
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_release_dependents();
-  Walk walk(a, a.n_kv_heads * a.subgroups);
+  const int items_per_row = a.n_kv_heads * a.subgroups;
+  Walk walk(a, items_per_row, locate_share<Engine::kThreads / 32>(a, items_per_row));
   int4 left_over = make_int4(0, 0, 0, 0);
   Piece now;
   if (walk.next(a, now)) {
     Engine engine(smem);
     const float* o = reinterpret_cast<const float*>(smem + Engine::kPublish);
-    float2* ml = reinterpret_cast<float2*>(smem + kWarps * Engine::kWarpBytes);
+    float2* ml = reinterpret_cast<float2*>(smem + kRings * Engine::kRingBytes);
     engine.start(a, now);
     engine.query(a, now);
     for (bool more = true; more;) {
@@ -367,7 +445,8 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
         left_over.y = now.item;
         left_over.z = 1;
       }
-      store_piece<GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o, Engine::kWarpBytes / 4, ml);
+      store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o,
+                                                                    Engine::kRingBytes / 4, ml);
       __syncthreads();  // the buffers are free again
       now = next;
     }
@@ -379,8 +458,8 @@ __global__ void __launch_bounds__(kWarps * 32, Engine::kCtasPerSm) attention_ker
 // Host: launch of one instance.
 template <typename Engine>
 int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
-  constexpr int smem = kWarps * (Engine::kWarpBytes + Engine::kHeads * static_cast<int>(sizeof(float2)));
-  static_assert(Engine::kWarpBytes >= Engine::kPublish + Engine::kHeads * Engine::kPitch * 4 && Engine::kWarpBytes % 128 == 0, "warp region");
+  constexpr int smem = kRings * (Engine::kRingBytes + Engine::kHeads * static_cast<int>(sizeof(float2)));
+  static_assert(Engine::kRingBytes >= Engine::kPublish + Engine::kHeads * Engine::kPitch * 4 && Engine::kRingBytes % 128 == 0, "ring region");
   static_assert(Engine::kCtasPerSm <= kMaxCtasPerSm && Engine::kCtasPerSm * (smem + 1024) <= 228 * 1024, "shared memory");
   auto kernel = attention_kernel<Engine>;
   if (smem > 48 * 1024) {  // once per device
@@ -393,7 +472,7 @@ int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
       if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  kernel<<<ctas, kWarps * 32, smem, stream>>>(args);
+  kernel<<<ctas, Engine::kThreads, smem, stream>>>(args);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }

@@ -5,46 +5,51 @@
 // the number of values and the lanes they are spread over) leaves one whole score per lane for about one
 // shuffle a score, and exponentials are taken once, by the lane that owns the score.  The weights come back
 // to all lanes by one shuffle each.
+//
+// Every warp has a ring of kStages batches in shared memory.  Where a lane's E features of a row are one aligned
+// vector (VEC), cp.async brings them there, several batches ahead; a lane copies what it will read itself.
+// Otherwise the lanes load element by element and store into the ring.
 #include "asg_paged_attention.cuh"
 
 namespace asg {
 namespace paged {
 
-template <typename T, int E, int GT, bool VEC>
+template <typename T, int E, int GT, bool VEC, int STAGES, int CTAS>
 struct General {
+  static constexpr int kThreads = kRings * 32;
   static constexpr int kHeads = GT;
+  static constexpr int kCtasPerSm = CTAS;
+  static constexpr int kStages = STAGES;
+  static constexpr bool kCoded = TypeOf<T>::coded;
+  static constexpr int TB = E == 8 || GT == 8 ? 4 : 8;  // tokens per batch
+  static constexpr int kBatches = kTile / TB;           // of a tile
+  static constexpr int N = TB * GT;                     // scores per batch: 4 ... 32
+  static constexpr int kShift = N == 32 ? 0 : N == 16 ? 1 : N == 8 ? 2 : 3;
+  static_assert(N == 32 || N == 16 || N == 8 || N == 4, "reduce-scatter sizes");
   static constexpr int kDim = 32 * E;
   static constexpr int kPitch = kDim;
-  static constexpr int kCtasPerSm = GT * E >= 32 ? 3 : 4;     // registers: q and o take 2 GT E, a batch 2 TB E
-  static constexpr int TB = E == 8 ? 4 : (GT == 8 ? 4 : 8);  // tokens per batch: K and V rows of a batch are in registers
-  static constexpr int N = TB * GT;                          // scores per batch: 4 ... 32
-  static constexpr int kShift = N == 32 ? 0 : N == 16 ? 1 : N == 8 ? 2 : 3;
-  static constexpr int kWarpBytes = GT * kPitch * 4;
-  static constexpr int kPublish = 0;
-  static_assert(N == 32 || N == 16 || N == 8 || N == 4, "reduce-scatter sizes");
+  static constexpr int kLaneBytes = E * static_cast<int>(sizeof(T));
+  static constexpr int kRowBytes = 32 * kLaneBytes;
+  static constexpr int kValues = TB * kRowBytes;
+  static constexpr int kExtras = 2 * TB * kRowBytes;  // the scales of a batch (key, value), then the mask of its seen tokens
+  static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * TB * 4 : 0) + 4 + 15) / 16 * 16;
+  static constexpr int kPublish = (kStages - 1) * kStageBytes;
+  static constexpr int kNeed = kPublish + (kStageBytes > GT * kPitch * 4 ? kStageBytes : GT * kPitch * 4);
+  static constexpr int kRingBytes = (kNeed + 127) / 128 * 128;
 
   float q[GT][E], o[GT][E];
   float m, l;  // of the head that this lane owns scores of: head (lane >> kShift) % GT
-  int lane, warp;
+  int lane, ring;
+  unsigned char* region;
+  Source s;
+  int batch;                              // of the tile that is copied next
+  bool held;                              // of the lane's token of that tile
+  long long key_offset, value_offset;     // in bytes
 
-  __device__ __forceinline__ explicit General(unsigned char*) : lane(threadIdx.x & 31), warp(threadIdx.x >> 5) {}
+  __device__ __forceinline__ explicit General(unsigned char* smem)
+      : lane(threadIdx.x & 31), ring(threadIdx.x >> 5), region(smem + (threadIdx.x >> 5) * kRingBytes) {}
 
   static __device__ __forceinline__ int feature(int lane, int e) { return VEC ? lane * E + e : e * 32 + lane; }
-
-  const T* keys;
-  const T* values;
-  const int64_t* ids;  // of the page that holds the piece's first token
-  int kv_head, place0, count;
-
-  __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
-    kv_head = p.kv_head;
-    keys = static_cast<const T*>(a.key.data) + kv_head * a.key.head_stride;
-    values = static_cast<const T*>(a.value.data) + kv_head * a.value.head_stride;
-    const long long first = p.first(), page0 = quotient(first, a.page_size);  // page arithmetic in 32 bits from here on
-    place0 = static_cast<int>(first - page0 * a.page_size);
-    ids = a.col + p.span.pages_begin + page0;
-    count = static_cast<int>(p.last() - first);
-  }
 
   __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
     const int head = p.kv_head * a.group + p.sub * GT, heads = min(GT, a.group - p.sub * GT);
@@ -58,131 +63,190 @@ struct General {
                       : 0.f;
         o[g][e] = 0.f;
       }
-    m = -CUDART_INF_F;
+    m = kNoScore;
     l = 0.f;
   }
 
-  __device__ __forceinline__ void load(float (&x)[E], const T* row, bool ok, int dim) const {
-    if constexpr (VEC) {
-      Pack<T, E> p;
-      if (ok && lane * E < dim) {
-        p.load(row + lane * E);
+  // Where the lane's token of the tile lies.
+  __device__ __forceinline__ void locate(const AttentionArgs& a) {
+    constexpr int item = static_cast<int>(sizeof(T));
+    held = s.held(a);
+    key_offset = held ? s.id * s.page_bytes + s.place * s.token_bytes : 0;
+    value_offset = held ? s.id * a.value.page_stride * item + s.place * a.value.token_stride * item : 0;
+  }
+
+  // Copies the next batch to a stage.
+  __device__ __forceinline__ void issue(const AttentionArgs& a, int stage) {
+    if (s.tile + batch * TB < s.count) {
+      const unsigned seen = __ballot_sync(kFull, held) >> (batch * TB) & ((1u << TB) - 1u);
+      unsigned char* at = region + stage * kStageBytes;
+      const int key_low = static_cast<int>(key_offset), key_high = static_cast<int>(key_offset >> 32);
+      const int value_low = static_cast<int>(value_offset), value_high = static_cast<int>(value_offset >> 32);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = to_float(p.v[e]);
-      } else {
+      for (int t = 0; t < TB; ++t) {
+        const int from = batch * TB + t;
+        const long long k = static_cast<long long>(__shfl_sync(kFull, key_high, from)) << 32 |
+                            static_cast<unsigned>(__shfl_sync(kFull, key_low, from));
+        const long long v = a.same_strides ? k : static_cast<long long>(__shfl_sync(kFull, value_high, from)) << 32 |
+                                                     static_cast<unsigned>(__shfl_sync(kFull, value_low, from));
+        const bool ok = (seen >> t & 1u) != 0;
+        unsigned char* to = at + t * kRowBytes + lane * kLaneBytes;
+        if constexpr (VEC) {
+          constexpr int kStep = kLaneBytes < 16 ? kLaneBytes : 16;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = 0.f;
+          for (int b = 0; b < kLaneBytes; b += kStep) {
+            copy_async<kStep>(smem_u32(to) + b, s.keys + k + lane * kLaneBytes + b, ok && lane * E < a.dim);
+            copy_async<kStep>(smem_u32(to) + kValues + b, s.values + v + lane * kLaneBytes + b, ok && lane * E < a.dim);
+          }
+        } else {
+          const T* keys = reinterpret_cast<const T*>(s.keys + k);
+          const T* values = reinterpret_cast<const T*>(s.values + v);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const bool in = ok && feature(lane, e) < a.dim;
+            reinterpret_cast<T*>(to)[e] = in ? keys[feature(lane, e)] : T{};
+            reinterpret_cast<T*>(to + kValues)[e] = in ? values[feature(lane, e)] : T{};
+          }
+        }
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = ok && feature(lane, e) < dim ? to_float(row[feature(lane, e)]) : 0.f;
+      if constexpr (kCoded) {
+        // lanes of the batch's tokens: their key scales; sixteen lanes on: their value scales
+        const int token = (lane & (kTile - 1)) - batch * TB;
+        if (token >= 0 && token < TB) {
+          const asg_page_pool& pool = lane < kTile ? a.key : a.value;
+          const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
+          if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
+          copy_async<4>(smem_u32(at + kExtras) + ((lane < kTile ? 0 : TB) + token) * 4, from, held);
+        }
+      }
+      if (lane == 0) *reinterpret_cast<unsigned*>(at + kStageBytes - 4) = seen;
+    }
+    copy_commit();
+    if (++batch == kBatches) {
+      batch = 0;
+      s.advance(a);
+      locate(a);
     }
   }
 
-  __device__ __forceinline__ void run(const AttentionArgs& a) {
-    for (int tile = warp * kTile; tile < count; tile += kUnit) {
-      // lane t < kTile finds token tile + t
-      int page = -1, place = 0;
-      float key_scale = 0.f, value_scale = 0.f;
-      if (lane < kTile && tile + lane < count) {
-        const unsigned at = static_cast<unsigned>(place0) + static_cast<unsigned>(tile + lane);
-        const unsigned nth = at / static_cast<unsigned>(a.page_size);
-        const long long id = ids[nth];
-        place = static_cast<int>(at - nth * static_cast<unsigned>(a.page_size));
-        if (id >= 0 && id < a.n_pages) page = static_cast<int>(id);
-        if (TypeOf<T>::coded && page >= 0) {
-          key_scale = a.key.scales[page * a.key.scale_page_stride + kv_head * a.key.scale_head_stride + place * a.key.scale_token_stride];
-          value_scale = a.value.scales[page * a.value.scale_page_stride + kv_head * a.value.scale_head_stride + place * a.value.scale_token_stride];
-        }
-      }
+  __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
+    s.start(a, p, ring, static_cast<int>(sizeof(T)));
+    batch = 0;
+    locate(a);
 #pragma unroll 1
-      for (int t0 = 0; t0 < kTile && tile + t0 < count; t0 += TB) {
-        float k[TB][E], v[TB][E];
-        bool any = false;
+    for (int i = 0; i < kStages - 1; ++i) issue(a, i);
+  }
+
+  __device__ __forceinline__ void run(const AttentionArgs& a) {
+    const int tiles = s.count <= ring * kTile ? 0 : (s.count - ring * kTile + kUnit - 1) / kUnit;
+    int stage = 0, fill = kStages - 1;
+#pragma unroll 1
+    for (int i = 0; i < tiles * kBatches; ++i) {
+      const int first = ring * kTile + i / kBatches * kUnit + i % kBatches * TB;
+      copy_wait<kStages - 2>();
+      __syncwarp();  // the batch has arrived for all lanes, and all have left the stage that is filled next
+      issue(a, fill);
+      if (first < s.count) compute(region + stage * kStageBytes);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      fill = fill + 1 == kStages ? 0 : fill + 1;
+    }
+    copy_wait<0>();
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void row_of(float (&x)[E], const unsigned char* at) const {
+    const T* from = reinterpret_cast<const T*>(at + lane * kLaneBytes);
+    Pack<T, E> p;
+    if constexpr (Pack<T, E>::kVec <= 16) {
+      Pack<T, E>::move(p.v, from);
+    } else {
 #pragma unroll
-        for (int t = 0; t < TB; ++t) {
-          const int p = __shfl_sync(kFull, page, t0 + t);
-          const int in = __shfl_sync(kFull, place, t0 + t);
-          any = any || p >= 0;
-          load(k[t], keys + p * a.key.page_stride + in * a.key.token_stride, p >= 0, a.dim);
-          load(v[t], values + p * a.value.page_stride + in * a.value.token_stride, p >= 0, a.dim);
-        }
-        if (!any) continue;  // only holes
-        float x[N];
+      for (int i = 0; i < kLaneBytes / 16; ++i) reinterpret_cast<uint4*>(p.v)[i] = reinterpret_cast<const uint4*>(from)[i];
+    }
 #pragma unroll
-        for (int t = 0; t < TB; ++t)
+    for (int e = 0; e < E; ++e) x[e] = to_float(p.v[e]);
+  }
+
+  __device__ __forceinline__ void compute(const unsigned char* at) {
+    float x[N];
 #pragma unroll
-          for (int g = 0; g < GT; ++g) {
-            float s = 0.f;
+    for (int t = 0; t < TB; ++t) {
+      float k[E];
+      row_of(k, at + t * kRowBytes);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(q[g][e], k[t][e], s);
-            x[t * GT + g] = s;
-          }
-        // reduce-scatter: afterwards lane L holds the whole score of index L >> kShift
-        int n = N;
+      for (int g = 0; g < GT; ++g) {
+        float sum = 0.f;
 #pragma unroll
-        for (int step = 16; step >= 1; step >>= 1) {
-          if (n > 1) {
-            n >>= 1;
+        for (int e = 0; e < E; ++e) sum = fmaf(q[g][e], k[e], sum);
+        x[t * GT + g] = sum;
+      }
+    }
+    // reduce-scatter: afterwards lane L holds the whole score of index L >> kShift
+    int n = N;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-              if (i < n) {
-                const bool upper = (lane & step) != 0;
-                const float keep = upper ? x[i + n] : x[i];
-                const float send = upper ? x[i] : x[i + n];
-                x[i] = keep + __shfl_xor_sync(kFull, send, step);
-              }
-            }
-          } else {
-            x[0] += __shfl_xor_sync(kFull, x[0], step);
-          }
-        }
-        const int mine = lane >> kShift;  // token mine / GT, head mine % GT
-        const int token = t0 + mine / GT;
-        const bool seen = __shfl_sync(kFull, page, token) >= 0;
-        float weight_scale = 1.f;
-        if (TypeOf<T>::coded) {
-          x[0] *= __shfl_sync(kFull, key_scale, token);
-          weight_scale = __shfl_sync(kFull, value_scale, token);
-        }
-        const float s = seen ? x[0] : -CUDART_INF_F;
-        float top = s;
+    for (int step = 16; step >= 1; step >>= 1) {
+      if (n > 1) {
+        n >>= 1;
 #pragma unroll
-        for (int step = 16; step >= GT << kShift; step >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, step));
-        top = fmaxf(top, m);
-        const float base = top == -CUDART_INF_F ? 0.f : top;
-        const float shrink = exp2f(m - base);
-        float w = exp2f(s - base);
-        l = l * shrink + w;
-        m = top;
-        w = seen ? w * weight_scale : 0.f;
-        if (__any_sync(kFull, shrink != 1.f)) {
-#pragma unroll
-          for (int g = 0; g < GT; ++g) {
-            const float f = __shfl_sync(kFull, shrink, g << kShift);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[g][e] *= f;
+        for (int i = 0; i < N / 2; ++i) {
+          if (i < n) {
+            const bool upper = (lane & step) != 0;
+            const float keep = upper ? x[i + n] : x[i];
+            const float send = upper ? x[i] : x[i + n];
+            x[i] = keep + __shfl_xor_sync(kFull, send, step);
           }
         }
+      } else {
+        x[0] += __shfl_xor_sync(kFull, x[0], step);
+      }
+    }
+    const int token = (lane >> kShift) / GT;  // and head (lane >> kShift) % GT
+    const unsigned seen = *reinterpret_cast<const unsigned*>(at + kStageBytes - 4);
+    const bool in = (seen >> token & 1u) != 0;
+    float weight_scale = 1.f;
+    if constexpr (kCoded) {
+      x[0] *= reinterpret_cast<const float*>(at + kExtras)[token];
+      weight_scale = reinterpret_cast<const float*>(at + kExtras)[TB + token];
+    }
+    const float score = in ? x[0] : -CUDART_INF_F;
+    if (__any_sync(kFull, score > m + kSlack)) {
+      float top = score;
 #pragma unroll
-        for (int t = 0; t < TB; ++t)
+      for (int step = 16; step >= GT << kShift; step >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, step));
+      top = fmaxf(top, m);
+      const float shrink = exp2f(m - top);
+      m = top;
+      l *= shrink;
 #pragma unroll
-          for (int g = 0; g < GT; ++g) {
-            const float f = __shfl_sync(kFull, w, (t * GT + g) << kShift);
+      for (int g = 0; g < GT; ++g) {
+        const float f = __shfl_sync(kFull, shrink, g << kShift);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[g][e] = fmaf(f, v[t][e], o[g][e]);
-          }
+        for (int e = 0; e < E; ++e) o[g][e] *= f;
+      }
+    }
+    float w = exp2f(score - m);
+    l += w;
+    w = in ? w * weight_scale : 0.f;
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      float v[E];
+      row_of(v, at + kValues + t * kRowBytes);
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
+        const float f = __shfl_sync(kFull, w, (t * GT + g) << kShift);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[g][e] = fmaf(f, v[e], o[g][e]);
       }
     }
   }
 
   __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
-    float* buffer = reinterpret_cast<float*>(smem) + warp * GT * kPitch;
+    float* buffer = reinterpret_cast<float*>(smem + ring * kRingBytes + kPublish);
     // the sum of a head is spread over the lanes that own its scores of different tokens
 #pragma unroll
     for (int step = 16; step >= GT << kShift; step >>= 1) l += __shfl_xor_sync(kFull, l, step);
     const int mine = lane >> kShift;
-    if (mine < GT && (lane & ((1 << kShift) - 1)) == 0) ml[warp * GT + mine] = make_float2(m, l);
+    if (mine < GT && (lane & ((1 << kShift) - 1)) == 0) ml[ring * GT + mine] = make_float2(published_max(m), l);
 #pragma unroll
     for (int g = 0; g < GT; ++g)
 #pragma unroll
@@ -190,23 +254,35 @@ struct General {
   }
 };
 
+// Stages: about 100 KB per SM in flight for float32 rows.  CTAs: q and o take 2 GT E registers.
+template <typename T, int E, int GT, bool VEC>
+static Choice pick() {
+  constexpr int batch = (E == 8 || GT == 8 ? 4 : 8) * 64 * E * static_cast<int>(sizeof(T));  // bytes of a stage
+  constexpr int ctas = GT * E >= 32 || batch >= 8192 ? 2 : 3;
+  constexpr int stages = !VEC ? 2 : batch >= 8192 ? 3 : batch >= 4096 ? 4 : 6;
+  return made<General<T, E, GT, VEC, stages, ctas>>();
+}
+
 // Heads per item: the group if it is small; a group of more takes several items, whose second reading of
 // the keys and values comes from L2.  Features wider than 128 leave room for four heads in registers.
 template <typename T, bool VEC>
 static Choice choose(const AttentionArgs& a) {
-  if (a.dim > 128) return a.group == 1 ? made<General<T, 8, 1, VEC>>() : made<General<T, 8, 4, VEC>>();
-  if (a.dim > 64) {
-    if (a.group == 1) return made<General<T, 4, 1, VEC>>();
-    return a.group <= 4 ? made<General<T, 4, 4, VEC>>() : made<General<T, 4, 8, VEC>>();
+  if (a.dim > 128) return a.group == 1 ? pick<T, 8, 1, VEC>() : pick<T, 8, 4, VEC>();
+  if (a.dim > 64 || sizeof(T) == 1) {  // (the smallest asynchronous copy is 4 bytes)
+    if (a.group == 1) return pick<T, 4, 1, VEC>();
+    return a.group <= 4 ? pick<T, 4, 4, VEC>() : pick<T, 4, 8, VEC>();
   }
-  if (a.group == 1) return made<General<T, 2, 1, VEC>>();
-  return a.group <= 4 ? made<General<T, 2, 4, VEC>>() : made<General<T, 2, 8, VEC>>();
+  if constexpr (sizeof(T) > 1) {
+    if (a.group == 1) return pick<T, 2, 1, VEC>();
+    return a.group <= 4 ? pick<T, 2, 4, VEC>() : pick<T, 2, 8, VEC>();
+  }
+  return Choice{};
 }
 
 template <typename T>
 static Choice choose(const AttentionArgs& a) {
-  const int lane_features = a.dim > 128 ? 8 : a.dim > 64 ? 4 : 2;
-  const int item = TypeOf<T>::id == ASG_TYPE_F32 ? 4 : TypeOf<T>::coded ? 1 : 2;
+  const int item = static_cast<int>(sizeof(T));
+  const int lane_features = a.dim > 128 ? 8 : a.dim > 64 || item == 1 ? 4 : 2;
   const int bytes = lane_features * item < 16 ? lane_features * item : 16;
   if (a.dim % lane_features == 0 && rows_aligned(a.key, item, bytes) && rows_aligned(a.value, item, bytes))
     return choose<T, true>(a);

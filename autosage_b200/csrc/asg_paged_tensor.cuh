@@ -62,28 +62,6 @@ __device__ __forceinline__ void mma16816<F16>(float (&d)[4], const uint32_t (&a)
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// bytes of global memory into shared memory, zeros if !ok (nothing is read then)
-__device__ __forceinline__ void copy_async16(uint32_t to, const void* from, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_async4(uint32_t to, const void* from, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(ok ? 4 : 0) : "memory");
-}
-// 2^x and log2(x) of the hardware (results and arguments below the normal range count as 0)
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float fast_log2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Two floats as two 16-bit numbers (first in the low half), and what they lose.
 template <typename H> __device__ __forceinline__ uint32_t pack2(float a, float b, float& rest_a, float& rest_b);
 template <>
@@ -103,25 +81,31 @@ __device__ __forceinline__ uint32_t pack2<F16>(float a, float b, float& rest_a, 
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Bytes I and J of x, codes of type T, as two f16 numbers.
-constexpr uint32_t byte_selector(uint32_t i, uint32_t j) { return i | (4u << 4) | (j << 8) | (5u << 12); }
-template <int I, int J>
-__device__ __forceinline__ uint32_t decode_pair(uint32_t x, INT8) {
-  const uint32_t biased = __byte_perm(x ^ 0x80808080u, 0x64646464u, byte_selector(I, J));
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// Four codes as four f16 numbers: bytes 0 and 1 in `a`, 2 and 3 in `b`.
+__device__ __forceinline__ void decode_neighbours(uint32_t x, uint32_t& a, uint32_t& b, INT8) {
+  const uint32_t lifted = x ^ 0x80808080u;
+  const uint32_t u = __byte_perm(lifted, 0x64646464u, 0x4140), v = __byte_perm(lifted, 0x64646464u, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+  const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&u), bias), q = __hsub2(*reinterpret_cast<const __half2*>(&v), bias);
+  a = *reinterpret_cast<const uint32_t*>(&p);
+  b = *reinterpret_cast<const uint32_t*>(&q);
 }
-template <int I, int J>
-__device__ __forceinline__ uint32_t decode_pair(uint32_t x, E4M3) {
-  const uint32_t two = I == 0 && J == 1 ? x : I == 2 && J == 3 ? x >> 16 : __byte_perm(x, 0u, I | (J << 4) | 0x4400u);
-  const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(v.x) | (static_cast<uint32_t>(v.y) << 16);
+__device__ __forceinline__ void decode_neighbours(uint32_t x, uint32_t& a, uint32_t& b, E4M3) {
+  asm("{\n\t.reg .b16 low, high;\n\tmov.b32 {low, high}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, low;\n\tcvt.rn.f16x2.e4m3x2 %1, high;\n\t}"
+      : "=r"(a), "=r"(b) : "r"(x));
+}
+// Bytes 0 and 2 in `a`, 1 and 3 in `b`.
+template <typename T>
+__device__ __forceinline__ void decode_alternate(uint32_t x, uint32_t& a, uint32_t& b, T type) {
+  decode_neighbours(__byte_perm(x, 0u, 0x3120), a, b, type);
 }
 
-// T: type of the pages; DP: features, padded; NT: groups of 8 heads.
-template <typename T, int DP, int NT, int STAGES, int CTAS>
+// T: type of the pages; DP: features, padded; SHARE: warps that share a ring's tiles, each with 8 query heads of its own.
+template <typename T, int DP, int SHARE, int STAGES, int CTAS>
 struct Tensor {
-  static constexpr int kHeads = 8 * NT;
+  static constexpr int kThreads = kRings * SHARE * 32;
+  static constexpr int kHeads = 8 * SHARE;
   static constexpr int kCtasPerSm = CTAS;
   static constexpr int kStages = STAGES;
   static constexpr bool kCoded = TypeOf<T>::coded;
@@ -135,22 +119,32 @@ struct Tensor {
   static constexpr int kPitch = DP + 4;                             // of the published accumulators: no bank conflicts
   static constexpr int kPublish = (kStages - 1) * kStageBytes;      // the next piece's first copies go to the stages before it
   static constexpr int kNeed = kPublish + (kStageBytes > kHeads * kPitch * 4 ? kStageBytes : kHeads * kPitch * 4);
-  static constexpr int kWarpBytes = (kNeed + 127) / 128 * 128;
+  static constexpr int kRingBytes = (kNeed + 127) / 128 * 128;
   static constexpr int kSteps = DP / 16;
   using H = typename std::conditional<kCoded, F16, T>::type;        // type of the products
-  // f16 weights are held 2^14 above their value: the pieces of small weights stay clear of f16's smallest step
-  static constexpr float kLift = std::is_same<H, F16>::value ? 14.f : 0.f;
+  // f16 weights are held 2^8 above their value: the pieces of small weights stay clear of f16's smallest step, and
+  // with kSlack there are still two powers of two to its largest number
+  static constexpr float kLift = std::is_same<H, F16>::value ? 8.f : 0.f;
+  static_assert(kSlack + 8.f <= 15.f, "weights in f16");
 
-  uint32_t q[NT][kSteps][2];
-  float o[NT][kSteps][4];
-  float m[NT][2], l[NT][2];  // of heads 8 nt + 2 (lane % 4) + {0, 1}
-  float ref[NT][2];          // 8-bit pages: the accumulator's own reference, and what undoes the query's power of two
-  float unit[NT][2];
-  int lane, warp, dim_bytes;
-  uint32_t ring;             // shared address of the warp's region
+  uint32_t q[kSteps][2];
+  float o[kSteps][4];
+  float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1} of the warp's eight
+  float ref[2];      // 8-bit pages: the accumulator's own reference, and what undoes the query's power of two
+  float unit[2];
+  int lane, ring, part;
+  uint32_t base;     // shared address of the ring's region
+  Source s;
 
   __device__ __forceinline__ explicit Tensor(unsigned char* smem)
-      : lane(threadIdx.x & 31), warp(threadIdx.x >> 5), ring(smem_u32(smem) + warp * kWarpBytes) {}
+      : lane(threadIdx.x & 31), ring((threadIdx.x >> 5) % kRings), part((threadIdx.x >> 5) / kRings),
+        base(smem_u32(smem) + ring * kRingBytes) {}
+
+  // All lanes of the ring's warps.
+  __device__ __forceinline__ void meet() const {
+    if constexpr (SHARE == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + ring), "n"(SHARE * 32) : "memory");
+  }
 
   // Feature that a lane's register holds in step `step`: entry 0 or 1 of the pair `half`.
   static __device__ __forceinline__ int query_feature(int step, int lane, int half, int entry) {
@@ -183,176 +177,132 @@ struct Tensor {
   }
 
   __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
-    const int head = p.kv_head * a.group + p.sub * kHeads, heads = min(kHeads, a.group - p.sub * kHeads);
+    const int first = p.sub * kHeads + 8 * part, h = lane >> 2;  // of the group's heads
+    const uint16_t* from = static_cast<const uint16_t*>(a.q) + p.row * a.q_token_stride +
+                           (static_cast<long long>(p.kv_head) * a.group + first + h) * a.q_head_stride;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int h = 8 * nt + (lane >> 2);
-      const uint16_t* from = static_cast<const uint16_t*>(a.q) + p.row * a.q_token_stride + (head + h) * a.q_head_stride;
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        const uint2 x = load_query(a, from, h < heads, step, lane);
-        q[nt][step][0] = x.x;
-        q[nt][step][1] = x.y;
-      }
-      if constexpr (kCoded) {
-        const bool bf16 = a.type == ASG_TYPE_BF16;
-        float top = 0.f;
-#pragma unroll
-        for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float2 x = widen(q[nt][step][half], bf16);
-            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
-          }
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-        int power = (__float_as_int(top) >> 23) - 127;  // top in [2^power, 2^(power + 1)); 0 and infinity: as they are
-        power = power < -126 || power > 126 ? 0 : power;
-        const float down = __int_as_float((127 - power) << 23), up = __int_as_float((127 + power) << 23);
-#pragma unroll
-        for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float2 x = widen(q[nt][step][half], bf16);
-            float none0, none1;
-            q[nt][step][half] = pack2<F16>(x.x * down, x.y * down, none0, none1);
-          }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          unit[nt][i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
-          ref[nt][i] = -CUDART_INF_F;
-        }
-      }
+    for (int step = 0; step < kSteps; ++step) {
+      const uint2 x = load_query(a, from, first + h < a.group, step, lane);
+      q[step][0] = x.x;
+      q[step][1] = x.y;
+    }
+    if constexpr (kCoded) {
+      const bool bf16 = a.type == ASG_TYPE_BF16;
+      float top = 0.f;
 #pragma unroll
       for (int step = 0; step < kSteps; ++step)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][step][i] = 0.f;
-      m[nt][0] = m[nt][1] = -CUDART_INF_F;
-      l[nt][0] = l[nt][1] = 0.f;
+        for (int half = 0; half < 2; ++half) {
+          const float2 x = widen(q[step][half], bf16);
+          top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+      int power = (__float_as_int(top) >> 23) - 127;  // top in [2^power, 2^(power + 1)); 0 and infinity: as they are
+      power = power < -126 || power > 126 ? 0 : power;
+      const float down = __int_as_float((127 - power) << 23), up = __int_as_float((127 + power) << 23);
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float2 x = widen(q[step][half], bf16);
+          float none0, none1;
+          q[step][half] = pack2<F16>(x.x * down, x.y * down, none0, none1);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        unit[i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
+        ref[i] = kNoScore;
+      }
     }
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[step][i] = 0.f;
+    m[0] = m[1] = kNoScore;
+    l[0] = l[1] = 0.f;
   }
 
-  // Where the copies of a piece come from, and how far they are.  Lane l looks after token l % 16 of the next tile:
-  // the page of the table it lies in, its place there, and the page's id, loaded one tile ahead.
-  struct Source {
-    const char* keys;
-    const char* values;
-    const int64_t* ids;  // of the page that holds the piece's first token
-    long long page_bytes, token_bytes;
-    int kv_head, count, tile;
-    int nth, place;
-    int step_pages, step_place;  // kUnit tokens on
-    long long id;
-  };
-  Source s;
-  __device__ __forceinline__ void look_up() {
-    s.id = s.tile + (lane & (kTile - 1)) < s.count ? s.ids[s.nth] : -1;
-  }
+  // Copies the next tile to a stage; the ring's warps take every SHARE-th of its rows.
   __device__ __forceinline__ void issue(const AttentionArgs& a, int stage) {
     if (s.tile < s.count) {
-      const bool held = s.id >= 0 && s.id < a.n_pages;
+      const bool held = s.held(a);
       const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
       const long long offset = held ? s.id * s.page_bytes + s.place * s.token_bytes : 0;
       const int offset_low = static_cast<int>(offset), offset_high = static_cast<int>(offset >> 32);
-      const uint32_t base = ring + stage * kStageBytes;
+      const uint32_t at = base + stage * kStageBytes;
       constexpr int kLines = 32 / kChunks;  // rows that one copy of all lanes covers
-      const int chunk = lane % kChunks * 16, line0 = lane / kChunks;
-      const uint32_t to = base + line0 * kRowPitch + chunk;
-      const bool inside = chunk < dim_bytes;
+      const int chunk = lane % kChunks * 16, line0 = part * kLines + lane / kChunks;
+      const uint32_t to = at + line0 * kRowPitch + chunk;
+      const bool inside = chunk < a.dim * static_cast<int>(sizeof(T));
 #pragma unroll
-      for (int n = 0; n < kTile / kLines; ++n) {
-        const int line = n * kLines + line0;
+      for (int n = 0; n < kTile / kLines / SHARE; ++n) {
+        const int line = n * kLines * SHARE + line0;
         const unsigned low = static_cast<unsigned>(__shfl_sync(kFull, offset_low, line));
         const int high = __shfl_sync(kFull, offset_high, line);
         const long long from = (static_cast<long long>(high) << 32 | low) + chunk;
-        const bool ok = (seen >> line & 1u) != 0;
         // zeros for a token that is not seen and for features past the head's end
-        copy_async16(to + n * kLines * kRowPitch, s.keys + from, ok && inside);
-        copy_async16(to + n * kLines * kRowPitch + kValues, s.values + from, ok && inside);
+        const bool ok = inside && (seen >> line & 1u) != 0;
+        copy_async<16>(to + n * kLines * SHARE * kRowPitch, s.keys + from, ok);
+        copy_async<16>(to + n * kLines * SHARE * kRowPitch + kValues, s.values + from, ok);
       }
-      if constexpr (kCoded) {
-        const asg_page_pool& pool = lane < kTile ? a.key : a.value;
-        const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
-        if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
-        copy_async4(base + kExtras + lane * 4, from, held);
+      if (part == 0) {
+        if constexpr (kCoded) {
+          const asg_page_pool& pool = lane < kTile ? a.key : a.value;
+          const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
+          if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
+          copy_async<4>(at + kExtras + lane * 4, from, held);
+        }
+        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + kStageBytes - 4), "r"(seen) : "memory");
       }
-      if (lane == 0)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + kStageBytes - 4), "r"(seen) : "memory");
     }
     copy_commit();
-    s.tile += kUnit;
-    s.nth += s.step_pages;
-    s.place += s.step_place;
-    if (s.place >= a.page_size) {
-      s.place -= a.page_size;
-      ++s.nth;
-    }
-    look_up();
+    s.advance(a);
   }
 
   __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
-    __syncwarp();  // all lanes have left the stages
-    dim_bytes = a.dim * static_cast<int>(sizeof(T));
-    const int kv_head = p.kv_head;
-    const long long first = p.first(), last = p.last();
-    s.keys = static_cast<const char*>(a.key.data) + kv_head * a.key.head_stride * static_cast<int>(sizeof(T));
-    s.values = static_cast<const char*>(a.value.data) + kv_head * a.value.head_stride * static_cast<int>(sizeof(T));
-    s.page_bytes = a.key.page_stride * static_cast<int>(sizeof(T));
-    s.token_bytes = a.key.token_stride * static_cast<int>(sizeof(T));
-    s.kv_head = kv_head;
-    const unsigned page_size = static_cast<unsigned>(a.page_size);
-    const long long page0 = quotient(first, a.page_size);  // page arithmetic in 32 bits from here on
-    s.ids = a.col + p.span.pages_begin + page0;
-    s.count = static_cast<int>(last - first);
-    s.tile = warp * kTile;
-    const unsigned at = static_cast<unsigned>(first - page0 * a.page_size) + s.tile + (lane & (kTile - 1));
-    s.nth = static_cast<int>(at / page_size);
-    s.place = static_cast<int>(at % page_size);
-    s.step_pages = static_cast<int>(kUnit / page_size);
-    s.step_place = static_cast<int>(kUnit % page_size);
-    look_up();
+    s.start(a, p, ring, static_cast<int>(sizeof(T)));
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(a, i);
   }
 
   __device__ __forceinline__ void run(const AttentionArgs& a) {
-    const int tiles = s.count <= warp * kTile ? 0 : (s.count - warp * kTile + kUnit - 1) / kUnit;
+    const int tiles = s.count <= ring * kTile ? 0 : (s.count - ring * kTile + kUnit - 1) / kUnit;
     int stage = 0, fill = kStages - 1;
     for (int i = 0; i < tiles; ++i) {
       copy_wait<kStages - 2>();
-      __syncwarp();  // the tile has arrived for all lanes, and all have left the stage that is filled next
+      meet();  // the tile has arrived for all lanes, and all have left the stage that is filled next
       issue(a, fill);
-      compute(a, ring + stage * kStageBytes);
+      compute(a, base + stage * kStageBytes);
       stage = stage + 1 == kStages ? 0 : stage + 1;
       fill = fill + 1 == kStages ? 0 : fill + 1;
     }
     copy_wait<0>();
-    __syncwarp();
+    meet();
   }
 
-  // Largest score of one head in the tile (the lanes of equal lane % 4 hold its tokens), and the one before.
-  static __device__ __forceinline__ float largest_of_tile(float x0, float x1, float before) {
+  // Raises `before` to the largest score of a head in the tile (the lanes of equal lane % 4 hold its tokens) and
+  // returns the factor of what has been added up so far.
+  static __device__ __forceinline__ float raise(float x0, float x1, float& before) {
     float top = fmaxf(x0, x1);
     top = fmaxf(top, __shfl_xor_sync(kFull, top, 4));
     top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
     top = fmaxf(top, __shfl_xor_sync(kFull, top, 16));
-    return fmaxf(top, before);
+    top = fmaxf(top, before);
+    const float shrink = fast_exp2(before - top);
+    before = top;
+    return shrink;
   }
 
-  __device__ __forceinline__ void compute(const AttentionArgs& a, uint32_t base) {
-    const uint32_t line16 = base + (lane & 15) * kRowPitch + (lane >> 4) * 16;
-    float dots[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dots[nt][i] = 0.f;
+  __device__ __forceinline__ void compute(const AttentionArgs& a, uint32_t at) {
+    const uint32_t line16 = at + (lane & 15) * kRowPitch + (lane >> 4) * 16;
+    float dots[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (!kCoded) {
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         uint32_t k[4];
         ldmatrix_x4(k, line16 + step * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<H>(dots[nt], k, q[nt][step][0], q[nt][step][1]);
+        mma16816<H>(dots, k, q[step][0], q[step][1]);
       }
     } else {
 #pragma unroll
@@ -361,16 +311,16 @@ struct Tensor {
         ldmatrix_x4(c, line16 + step * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t k[4] = {decode_pair<0, 1>(c[2 * i], T{}), decode_pair<0, 1>(c[2 * i + 1], T{}),
-                                 decode_pair<2, 3>(c[2 * i], T{}), decode_pair<2, 3>(c[2 * i + 1], T{})};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<H>(dots[nt], k, q[nt][step + i][0], q[nt][step + i][1]);
+          uint32_t k[4];
+          decode_neighbours(c[2 * i], k[0], k[2], T{});
+          decode_neighbours(c[2 * i + 1], k[1], k[3], T{});
+          mma16816<H>(dots, k, q[step + i][0], q[step + i][1]);
         }
       }
     }
-    // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 8 nt + 2 (lane % 4) + {0, 1}
+    // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) + {0, 1}
     unsigned seen;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(base + kStageBytes - 4));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(at + kStageBytes - 4));
     float key_scale[2], value_log[2], value_sign[2];
     bool in[2];
 #pragma unroll
@@ -379,76 +329,69 @@ struct Tensor {
       in[t] = (seen >> token & 1u) != 0;
       if constexpr (kCoded) {
         float scale;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale[t]) : "r"(base + kExtras + token * 4));
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(base + kExtras + (kTile + token) * 4));
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale[t]) : "r"(at + kExtras + token * 4));
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(at + kExtras + (kTile + token) * 4));
         value_log[t] = fast_log2(fabsf(scale));
         value_sign[t] = copysignf(1.f, scale);
       }
     }
-    float shrink[NT][2];  // of the accumulator
-    bool moved = false;
-    uint32_t high[NT][2], low[NT][2];
+    float x[2][2], y[2][2];  // [token][head]: scores, and with the value scales
+    bool above = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[2][2];  // [token][head]
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float x[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if constexpr (kCoded) x[t] = in[t] ? dots[nt][2 * t + h] * (key_scale[t] * unit[nt][h]) : -CUDART_INF_F;
-          else x[t] = in[t] ? dots[nt][2 * t + h] * a.scale_log2 : -CUDART_INF_F;
-        }
-        const float top = largest_of_tile(x[0], x[1], m[nt][h]);
-        const float at = top == -CUDART_INF_F ? 0.f : top;
-        const float fade = fast_exp2(m[nt][h] - at);
-        m[nt][h] = top;
-        const float lifted = at - kLift;
-        w[0][h] = fast_exp2(x[0] - lifted);
-        w[1][h] = fast_exp2(x[1] - lifted);
-        l[nt][h] = l[nt][h] * fade + (w[0][h] + w[1][h]);
-        shrink[nt][h] = fade;
         if constexpr (kCoded) {
-          x[0] = in[0] ? x[0] + value_log[0] : -CUDART_INF_F;  // (a scale of 0 weighs nothing)
-          x[1] = in[1] ? x[1] + value_log[1] : -CUDART_INF_F;
-          const float new_ref = largest_of_tile(x[0], x[1], ref[nt][h]);
-          const float from = new_ref == -CUDART_INF_F ? 0.f : new_ref;
-          shrink[nt][h] = fast_exp2(ref[nt][h] - from);
-          ref[nt][h] = new_ref;
-          w[0][h] = value_sign[0] * fast_exp2(x[0] - (from - kLift));
-          w[1][h] = value_sign[1] * fast_exp2(x[1] - (from - kLift));
+          x[t][h] = in[t] ? dots[2 * t + h] * (key_scale[t] * unit[h]) : -CUDART_INF_F;
+          y[t][h] = in[t] ? x[t][h] + value_log[t] : -CUDART_INF_F;  // (a scale of 0 weighs nothing)
+          above = above || x[t][h] > m[h] + kSlack || y[t][h] > ref[h] + kSlack;
+        } else {
+          x[t][h] = in[t] ? dots[2 * t + h] * a.scale_log2 : -CUDART_INF_F;
+          above = above || x[t][h] > m[h] + kSlack;
         }
-        moved = moved || shrink[nt][h] != 1.f;
+      }
+    if (__any_sync(kFull, above)) {
+      float shrink[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        shrink[h] = raise(x[0][h], x[1][h], m[h]);
+        l[h] *= shrink[h];
+        if constexpr (kCoded) shrink[h] = raise(y[0][h], y[1][h], ref[h]);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float rest0, rest1, none0, none1;
-        high[nt][t] = transpose_8x8(pack2<H>(w[t][0], w[t][1], rest0, rest1));
-        low[nt][t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));
+      for (int step = 0; step < kSteps; ++step) {
+        o[step][0] *= shrink[0];
+        o[step][1] *= shrink[1];
+        o[step][2] *= shrink[0];
+        o[step][3] *= shrink[1];
       }
     }
-    if (__any_sync(kFull, moved)) {
+    float w[2][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          o[nt][step][0] *= shrink[nt][0];
-          o[nt][step][1] *= shrink[nt][1];
-          o[nt][step][2] *= shrink[nt][0];
-          o[nt][step][3] *= shrink[nt][1];
-        }
+      for (int t = 0; t < 2; ++t) w[t][h] = fast_exp2(x[t][h] - (m[h] - kLift));
+      l[h] += w[0][h] + w[1][h];
+      if constexpr (kCoded) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) w[t][h] = value_sign[t] * fast_exp2(y[t][h] - (ref[h] - kLift));
+      }
+    }
+    uint32_t high[2], low[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float rest0, rest1, none0, none1;
+      high[t] = transpose_8x8(pack2<H>(w[t][0], w[t][1], rest0, rest1));
+      low[t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));
     }
     if constexpr (!kCoded) {
-      const uint32_t line_v = base + kValues + ((lane & 7) + ((lane >> 4) << 3)) * kRowPitch + ((lane >> 3) & 1) * 16;
+      const uint32_t line_v = at + kValues + ((lane & 7) + ((lane >> 4) << 3)) * kRowPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         uint32_t v[4];
         ldmatrix_x4_trans(v, line_v + step * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816<H>(o[nt][step], v, high[nt][0], high[nt][1]);
-          mma16816<H>(o[nt][step], v, low[nt][0], low[nt][1]);
-        }
+        mma16816<H>(o[step], v, high[0], high[1]);
+        mma16816<H>(o[step], v, low[0], low[1]);
       }
     } else {
 #pragma unroll
@@ -457,64 +400,57 @@ struct Tensor {
         ldmatrix_x4_trans(c, line16 + kValues + step * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t v[4] = {decode_pair<0, 2>(c[2 * i], T{}), decode_pair<1, 3>(c[2 * i], T{}),
-                                 decode_pair<0, 2>(c[2 * i + 1], T{}), decode_pair<1, 3>(c[2 * i + 1], T{})};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<H>(o[nt][step + i], v, high[nt][0], high[nt][1]);
-            mma16816<H>(o[nt][step + i], v, low[nt][0], low[nt][1]);
-          }
+          uint32_t v[4];
+          decode_alternate(c[2 * i], v[0], v[1], T{});
+          decode_alternate(c[2 * i + 1], v[2], v[3], T{});
+          mma16816<H>(o[step + i], v, high[0], high[1]);
+          mma16816<H>(o[step + i], v, low[0], low[1]);
         }
       }
     }
   }
 
   __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
-    float* to = reinterpret_cast<float*>(smem + warp * kWarpBytes + kPublish);
-    constexpr float undo = kLift == 0.f ? 1.f : 1.f / 16384.f;
-    static_assert(kLift == 0.f || kLift == 14.f, "2^-kLift");
+    float* to = reinterpret_cast<float*>(smem + ring * kRingBytes + kPublish);
+    constexpr float undo = kLift == 0.f ? 1.f : 1.f / 256.f;
+    static_assert(kLift == 0.f || kLift == 8.f, "2^-kLift");
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int h = 0; h < 2; ++h) {
+      const int head = 8 * part + 2 * (lane & 3) + h;
+      float sum = l[h];
+      sum += __shfl_xor_sync(kFull, sum, 4);
+      sum += __shfl_xor_sync(kFull, sum, 8);
+      sum += __shfl_xor_sync(kFull, sum, 16);
+      if (lane < 4) ml[ring * kHeads + head] = make_float2(published_max(m[h]), sum * undo);
+      float back = undo;  // of the accumulator, to the maximum m
+      if (kCoded && ref[h] != kNoScore) back *= exp2f(ref[h] - m[h]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int head = 8 * nt + 2 * (lane & 3) + h;
-        float sum = l[nt][h];
-        sum += __shfl_xor_sync(kFull, sum, 4);
-        sum += __shfl_xor_sync(kFull, sum, 8);
-        sum += __shfl_xor_sync(kFull, sum, 16);
-        if (lane < 4) ml[warp * kHeads + head] = make_float2(m[nt][h], sum * undo);
-        float back = undo;  // of the accumulator, to the maximum m
-        if (kCoded && ref[nt][h] != -CUDART_INF_F) back *= exp2f(ref[nt][h] - m[nt][h]);
+      for (int step = 0; step < kSteps; ++step)
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            to[head * kPitch + output_feature(step, lane, half)] = o[nt][step][2 * half + h] * back;
-      }
+        for (int half = 0; half < 2; ++half) to[head * kPitch + output_feature(step, lane, half)] = o[step][2 * half + h] * back;
     }
   }
 };
 
-// Stages of a warp's ring and CTAs per SM.  About 100 KB of the cache in flight per SM cover the latency of
-// HBM at full rate; the rest of the 227 KB decides how many warps share the arithmetic.
-template <typename T, int NT>
+// Stages of a ring and CTAs per SM.  About 100 KB of the cache in flight per SM cover the latency of HBM at full
+// rate; the rest of the 227 KB decides how many warps share the arithmetic.
+template <typename T, int SHARE>
 inline Choice choose_padded(const AttentionArgs& a) {
   if constexpr (sizeof(T) == 1) {
-    if (a.dim <= 64) return made<Tensor<T, 64, NT, 4, 4>>();
-    if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 3>>();
-    return made<Tensor<T, 256, NT, NT == 1 ? 3 : 2, 2>>();
+    if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 4, SHARE == 1 ? 4 : 2>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 3, SHARE == 1 ? 3 : 2>>();
+    return made<Tensor<T, 256, SHARE, 3, SHARE == 1 ? 2 : 1>>();
   } else {
-    if (a.dim <= 64) return made<Tensor<T, 64, NT, 3, 3>>();
-    if (a.dim <= 128) return made<Tensor<T, 128, NT, 3, 2>>();
-    return made<Tensor<T, 256, NT, 3, 1>>();
+    if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 3, SHARE == 1 ? 3 : 2>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 3, 2>>();
+    return made<Tensor<T, 256, SHARE, 3, 1>>();
   }
 }
 template <typename T>
 inline Choice choose_tensor(const AttentionArgs& a) {
   const int item = static_cast<int>(sizeof(T));
   if (a.dim * item % 16 != 0 || !rows_aligned(a.key, item, 16) || !rows_aligned(a.value, item, 16)) return Choice{};
-  // one offset serves a token's key and value
-  if (a.key.page_stride != a.value.page_stride || a.key.token_stride != a.value.token_stride) return Choice{};
+  if (!a.same_strides) return Choice{};
   return a.group <= 8 ? choose_padded<T, 1>(a) : choose_padded<T, 2>(a);
 }
 
