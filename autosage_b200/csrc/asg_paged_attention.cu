@@ -19,23 +19,14 @@ constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs a, int ctas, int gt, bool sliced) {
   __shared__ float4 s_acc[kJoinThreads];
   __shared__ float2 s_stat[kJoinThreads];
-  __shared__ int s_last;
   const int c = blockIdx.x, tid = threadIdx.x;
   if (blockIdx.y == 0) clear_empty_rows(a, c, ctas);
   pdl_wait_for_primary();
   const int4 piece = a.pieces[c];
-  if (piece.z == 0) return;
+  const int n = min(piece.z, ctas - c);  // of its pieces; 0: none starts here
+  if (n <= 0) return;
   const int kv_head = piece.y / a.subgroups, sub = piece.y - kv_head * a.subgroups;
   const int heads = min(gt, a.group - sub * gt);
-  // the CTA that ends the item: the first after c whose first piece does not go on
-  if (tid == 0) s_last = ctas - 1;
-  __syncthreads();
-  for (int base = c + 1; base < ctas; base += kJoinThreads) {
-    const bool ends = base + tid < ctas && a.pieces[base + tid].w != 2;
-    if (ends) atomicMin(&s_last, base + tid);
-    if (__syncthreads_or(ends)) break;
-  }
-  const int n = s_last - c + 1;
   const int fours = (a.dim + 3) / 4;
   int slices = 1;  // a power of two
   while (sliced && slices * 2 * fours <= kJoinThreads) slices *= 2;

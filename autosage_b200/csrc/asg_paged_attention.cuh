@@ -58,10 +58,8 @@ struct AttentionArgs {
   int partial_pitch;
   float* partial;   // [G][2][GT][partial_pitch] accumulators of unfinished pieces
   float2* stats;    // [G][2][GT] their (m, l)
-  int4* pieces;     // [G] (row, item, starts an item it does not finish, 0 / 1 / 2: see below)
+  int4* pieces;     // [G] (row, item, n, 0): CTA c starts an item that it does not finish, cut into n pieces; n = 0: none
 };
-// pieces[c].w: how CTA c's first piece continues an earlier CTA's item: 0 it does not, 1 it ends it,
-// 2 the item goes on into CTA c + 1.
 
 size_t workspace_bytes_for(int ctas, int gt, int dim);
 
@@ -96,6 +94,7 @@ __device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
 struct Share {
   long long pos, end;   // entries of the list, flat
   long long row_begin;  // entry at which the row begins
+  long long per_cta;
   int row;
   int start;            // empty units before each item
 };
@@ -143,9 +142,9 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
   Share s;
   s.start = all_units * items_per_row > gridDim.x ? kStart : 0;
   const long long total = (all_units + s.start * all_rows) * items_per_row;
-  const long long per_cta = quotient(total + gridDim.x - 1, gridDim.x);
-  s.pos = per_cta * blockIdx.x;
-  s.end = s.pos + per_cta < total ? s.pos + per_cta : total;
+  s.per_cta = quotient(total + gridDim.x - 1, gridDim.x);
+  s.pos = s.per_cta * blockIdx.x;
+  s.end = s.pos + s.per_cta < total ? s.pos + s.per_cta : total;
   long long at = (units_before + s.start * rows_before) * items_per_row;
   if (s.pos < s.end && s.pos >= at && s.pos < at + (units + s.start * rows) * items_per_row) {  // exactly one thread
     long long r = r0;
@@ -285,6 +284,7 @@ __device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a, int blo
 struct Piece {
   RowSpan span;
   int row, item, kv_head, sub;
+  long long entry;          // of the list at which the item's tokens begin
   long long units, u0, u1;  // of the item; the piece's
   __device__ __forceinline__ long long first() const { return span.first + u0 * kUnit; }
   __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + u1 * kUnit; }
@@ -312,6 +312,7 @@ struct Walk {
       p.row = s.row;
       p.item = item;
       p.units = units;
+      p.entry = s.pos - at + s.start;
       p.u0 = at > s.start ? at - s.start : 0;
       p.u1 = to > s.start ? to - s.start : 0;
       s.pos += to - at;
@@ -435,23 +436,17 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       engine.publish(smem, ml);
       if (more) engine.query(a, next);
       __syncthreads();
-      int slot = -1;  // a whole item
-      if (now.u0 > 0) {
-        slot = 0;
-        left_over.w = now.u1 == now.units ? 1 : 2;
-      } else if (now.u1 < now.units) {
-        slot = 1;
-        left_over.x = now.row;
-        left_over.y = now.item;
-        left_over.z = 1;
-      }
+      const int slot = now.u0 > 0 ? 0 : now.u1 < now.units ? 1 : -1;  // -1: a whole item
+      if (slot == 1)  // the CTA of the item's last unit is the one of its last piece
+        left_over = make_int4(now.row, now.item,
+                              static_cast<int>(quotient(now.entry + now.units - 1, walk.s.per_cta)) - static_cast<int>(blockIdx.x) + 1, 0);
       store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o,
                                                                     Engine::kRingBytes / 4, ml);
       __syncthreads();  // the buffers are free again
       now = next;
     }
   }
-  if (threadIdx.x == 0) a.pieces[blockIdx.x] = left_over;
+  if (a.join && threadIdx.x == 0) a.pieces[blockIdx.x] = left_over;
   if (!a.join) clear_empty_rows(a, blockIdx.x, gridDim.x);  // otherwise the join kernel does, while this one runs
 }
 

@@ -127,6 +127,20 @@ def test_one_long_row_is_split_and_joined(kinds):
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, INT8)], ids=str)
+def test_shared_rows_of_every_size(kinds):
+    """Rows cut into two pieces, into dozens and into hundreds, one call after another on one workspace."""
+    cases = [Case((2, 1, 64, 16), kinds, lengths, seed=30 + i) for i, lengths in enumerate(
+        ([5000] * 10, [4000, 3000, 1, 0, 2500, 7001] * 3, [300] * 200, [40000], [2000 + 37 * r for r in range(24)], [64] * 7))]
+    expected = [case.expected() for case in cases]
+    first = [case.run() for case in cases]
+    for case, got, exact in zip(cases, first, expected):
+        case.check(got, exact)
+    for case, got in zip(reversed(cases), reversed(first)):
+        again = case.run()
+        assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
 @pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (BF16, E4M3)], ids=str)
 def test_many_short_rows(kinds):
     gen = torch.Generator().manual_seed(3)
