@@ -417,6 +417,7 @@ template <typename Engine>
 __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attention_kernel(const AttentionArgs a) {
   constexpr int GT = Engine::kHeads;
   extern __shared__ __align__(128) unsigned char smem[];
+  pdl_wait_for_primary();  // launched while the kernel before on the stream ends
   pdl_release_dependents();
   const int items_per_row = a.n_kv_heads * a.subgroups;
   Walk walk(a, items_per_row, locate_share<Engine::kThreads / 32>(a, items_per_row));
@@ -467,8 +468,7 @@ int launch_engine(const AttentionArgs& args, int ctas, cudaStream_t stream) {
       if (device < 64) known.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  kernel<<<ctas, Engine::kThreads, smem, stream>>>(args);
-  ASG_CUDA(cudaGetLastError());
+  ASG_CUDA(launch_overlapped(kernel, ctas, Engine::kThreads, static_cast<size_t>(smem), stream, args));
   return ASG_OK;
 }
 
