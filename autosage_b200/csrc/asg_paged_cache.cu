@@ -31,6 +31,53 @@ struct CacheArgs {
   asg_token_rows rows[2];   // key, value
   asg_page_pool pools[2];
   int page_size, n_heads, dim;
+  Divisor by_heads, by_page;
+  bool small;       // rows and slots have 31-bit numbers
+  bool same_rows;   // keys and values have the same strides: in the tokens, ...
+  bool same_pools;  // ... in the pages and scales
+};
+
+// Where row r = (token, head) of the tokens and its place in the pages lie, in elements; one offset each for key and
+// value.  `held`: the row's slot is inside the cache.
+struct RowPlace {
+  long long token_at[2], page_at[2], scale_at[2];
+  bool held;
+  __device__ __forceinline__ RowPlace(const CacheArgs& a, long long r, bool coded) {
+    long long token, page = 0, slot;
+    int head, place = 0;
+    if (a.small) {  // a handful of instructions instead of some hundreds
+      const unsigned t = divide(static_cast<unsigned>(r), a.by_heads);
+      token = t;
+      head = static_cast<int>(static_cast<unsigned>(r) - t * a.by_heads.d);
+      slot = a.slots[t];
+      held = slot >= 0 && slot < a.n_slots;
+      if (held) {
+        const unsigned p = divide(static_cast<unsigned>(slot), a.by_page);
+        page = p;
+        place = static_cast<int>(static_cast<unsigned>(slot) - p * a.by_page.d);
+      }
+    } else {
+      token = r / a.n_heads;
+      head = static_cast<int>(r - token * a.n_heads);
+      slot = a.slots[token];
+      held = slot >= 0 && slot < a.n_slots;
+      if (held) {
+        page = slot / a.page_size;
+        place = static_cast<int>(slot - page * a.page_size);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      token_at[w] = w == 1 && a.same_rows ? token_at[0] : token * a.rows[w].token_stride + head * a.rows[w].head_stride;
+      const asg_page_pool& pool = a.pools[w];
+      page_at[w] = w == 1 && a.same_pools ? page_at[0]
+                                          : page * pool.page_stride + place * pool.token_stride + head * pool.head_stride;
+      if (coded)
+        scale_at[w] = w == 1 && a.same_pools
+                          ? scale_at[0]
+                          : page * pool.scale_page_stride + head * pool.scale_head_stride + place * pool.scale_token_stride;
+    }
+  }
 };
 
 constexpr int kThreads = 256;
@@ -50,7 +97,7 @@ __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
 // The same by way of float64: a quotient of two 24-bit numbers is never nearer to a border between codes than
 // 2^-40 of itself without lying on it, so 53 bits decide; they are rounded to odd too.
 __device__ __noinline__ float quotient_by_double(float x, float s) {
-  const double wide = s == 0.f ? 0.0 : static_cast<double>(x) / static_cast<double>(s);
+  const double wide = static_cast<double>(x) / static_cast<double>(s);
   const float q = static_cast<float>(wide);
   const double rest = wide - static_cast<double>(q);
   const int bits = __float_as_int(q);
@@ -99,31 +146,33 @@ __device__ __forceinline__ void store_row(const Pack<T, lane_features(P)>& x, T*
   }
 }
 
-// The largest magnitude of a row, by its bits: a NaN is above everything and is not lost.
+// The largest magnitude of a row, by its bits: a NaN is above everything and is not lost.  All lanes of the warp.
 template <typename IN, int N>
-__device__ __forceinline__ float largest_of_row(const Pack<IN, N>& x, int group, unsigned mask) {
+__device__ __forceinline__ float largest_of_row(const Pack<IN, N>& x, int group) {
   if constexpr (sizeof(IN) == 2) {
     const uint32_t* two = reinterpret_cast<const uint32_t*>(x.v);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) top = __vmaxu2(top, two[i] & 0x7fff7fffu);
-    for (int o = group >> 1; o >= 1; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(mask, top, o));
+    for (int o = group >> 1; o >= 1; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(kFull, top, o));
     const uint16_t one = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
     return to_float(*reinterpret_cast<const IN*>(&one));
   } else {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x.v[i]) & 0x7fffffffu);
-    for (int o = group >> 1; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+    for (int o = group >> 1; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
     return __uint_as_float(top);
   }
 }
 
+// Codes and scale of a row whose largest magnitude is `top`.
 template <typename IN, typename CACHE, int N>
-__device__ __forceinline__ float quantise(const Pack<IN, N>& x, Pack<CACHE, N>& c, int group, unsigned mask) {
-  const float top = largest_of_row(x, group, mask), most = largest_code(CACHE{});
+__device__ __forceinline__ float quantise(const Pack<IN, N>& x, float top, Pack<CACHE, N>& c) {
+  const float most = largest_code(CACHE{});
   const float s = top / most;
-  uint32_t codes[N / 2];
+  float v[N];
+  to_floats(x, v);
   if (s > 0x1p-90f && s < 0x1p90f) {
     if constexpr (sizeof(IN) == 2) {
       float inv;
@@ -132,37 +181,35 @@ __device__ __forceinline__ float quantise(const Pack<IN, N>& x, Pack<CACHE, N>& 
       if (off != 0.f) {
         const float w = inv * (off > 0.f ? 1.f + 0x1p-21f : 1.f - 0x1p-21f);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-          codes[i] = nearest_codes(to_float(x.v[2 * i]) * w, to_float(x.v[2 * i + 1]) * w, CACHE{});
+        for (int i = 0; i < N; ++i) v[i] *= w;
       } else {
         inv = fmaf(fmaf(-inv, s, 1.f), inv, inv);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          float q[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float v = to_float(x.v[2 * i + j]), q0 = v * inv;
-            q[j] = fmaf(fmaf(-q0, s, v), inv, q0);
-          }
-          codes[i] = nearest_codes(q[0], q[1], CACHE{});
+        for (int i = 0; i < N; ++i) {
+          const float q0 = v[i] * inv;
+          v[i] = fmaf(fmaf(-q0, s, v[i]), inv, q0);
         }
       }
     } else {
       const float inv = 1.f / s;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i)
-        codes[i] = nearest_codes(quotient_to_odd(x.v[2 * i], s, inv), quotient_to_odd(x.v[2 * i + 1], s, inv), CACHE{});
+      for (int i = 0; i < N; ++i) v[i] = quotient_to_odd(v[i], s, inv);
     }
+  } else if (s == 0.f) {  // nothing but zeros, or values that a scale above 0 cannot reach
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
   } else {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i)
-      codes[i] = nearest_codes(quotient_by_double(to_float(x.v[2 * i]), s), quotient_by_double(to_float(x.v[2 * i + 1]), s), CACHE{});
+      for (int j = 0; j < N; ++j)  // (registers cannot be indexed)
+        if (j == i) v[j] = quotient_by_double(v[j], s);
+    }
   }
+  static_assert(N % 4 == 0, "codes are packed four at a time");
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint8_t code = static_cast<uint8_t>(codes[i / 2] >> (8 * (i & 1)));
-    c.v[i] = *reinterpret_cast<const CACHE*>(&code);
-  }
+  for (int i = 0; i < N / 4; ++i)
+    reinterpret_cast<uint32_t*>(c.v)[i] = nearest_codes(v[4 * i], v[4 * i + 1], CACHE{}) | nearest_codes(v[4 * i + 2], v[4 * i + 3], CACHE{}) << 16;
   return s;
 }
 
@@ -170,50 +217,32 @@ template <typename IN, typename CACHE, int P>
 __global__ void __launch_bounds__(kThreads) write_kernel(const CacheArgs a, int group) {
   constexpr int N = lane_features(P);
   const int lane = threadIdx.x & (group - 1);
-  const unsigned mask = group == 32 ? kFull : ((1u << group) - 1u) << ((threadIdx.x & 31) & ~(group - 1));
   const long long n_rows = a.n_tokens * a.n_heads;
   const int groups = kThreads / group;
   const long long stride = static_cast<long long>(gridDim.x) * groups;
-  for (long long r = static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group; r < n_rows; r += stride) {
-    long long token;
-    int head;
-    split_slot(r, a.n_heads, token, head);
-    const long long slot = a.slots[token];
-    if (slot < 0 || slot >= a.n_slots) continue;  // the whole group leaves together
+  // all groups of a block go round together (the largest of a row is found by the whole warp)
+  for (long long base = static_cast<long long>(blockIdx.x) * groups; base < n_rows; base += stride) {
+    const long long r = base + threadIdx.x / group;
+    const RowPlace at(a, r < n_rows ? r : n_rows - 1, TypeOf<CACHE>::coded);
+    const bool ok = r < n_rows && at.held;
     Pack<IN, N> x[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w)
-      load_row<P>(x[w], static_cast<const IN*>(a.rows[w].data) + token * a.rows[w].token_stride +
-                            head * a.rows[w].head_stride, lane, a.dim);
-    long long page;
-    int place;
-    split_slot(slot, a.page_size, page, place);
+      load_row<P>(x[w], static_cast<const IN*>(a.rows[w].data) + at.token_at[w], lane, ok ? a.dim : 0);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const asg_page_pool& pool = a.pools[w];
-      CACHE* to = static_cast<CACHE*>(pool.data) + page * pool.page_stride + place * pool.token_stride + head * pool.head_stride;
+      CACHE* to = static_cast<CACHE*>(a.pools[w].data) + at.page_at[w];
       if constexpr (!TypeOf<CACHE>::coded) {
-        store_row<P>(x[w], to, lane, a.dim);
+        store_row<P>(x[w], to, lane, ok ? a.dim : 0);
       } else {
+        const float top = largest_of_row(x[w], group);
         Pack<CACHE, N> c;
-        const float s = quantise(x[w], c, group, mask);
-        store_row<P>(c, to, lane, a.dim);
-        if (lane == 0)
-          pool.scales[page * pool.scale_page_stride + head * pool.scale_head_stride + place * pool.scale_token_stride] = s;
+        const float s = quantise(x[w], top, c);
+        store_row<P>(c, to, lane, ok ? a.dim : 0);
+        if (ok && lane == 0) a.pools[w].scales[at.scale_at[w]] = s;
       }
     }
   }
-}
-
-// Codes 2 i and 2 i + 1 of a pack as floats.
-template <int N>
-__device__ __forceinline__ float2 two_values(const Pack<E4M3, N>& c, int i) {
-  const uint16_t two = reinterpret_cast<const uint16_t*>(c.v)[i];
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
-}
-template <typename T, int N>
-__device__ __forceinline__ float2 two_values(const Pack<T, N>& c, int i) {
-  return make_float2(to_float(c.v[2 * i]), to_float(c.v[2 * i + 1]));
 }
 
 template <typename CACHE, typename OUT, int P>
@@ -224,36 +253,22 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int g
   const int groups = kThreads / group;
   const long long stride = static_cast<long long>(gridDim.x) * groups;
   for (long long r = static_cast<long long>(blockIdx.x) * groups + threadIdx.x / group; r < n_rows; r += stride) {
-    long long token;
-    int head;
-    split_slot(r, a.n_heads, token, head);
-    const long long slot = a.slots[token];
-    const bool held = slot >= 0 && slot < a.n_slots;
-    long long page = 0;
-    int place = 0;
-    if (held) split_slot(slot, a.page_size, page, place);
+    const RowPlace at(a, r, TypeOf<CACHE>::coded);
     Pack<CACHE, N> c[2];
     float s[2] = {1.f, 1.f};
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const asg_page_pool& pool = a.pools[w];
-      load_row<P>(c[w], static_cast<const CACHE*>(pool.data) + page * pool.page_stride + place * pool.token_stride +
-                            head * pool.head_stride, lane, held ? a.dim : 0);
-      if (TypeOf<CACHE>::coded && held)
-        s[w] = pool.scales[page * pool.scale_page_stride + head * pool.scale_head_stride + place * pool.scale_token_stride];
+      load_row<P>(c[w], static_cast<const CACHE*>(a.pools[w].data) + at.page_at[w], lane, at.held ? a.dim : 0);
+      if (TypeOf<CACHE>::coded && at.held) s[w] = a.pools[w].scales[at.scale_at[w]];
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
+      float v[N];
+      to_floats(c[w], v);
       Pack<OUT, N> x;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        float2 v = two_values(c[w], i);
-        if (TypeOf<CACHE>::coded) v = make_float2(v.x * s[w], v.y * s[w]);
-        x.v[2 * i] = from_float<OUT>(v.x);
-        x.v[2 * i + 1] = from_float<OUT>(v.y);
-      }
-      store_row<P>(x, static_cast<OUT*>(a.rows[w].data) + token * a.rows[w].token_stride + head * a.rows[w].head_stride,
-                   lane, a.dim);
+      for (int i = 0; i < N; ++i) x.v[i] = from_float<OUT>(TypeOf<CACHE>::coded ? v[i] * s[w] : v[i]);
+      store_row<P>(x, static_cast<OUT*>(a.rows[w].data) + at.token_at[w], lane, a.dim);
     }
   }
 }
@@ -338,6 +353,15 @@ static int fill_args(CacheArgs& a, const int64_t* slots, int64_t n_tokens, const
   a.page_size = static_cast<int>(page_size);
   a.n_heads = n_heads;
   a.dim = head_dim;
+  a.by_heads = divisor_of(static_cast<unsigned>(n_heads));
+  a.by_page = divisor_of(static_cast<unsigned>(page_size));
+  a.small = n_tokens * n_heads < (1ll << 31) && a.n_slots < (1ll << 31);
+  a.same_rows = key->token_stride == value->token_stride && key->head_stride == value->head_stride;
+  a.same_pools = key_pool->page_stride == value_pool->page_stride && key_pool->token_stride == value_pool->token_stride &&
+                 key_pool->head_stride == value_pool->head_stride &&
+                 key_pool->scale_page_stride == value_pool->scale_page_stride &&
+                 key_pool->scale_head_stride == value_pool->scale_head_stride &&
+                 key_pool->scale_token_stride == value_pool->scale_token_stride;
   return ASG_OK;
 }
 

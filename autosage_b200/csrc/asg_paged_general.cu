@@ -163,8 +163,7 @@ struct General {
 #pragma unroll
       for (int i = 0; i < kLaneBytes / 16; ++i) reinterpret_cast<uint4*>(p.v)[i] = reinterpret_cast<const uint4*>(from)[i];
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = to_float(p.v[e]);
+    to_floats(p, x);
   }
 
   __device__ __forceinline__ void compute(const unsigned char* at) {

@@ -26,8 +26,9 @@
 //   - a query head is multiplied by the power of two that brings its largest feature into [1, 2) (features
 //     below 2^-14 of that lose what lies below 2^-24 of it), undone in the factor of its scores;
 //   - the accumulator has a running reference of its own: with value scales c_t it holds
-//     sum_t 2^(s_t + log2 |c_t| - r) sign(c_t) code_t, r the largest s_t + log2 |c_t| so far, so its weights are
-//     at most 1 whatever the scales are, and 2^(r - m) brings it to the common maximum m in the end.
+//     sum_t 2^(s_t - r) c_t code_t, r about the largest s_t + log2 |c_t| so far, so its weights are small numbers
+//     whatever the scales are (the weight 2^(s_t - m) of the sum, times c_t 2^(m - r)); 2^(r - m) brings it to the
+//     common maximum m in the end.
 #pragma once
 
 #include "asg_paged_attention.cuh"
@@ -130,8 +131,9 @@ struct Tensor {
   uint32_t q[kSteps][2];
   float o[kSteps][4];
   float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1} of the warp's eight
-  float ref[2];      // 8-bit pages: the accumulator's own reference, and what undoes the query's power of two
-  float unit[2];
+  float ref[2];      // 8-bit pages: the accumulator's own reference r, 2^(m - r), ...
+  float to_ref[2];
+  float unit[2];     // ... and what undoes the query's power of two
   int lane, ring, part;
   uint32_t base;     // shared address of the ring's region
   Source s;
@@ -213,6 +215,7 @@ struct Tensor {
       for (int i = 0; i < 2; ++i) {
         unit[i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
         ref[i] = kNoScore;
+        to_ref[i] = 0.f;
       }
     }
 #pragma unroll
@@ -321,42 +324,55 @@ struct Tensor {
     // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) + {0, 1}
     unsigned seen;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(at + kStageBytes - 4));
-    float key_scale[2], value_log[2], value_sign[2];
-    bool in[2];
+    float key_scale[2] = {1.f, 1.f}, value_scale[2] = {1.f, 1.f};
+    if constexpr (kCoded) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int token = (lane >> 2) + 8 * t;
-      in[t] = (seen >> token & 1u) != 0;
-      if constexpr (kCoded) {
-        float scale;
+      for (int t = 0; t < 2; ++t) {
+        const int token = (lane >> 2) + 8 * t;
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale[t]) : "r"(at + kExtras + token * 4));
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(at + kExtras + (kTile + token) * 4));
-        value_log[t] = fast_log2(fabsf(scale));
-        value_sign[t] = copysignf(1.f, scale);
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value_scale[t]) : "r"(at + kExtras + (kTile + token) * 4));
       }
     }
-    float x[2][2], y[2][2];  // [token][head]: scores, and with the value scales
-    bool above = false;
+    float x[2][2], w[2][2], u[2][2];  // [token][head]: scores, weights of the sum and of the accumulator
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (kCoded) {
-          x[t][h] = in[t] ? dots[2 * t + h] * (key_scale[t] * unit[h]) : -CUDART_INF_F;
-          y[t][h] = in[t] ? x[t][h] + value_log[t] : -CUDART_INF_F;  // (a scale of 0 weighs nothing)
-          above = above || x[t][h] > m[h] + kSlack || y[t][h] > ref[h] + kSlack;
-        } else {
-          x[t][h] = in[t] ? dots[2 * t + h] * a.scale_log2 : -CUDART_INF_F;
-          above = above || x[t][h] > m[h] + kSlack;
+      for (int h = 0; h < 2; ++h) x[t][h] = dots[2 * t + h] * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
+    if (seen != 0xffffu) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if ((seen >> ((lane >> 2) + 8 * t) & 1u) == 0) x[t][0] = x[t][1] = -CUDART_INF_F;
+    }
+    auto weigh = [&]() {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          w[t][h] = fast_exp2(x[t][h] - (m[h] - kLift));
+          u[t][h] = kCoded ? w[t][h] * (value_scale[t] * to_ref[h]) : w[t][h];
         }
-      }
-    if (__any_sync(kFull, above)) {
+    };
+    weigh();
+    float largest = fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[1][0], w[1][1]));
+    if constexpr (kCoded) {
+      const float other = fmaxf(fmaxf(fabsf(u[0][0]), fabsf(u[0][1])), fmaxf(fabsf(u[1][0]), fabsf(u[1][1])));
+      largest = fmaxf(largest, other);
+    }
+    constexpr float limit = kLift == 0.f ? 64.f : 16384.f;
+    static_assert(kSlack == 6.f, "2^(kSlack + kLift)");
+    if (__any_sync(kFull, largest > limit)) {
       float shrink[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         shrink[h] = raise(x[0][h], x[1][h], m[h]);
         l[h] *= shrink[h];
-        if constexpr (kCoded) shrink[h] = raise(y[0][h], y[1][h], ref[h]);
+        if constexpr (kCoded) {
+          const float before = ref[h];
+          raise(x[0][h] + fast_log2(fabsf(value_scale[0])), x[1][h] + fast_log2(fabsf(value_scale[1])), ref[h]);
+          ref[h] = fmaxf(ref[h], m[h] - 120.f);  // 2^(m - r) stays a number; scales below 2^-120 count little
+          shrink[h] = fast_exp2(before - ref[h]);
+          to_ref[h] = fast_exp2(m[h] - ref[h]);
+        }
       }
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
@@ -365,23 +381,15 @@ struct Tensor {
         o[step][2] *= shrink[0];
         o[step][3] *= shrink[1];
       }
+      weigh();
     }
-    float w[2][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) w[t][h] = fast_exp2(x[t][h] - (m[h] - kLift));
-      l[h] += w[0][h] + w[1][h];
-      if constexpr (kCoded) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) w[t][h] = value_sign[t] * fast_exp2(y[t][h] - (ref[h] - kLift));
-      }
-    }
+    l[0] += w[0][0] + w[1][0];
+    l[1] += w[0][1] + w[1][1];
     uint32_t high[2], low[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float rest0, rest1, none0, none1;
-      high[t] = transpose_8x8(pack2<H>(w[t][0], w[t][1], rest0, rest1));
+      high[t] = transpose_8x8(pack2<H>(u[t][0], u[t][1], rest0, rest1));
       low[t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));
     }
     if constexpr (!kCoded) {
@@ -442,7 +450,7 @@ inline Choice choose_padded(const AttentionArgs& a) {
     return made<Tensor<T, 256, SHARE, 3, SHARE == 1 ? 2 : 1>>();
   } else {
     if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 3, SHARE == 1 ? 3 : 2>>();
-    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 3, 2>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, SHARE == 1 ? 2 : 3, 2>>();
     return made<Tensor<T, 256, SHARE, 3, 1>>();
   }
 }

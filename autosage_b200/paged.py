@@ -98,7 +98,8 @@ def _checking() -> bool:
 
 
 def _check_writable(name: str, tensor: Optional[torch.Tensor]) -> None:
-    if tensor is not None and any(step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
+    if tensor is not None and 0 in tensor.stride() and any(
+            step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
         raise ValueError(f"{name} is written and must not repeat memory (it has a stride of 0)")
 
 
