@@ -111,11 +111,15 @@ struct Tensor {
   static constexpr int kStages = STAGES;
   static constexpr bool kCoded = TypeOf<T>::coded;
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
-  static constexpr int kRowPitch = kRowBytes + 16;
+  // Rows of 128 bytes: the 16-byte piece c of row r lies at place c ^ (r mod 8); other rows are padded by 16 bytes.
+  // Either way the eight rows that an ldmatrix reads lie in different banks.
+  static constexpr bool kSwizzled = kRowBytes == 128;
+  static constexpr int kRowPitch = kSwizzled ? kRowBytes : kRowBytes + 16;
   static constexpr int kChunks = kRowBytes / 16;                    // 16-byte pieces of a row
   static constexpr int kValues = kTile * kRowPitch;                 // offset of the V tile in a stage
   static constexpr int kExtras = 2 * kTile * kRowPitch;             // then the scales (key, value), then the mask of seen tokens
-  static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * kTile * 4 : 0) + 4 + 15) / 16 * 16;
+  static constexpr int kStageAlign = kSwizzled ? 128 : 16;
+  static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * kTile * 4 : 0) + 4 + kStageAlign - 1) / kStageAlign * kStageAlign;
   static constexpr int kDim = DP;
   static constexpr int kPitch = DP + 4;                             // of the published accumulators: no bank conflicts
   static constexpr int kPublish = (kStages - 1) * kStageBytes;      // the next piece's first copies go to the stages before it
@@ -130,6 +134,8 @@ struct Tensor {
 
   uint32_t q[kSteps][2];
   float o[kSteps][4];
+  float dots[2][4];         // the next tile's scores, in two chains of products
+  uint32_t high[2], low[2]; // this tile's weights
   float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1} of the warp's eight
   float ref[2];      // 8-bit pages: the accumulator's own reference r, 2^(m - r), ...
   float to_ref[2];
@@ -236,7 +242,7 @@ struct Tensor {
       const uint32_t at = base + stage * kStageBytes;
       constexpr int kLines = 32 / kChunks;  // rows that one copy of all lanes covers
       const int chunk = lane % kChunks * 16, line0 = part * kLines + lane / kChunks;
-      const uint32_t to = at + line0 * kRowPitch + chunk;
+      const uint32_t to = at + line0 * kRowPitch, piece = kSwizzled ? chunk ^ (line0 & 7) * 16 : chunk;
       const bool inside = chunk < a.dim * static_cast<int>(sizeof(T));
 #pragma unroll
       for (int n = 0; n < kTile / kLines / SHARE; ++n) {
@@ -246,8 +252,10 @@ struct Tensor {
         const long long from = (static_cast<long long>(high) << 32 | low) + chunk;
         // zeros for a token that is not seen and for features past the head's end
         const bool ok = inside && (seen >> line & 1u) != 0;
-        copy_async<16>(to + n * kLines * SHARE * kRowPitch, s.keys + from, ok);
-        copy_async<16>(to + n * kLines * SHARE * kRowPitch + kValues, s.values + from, ok);
+        const int rows = n * kLines * SHARE;  // (a multiple of a power of two above line0: the bits do not meet)
+        const uint32_t here = to + rows * kRowPitch + (kSwizzled ? piece ^ (rows & 7) * 16 : piece);
+        copy_async<16>(here, s.keys + from, ok);
+        copy_async<16>(here + kValues, s.values + from, ok);
       }
       if (part == 0) {
         if constexpr (kCoded) {
@@ -269,16 +277,38 @@ struct Tensor {
     for (int i = 0; i < kStages - 1; ++i) issue(a, i);
   }
 
+  // A tile's products with V are issued together with the next tile's products with K: the two chains hide one
+  // another's latency, and the softmax between them is all that a warp ever waits for alone.
   __device__ __forceinline__ void run(const AttentionArgs& a) {
     const int tiles = s.count <= ring * kTile ? 0 : (s.count - ring * kTile + kUnit - 1) / kUnit;
-    int stage = 0, fill = kStages - 1;
-    for (int i = 0; i < tiles; ++i) {
+    if (tiles > 0) {
       copy_wait<kStages - 2>();
-      meet();  // the tile has arrived for all lanes, and all have left the stage that is filled next
-      issue(a, fill);
-      compute(a, base + stage * kStageBytes);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-      fill = fill + 1 == kStages ? 0 : fill + 1;
+      meet();  // the first tile has arrived for all lanes
+      clear_dots();
+#pragma unroll
+      for (int step = 0; step < kSteps; step += 2) score_steps(base, step);
+      int stage = 0, fill = kStages - 1;
+#pragma unroll 1
+      for (int i = 1; i < tiles; ++i) {
+        const uint32_t at = base + stage * kStageBytes;
+        weigh(a, at);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        const uint32_t next = base + stage * kStageBytes;
+        copy_wait<kStages - 3>();
+        meet();  // the next tile has arrived, and all lanes have left the one before this, whose stage is filled now
+        issue(a, fill);
+        fill = fill + 1 == kStages ? 0 : fill + 1;
+        clear_dots();
+#pragma unroll
+        for (int step = 0; step < kSteps; step += 2) {
+          score_steps(next, step);
+          value_steps(at, step);
+        }
+      }
+      const uint32_t at = base + stage * kStageBytes;
+      weigh(a, at);
+#pragma unroll
+      for (int step = 0; step < kSteps; step += 2) value_steps(at, step);
     }
     copy_wait<0>();
     meet();
@@ -297,30 +327,68 @@ struct Tensor {
     return shrink;
   }
 
-  __device__ __forceinline__ void compute(const AttentionArgs& a, uint32_t at) {
-    const uint32_t line16 = at + (lane & 15) * kRowPitch + (lane >> 4) * 16;
-    float dots[4] = {0.f, 0.f, 0.f, 0.f};
+  // Where piece `chunk` (0 or 1) of a row of the tile at `tile` lies, and the piece `bytes` (a multiple of 32) further on.
+  static __device__ __forceinline__ uint32_t place_of(uint32_t tile, int row, int chunk) {
+    return tile + row * kRowPitch + (kSwizzled ? (chunk ^ (row & 7)) * 16 : chunk * 16);
+  }
+  static __device__ __forceinline__ uint32_t further(uint32_t place, int bytes) { return kSwizzled ? place ^ bytes : place + bytes; }
+
+  __device__ __forceinline__ void clear_dots() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dots[0][i] = dots[1][i] = 0.f;
+  }
+
+  // Steps `step` and `step` + 1 (32 features) of the products with K.
+  __device__ __forceinline__ void score_steps(uint32_t at, int step) {
+    const uint32_t line = place_of(at, lane & 15, lane >> 4);
     if constexpr (!kCoded) {
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t k[4];
-        ldmatrix_x4(k, line16 + step * 32);
-        mma16816<H>(dots, k, q[step][0], q[step][1]);
+        ldmatrix_x4(k, further(line, (step + i) * 32));
+        mma16816<H>(dots[i], k, q[step + i][0], q[step + i][1]);
       }
     } else {
+      uint32_t c[4];
+      ldmatrix_x4(c, further(line, step * 16));
 #pragma unroll
-      for (int step = 0; step < kSteps; step += 2) {  // 32 bytes: two steps of 16 features
-        uint32_t c[4];
-        ldmatrix_x4(c, line16 + step * 16);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t k[4];
-          decode_neighbours(c[2 * i], k[0], k[2], T{});
-          decode_neighbours(c[2 * i + 1], k[1], k[3], T{});
-          mma16816<H>(dots, k, q[step + i][0], q[step + i][1]);
-        }
+      for (int i = 0; i < 2; ++i) {
+        uint32_t k[4];
+        decode_neighbours(c[2 * i], k[0], k[2], T{});
+        decode_neighbours(c[2 * i + 1], k[1], k[3], T{});
+        mma16816<H>(dots[i], k, q[step + i][0], q[step + i][1]);
       }
     }
+  }
+
+  // The same features of the products with V.
+  __device__ __forceinline__ void value_steps(uint32_t at, int step) {
+    if constexpr (!kCoded) {
+      const uint32_t line = place_of(at + kValues, (lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t v[4];
+        ldmatrix_x4_trans(v, further(line, (step + i) * 32));
+        mma16816<H>(o[step + i], v, high[0], high[1]);
+        mma16816<H>(o[step + i], v, low[0], low[1]);
+      }
+    } else {
+      const uint32_t line = place_of(at + kValues, lane & 15, lane >> 4);
+      uint32_t c[4];
+      ldmatrix_x4_trans(c, further(line, step * 16));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t v[4];
+        decode_alternate(c[2 * i], v[0], v[1], T{});
+        decode_alternate(c[2 * i + 1], v[2], v[3], T{});
+        mma16816<H>(o[step + i], v, high[0], high[1]);
+        mma16816<H>(o[step + i], v, low[0], low[1]);
+      }
+    }
+  }
+
+  // Scores to weights.
+  __device__ __forceinline__ void weigh(const AttentionArgs& a, uint32_t at) {
     // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) + {0, 1}
     unsigned seen;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(at + kStageBytes - 4));
@@ -337,13 +405,13 @@ struct Tensor {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) x[t][h] = dots[2 * t + h] * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
+      for (int h = 0; h < 2; ++h) x[t][h] = (dots[0][2 * t + h] + dots[1][2 * t + h]) * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
     if (seen != 0xffffu) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if ((seen >> ((lane >> 2) + 8 * t) & 1u) == 0) x[t][0] = x[t][1] = -CUDART_INF_F;
     }
-    auto weigh = [&]() {
+    auto powers = [&]() {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -352,7 +420,7 @@ struct Tensor {
           u[t][h] = kCoded ? w[t][h] * (value_scale[t] * to_ref[h]) : w[t][h];
         }
     };
-    weigh();
+    powers();
     float largest = fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[1][0], w[1][1]));
     if constexpr (kCoded) {
       const float other = fmaxf(fmaxf(fabsf(u[0][0]), fabsf(u[0][1])), fmaxf(fabsf(u[1][0]), fabsf(u[1][1])));
@@ -381,40 +449,15 @@ struct Tensor {
         o[step][2] *= shrink[0];
         o[step][3] *= shrink[1];
       }
-      weigh();
+      powers();
     }
     l[0] += w[0][0] + w[1][0];
     l[1] += w[0][1] + w[1][1];
-    uint32_t high[2], low[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float rest0, rest1, none0, none1;
       high[t] = transpose_8x8(pack2<H>(u[t][0], u[t][1], rest0, rest1));
       low[t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));
-    }
-    if constexpr (!kCoded) {
-      const uint32_t line_v = at + kValues + ((lane & 7) + ((lane >> 4) << 3)) * kRowPitch + ((lane >> 3) & 1) * 16;
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        uint32_t v[4];
-        ldmatrix_x4_trans(v, line_v + step * 32);
-        mma16816<H>(o[step], v, high[0], high[1]);
-        mma16816<H>(o[step], v, low[0], low[1]);
-      }
-    } else {
-#pragma unroll
-      for (int step = 0; step < kSteps; step += 2) {
-        uint32_t c[4];
-        ldmatrix_x4_trans(c, line16 + kValues + step * 16);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t v[4];
-          decode_alternate(c[2 * i], v[0], v[1], T{});
-          decode_alternate(c[2 * i + 1], v[2], v[3], T{});
-          mma16816<H>(o[step + i], v, high[0], high[1]);
-          mma16816<H>(o[step + i], v, low[0], low[1]);
-        }
-      }
     }
   }
 
@@ -440,17 +483,18 @@ struct Tensor {
   }
 };
 
-// Stages of a ring and CTAs per SM.  About 100 KB of the cache in flight per SM cover the latency of HBM at full
-// rate; the rest of the 227 KB decides how many warps share the arithmetic.
+// Stages of a ring and CTAs per SM: one tile is being used with the next, the others are in flight.  16-bit pages want
+// few bytes in flight (64 x 8192 float16 of 8 x 128 take 174 us with one tile of each ring under way, 183 with two:
+// more requests from more rows spoil the order in which HBM serves them), 8-bit pages want the warps for their decoding.
 template <typename T, int SHARE>
 inline Choice choose_padded(const AttentionArgs& a) {
   if constexpr (sizeof(T) == 1) {
     if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 4, SHARE == 1 ? 4 : 2>>();
-    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 3, SHARE == 1 ? 3 : 2>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 4, SHARE == 1 ? 3 : 2>>();
     return made<Tensor<T, 256, SHARE, 3, SHARE == 1 ? 2 : 1>>();
   } else {
-    if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 3, SHARE == 1 ? 3 : 2>>();
-    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, SHARE == 1 ? 2 : 3, 2>>();
+    if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 3, SHARE == 1 ? 4 : 2>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 3, 2>>();
     return made<Tensor<T, 256, SHARE, 3, 1>>();
   }
 }
