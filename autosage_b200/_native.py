@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import weakref
 from collections import OrderedDict
 from pathlib import Path
@@ -33,22 +34,6 @@ _INT = ctypes.c_int
 _U32 = ctypes.c_uint
 _SZ = ctypes.c_size_t
 _F32 = ctypes.c_float
-
-class PagePool(ctypes.Structure):
-    """``asg_page_pool`` of the header."""
-
-    _fields_ = [("data", _P), ("scales", _P), ("page_stride", _I64), ("token_stride", _I64), ("head_stride", _I64),
-                ("scale_page_stride", _I64), ("scale_head_stride", _I64), ("scale_token_stride", _I64)]
-
-
-class TokenRows(ctypes.Structure):
-    """``asg_token_rows`` of the header."""
-
-    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
-
-
-_ROWS = ctypes.POINTER(TokenRows)
-_POOL = ctypes.POINTER(PagePool)
 
 # name -> (restype, argtypes); kept in the order of the header
 SIGNATURES = {
@@ -87,13 +72,11 @@ SIGNATURES = {
     "asg_spmm_csr_split_noalloc": (_INT, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _I64, _P]),
     "asg_static_max_rows": (_I64, []),
     "asg_static_status": (_INT, [_P, _P, _P]),
-    "asg_paged_cache_write": (_INT, [_P, _I64, _ROWS, _ROWS, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
-    "asg_paged_cache_read": (_INT, [_P, _I64, _ROWS, _ROWS, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _INT, _P]),
+    "asg_paged_cache_write": (_INT, [ctypes.c_char_p]),
+    "asg_paged_cache_read": (_INT, [ctypes.c_char_p]),
     "asg_paged_attention_workspace_bytes": (_SZ, [_INT, _INT, _INT]),
-    "asg_paged_attention": (_INT, [_P, _P, _P, _I64, _I64, _ROWS, _P, _P, _POOL, _POOL, _I64, _I64, _INT, _INT, _INT, _F32, _I64,
-                                   _INT, _INT, _P, _SZ, _P]),
+    "asg_paged_attention": (_INT, [ctypes.c_char_p]),
 }
-
 
 # ASG_TYPE_* of the header
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
@@ -459,42 +442,41 @@ def conv_fused(crow: torch.Tensor, col: torch.Tensor, val: Optional[torch.Tensor
     return workspace
 
 
-def _page_pool(pages: torch.Tensor, scales: Optional[torch.Tensor]) -> PagePool:
-    page, token, head, _ = pages.stride()
-    if scales is None:
-        return PagePool(pages.data_ptr(), None, page, token, head)
-    return PagePool(pages.data_ptr(), scales.data_ptr(), page, token, head, *scales.stride())
-
-
-def _token_rows(rows: torch.Tensor) -> TokenRows:
-    token, head, _ = rows.stride()
-    return TokenRows(rows.data_ptr(), token, head)
-
-
-# One token is little work for the GPU, so the calls of the paged cache are made of little else than the call:
-# the stream's handle as torch's own extensions take it, no keyword arguments, no copies of what is at hand.
+# One token is little work for the GPU, so the calls of the paged cache are made of little else than the call: their
+# arguments are one C struct of 8-byte fields, packed in one go, and the stream's handle is taken as torch's own
+# extensions take it.
+_CACHE_ARGS = struct.Struct("=" + 31 * "q")               # asg_paged_cache_args
+_ATTENTION_ARGS = struct.Struct("=" + 34 * "q" + "d3q")   # asg_paged_attention_args
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _page_pool(pages: torch.Tensor, scales: Optional[torch.Tensor]) -> tuple:
+    """asg_page_pool: data, scales, strides of pages, tokens and heads, strides of the scales."""
+    page, token, head, _ = pages.stride()
+    if scales is None:
+        return pages.data_ptr(), 0, page, token, head, 0, 0, 0
+    return (pages.data_ptr(), scales.data_ptr(), page, token, head, *scales.stride())
+
+
+def _paged_cache_args(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> bytes:
+    key_token, key_head, _ = key.stride()
+    value_token, value_head, _ = value.stride()
+    return _CACHE_ARGS.pack(slots.data_ptr(), slots.numel(), key.data_ptr(), key_token, key_head, value.data_ptr(), value_token,
+                            value_head, *_page_pool(key_pages, key_scales), *_page_pool(value_pages, value_scales),
+                            *key_pages.shape, TYPES[key.dtype], TYPES[key_pages.dtype], _raw_stream(key_pages.device.index))
+
+
 def paged_cache_write(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
     """Rows [T, heads, dim] into the slots of the pages, quantised where the pages are 8-bit."""
-    n_pages, page_size, heads, dim = key_pages.shape
-    code = library().asg_paged_cache_write(
-        slots.data_ptr(), slots.numel(), _token_rows(key), _token_rows(value), _page_pool(key_pages, key_scales),
-        _page_pool(value_pages, value_scales), n_pages, page_size, heads, dim, TYPES[key.dtype], TYPES[key_pages.dtype],
-        _raw_stream(key_pages.device.index))
+    code = library().asg_paged_cache_write(_paged_cache_args(slots, key, value, key_pages, value_pages, key_scales, value_scales))
     if code:
         check(code)
 
 
 def paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> None:
     """The slots of the pages into the rows key and value."""
-    n_pages, page_size, heads, dim = key_pages.shape
-    code = library().asg_paged_cache_read(
-        slots.data_ptr(), slots.numel(), _token_rows(key), _token_rows(value), _page_pool(key_pages, key_scales),
-        _page_pool(value_pages, value_scales), n_pages, page_size, heads, dim, TYPES[key.dtype], TYPES[key_pages.dtype],
-        _raw_stream(key_pages.device.index))
+    code = library().asg_paged_cache_read(_paged_cache_args(slots, key, value, key_pages, value_pages, key_scales, value_scales))
     if code:
         check(code)
 
@@ -509,15 +491,15 @@ def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages,
     """out[r] = softmax(scale q_r K^T) V over the tokens of row r's pages (one query token a row)."""
     n_rows, n_heads, head_dim = query.shape
     n_pages, page_size, n_kv_heads, _ = key_pages.shape
+    q_token, q_head, _ = query.stride()
     device = query.device
     stream = _raw_stream(device.index)
-    need = _paged_attention_bytes(n_heads, n_kv_heads, head_dim)
-    workspace = _scratch_on(device, device.index, stream, need)
-    code = library().asg_paged_attention(
-        crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), _token_rows(query), out.data_ptr(),
-        None if lse is None else lse.data_ptr(), _page_pool(key_pages, key_scales), _page_pool(value_pages, value_scales),
-        n_pages, page_size, n_heads, n_kv_heads, head_dim, scale, window, TYPES[query.dtype], TYPES[key_pages.dtype],
-        workspace.data_ptr(), workspace.numel(), stream)
+    workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(n_heads, n_kv_heads, head_dim))
+    code = library().asg_paged_attention(_ATTENTION_ARGS.pack(
+        crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), query.data_ptr(), q_token, q_head,
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), *_page_pool(key_pages, key_scales),
+        *_page_pool(value_pages, value_scales), n_pages, page_size, n_heads, n_kv_heads, head_dim, window,
+        TYPES[query.dtype], TYPES[key_pages.dtype], scale, workspace.data_ptr(), workspace.numel(), stream))
     if code:
         check(code)
 

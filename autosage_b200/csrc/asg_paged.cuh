@@ -14,9 +14,9 @@ namespace paged {
 
 constexpr int kMaxDim = 256;
 
-inline bool is_wide(int type) { return type == ASG_TYPE_F32 || type == ASG_TYPE_BF16 || type == ASG_TYPE_F16; }
-inline bool is_coded(int type) { return type == ASG_TYPE_E4M3 || type == ASG_TYPE_INT8; }
-inline int type_bytes(int type) { return type == ASG_TYPE_F32 ? 4 : is_coded(type) ? 1 : 2; }
+inline bool is_wide(int64_t type) { return type == ASG_TYPE_F32 || type == ASG_TYPE_BF16 || type == ASG_TYPE_F16; }
+inline bool is_coded(int64_t type) { return type == ASG_TYPE_E4M3 || type == ASG_TYPE_INT8; }
+inline int type_bytes(int64_t type) { return type == ASG_TYPE_F32 ? 4 : is_coded(type) ? 1 : 2; }
 
 // Whether every row of a pool, or of token rows, starts on a multiple of `bytes`.
 inline bool rows_aligned(const asg_page_pool& p, int item, int bytes) {
@@ -47,8 +47,8 @@ inline Divisor divisor_of(unsigned d) {
 }
 
 // The checks that the three entry points share (host).
-inline int check_pools(const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
-                       int64_t page_size, int n_heads, int head_dim, int wide_type, int cache_type) {
+inline int check_pools(const asg_page_pool& key_pool, const asg_page_pool& value_pool, int64_t n_pages,
+                       int64_t page_size, int64_t n_heads, int64_t head_dim, int64_t wide_type, int64_t cache_type) {
   ASG_REQUIRE(is_wide(wide_type), ASG_EINVAL, "the type of the tokens must be float32, bfloat16 or float16");
   ASG_REQUIRE(is_wide(cache_type) || is_coded(cache_type), ASG_EINVAL, "unknown type of the pages");
   ASG_REQUIRE(n_pages >= 0 && page_size >= 1 && n_heads >= 1 && head_dim >= 1, ASG_EINVAL,
@@ -56,11 +56,10 @@ inline int check_pools(const asg_page_pool* key_pool, const asg_page_pool* value
   ASG_REQUIRE(head_dim <= kMaxDim, ASG_ERANGE, "the paged kernels hold at most 256 features per head");
   ASG_REQUIRE(n_pages <= 2147483647ll && page_size < (1ll << 30) && n_heads <= 65535, ASG_ERANGE,
               "n_pages, page_size or n_heads exceeds the kernel index range");
-  ASG_REQUIRE(key_pool != nullptr && value_pool != nullptr, ASG_EINVAL, "key_pool and value_pool must not be null");
-  ASG_REQUIRE(n_pages == 0 || (key_pool->data != nullptr && value_pool->data != nullptr), ASG_EINVAL,
+  ASG_REQUIRE(n_pages == 0 || (key_pool.data != nullptr && value_pool.data != nullptr), ASG_EINVAL,
               "the pages must not be null");
   if (is_coded(cache_type))
-    ASG_REQUIRE(n_pages == 0 || (key_pool->scales != nullptr && value_pool->scales != nullptr), ASG_EINVAL,
+    ASG_REQUIRE(n_pages == 0 || (key_pool.scales != nullptr && value_pool.scales != nullptr), ASG_EINVAL,
                 "8-bit pages need scales");
   return ASG_OK;
 }

@@ -97,73 +97,74 @@ size_t asg_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head
   if (n_heads < 1 || n_kv_heads < 1 || head_dim < 1 || head_dim > kMaxDim || n_heads % n_kv_heads != 0) return 0;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) cudaGetLastError();
-  return workspace_bytes_for(asg::sm_count(device) * kMaxCtasPerSm, 16, head_dim);
+  return workspace_bytes_for(asg::sm_count(device) * kMaxCtasPerSm, n_heads / n_kv_heads > 8 ? 16 : 8, head_dim);
 }
 
-int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* lengths, int64_t n_rows, int64_t n_cols,
-                        const asg_token_rows* q, void* out, float* lse, const asg_page_pool* key_pool,
-                        const asg_page_pool* value_pool, int64_t n_pages, int64_t page_size, int n_heads,
-                        int n_kv_heads, int head_dim, float scale, int64_t window, int type, int cache_type,
-                        void* workspace, size_t workspace_bytes, void* stream_ptr) {
+int asg_paged_attention(const asg_paged_attention_args* args) {
   using namespace asg;
   using namespace asg::paged;
-  if (int rc = check_pools(key_pool, value_pool, n_pages, page_size, n_kv_heads, head_dim, type, cache_type)) return rc;
+  ASG_REQUIRE(args != nullptr, ASG_EINVAL, "args must not be null");
+  const int64_t n_rows = args->n_rows, n_cols = args->n_cols, n_heads = args->n_heads, n_kv_heads = args->n_kv_heads;
+  const int64_t page_size = args->page_size, head_dim = args->head_dim, type = args->type, cache_type = args->cache_type;
+  if (int rc = check_pools(args->key_pool, args->value_pool, args->n_pages, page_size, n_kv_heads, head_dim, type, cache_type))
+    return rc;
   ASG_REQUIRE(is_coded(cache_type) || cache_type == type, ASG_EINVAL,
               "the pages must have the type of the query or an 8-bit type");
   ASG_REQUIRE(n_heads >= 1 && n_heads <= 65535 && n_heads % n_kv_heads == 0, ASG_EINVAL,
               "n_heads must be a positive multiple of n_kv_heads");
   ASG_REQUIRE(n_rows >= 0 && n_cols >= 0, ASG_EINVAL, "sizes must be non-negative");
   ASG_REQUIRE(n_rows < 2147483647ll - 2048 && n_cols < (1ll << 31), ASG_ERANGE, "n_rows or n_cols exceeds the kernel index range");
-  ASG_REQUIRE(window >= 0, ASG_EINVAL, "window must not be negative");
+  ASG_REQUIRE(args->window >= 0, ASG_EINVAL, "window must not be negative");
   if (n_rows == 0) return ASG_OK;
-  ASG_REQUIRE(crow != nullptr && lengths != nullptr && q != nullptr && q->data != nullptr && out != nullptr, ASG_EINVAL,
+  ASG_REQUIRE(args->crow != nullptr && args->lengths != nullptr && args->q.data != nullptr && args->out != nullptr, ASG_EINVAL,
               "crow, lengths, query and out must not be null");
-  ASG_REQUIRE(n_cols == 0 || col != nullptr, ASG_EINVAL, "col must not be null");
-  ASG_REQUIRE(workspace != nullptr, ASG_EWORKSPACE, "workspace pointer is null");
-  ASG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, ASG_EWORKSPACE, "workspace must be 256-byte aligned");
-  DeviceGuard guard(out);
+  ASG_REQUIRE(n_cols == 0 || args->col != nullptr, ASG_EINVAL, "col must not be null");
+  ASG_REQUIRE(args->workspace != nullptr, ASG_EWORKSPACE, "workspace pointer is null");
+  ASG_REQUIRE((reinterpret_cast<uintptr_t>(args->workspace) & 255u) == 0, ASG_EWORKSPACE, "workspace must be 256-byte aligned");
+  DeviceGuard guard(args->out);
   ASG_CUDA(guard.status);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  cudaStream_t stream = static_cast<cudaStream_t>(args->stream);
   AttentionArgs a = {};
-  a.crow = crow;
-  a.col = col;
-  a.lengths = lengths;
-  a.q = q->data;
-  a.out = out;
-  a.lse = lse;
-  a.key = *key_pool;
-  a.value = *value_pool;
-  a.q_token_stride = q->token_stride;
-  a.q_head_stride = q->head_stride;
+  a.crow = args->crow;
+  a.col = args->col;
+  a.lengths = args->lengths;
+  a.q = args->q.data;
+  a.out = args->out;
+  a.lse = args->lse;
+  a.key = args->key_pool;
+  a.value = args->value_pool;
+  a.q_token_stride = args->q.token_stride;
+  a.q_head_stride = args->q.head_stride;
   a.n_cols = n_cols;
-  a.n_pages = n_pages;
-  a.window = window;
+  a.n_pages = args->n_pages;
+  a.window = args->window;
   a.n_rows = static_cast<int>(n_rows);
   a.page_size = static_cast<int>(page_size);
-  a.n_heads = n_heads;
-  a.n_kv_heads = n_kv_heads;
-  a.dim = head_dim;
-  a.group = n_heads / n_kv_heads;
-  a.type = type;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.q_pairs = rows_aligned(*q, type_bytes(type), 8);
+  a.n_heads = static_cast<int>(n_heads);
+  a.n_kv_heads = static_cast<int>(n_kv_heads);
+  a.dim = static_cast<int>(head_dim);
+  a.group = static_cast<int>(n_heads / n_kv_heads);
+  a.type = static_cast<int>(type);
+  a.scale_log2 = static_cast<float>(args->scale * 1.4426950408889634);
+  a.q_pairs = rows_aligned(args->q, type_bytes(type), 8);
   a.same_strides = a.key.page_stride == a.value.page_stride && a.key.token_stride == a.value.token_stride;
-  a.out_vector = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-  a.partial_pitch = (head_dim + 3) / 4 * 4;
+  a.out_vector = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+  a.partial_pitch = static_cast<int>((head_dim + 3) / 4 * 4);
   // 16-bit queries run on the tensor cores wherever 16-byte copies can fetch the rows; float32 queries, whose
   // products have to keep 24 bits, and everything else on the FMA pipe
-  Choice choice = is_coded(cache_type) ? choose_tensor8(a, cache_type) : choose_tensor16(a, cache_type);
-  if (choice.launch == nullptr) choice = choose_general(a, cache_type);
+  const int pages_type = static_cast<int>(cache_type);
+  Choice choice = is_coded(cache_type) ? choose_tensor8(a, pages_type) : choose_tensor16(a, pages_type);
+  if (choice.launch == nullptr) choice = choose_general(a, pages_type);
   a.subgroups = (a.group + choice.gt - 1) / choice.gt;
   // no more CTAs than units there can be (every row may end in a partly filled one)
-  const int64_t items = static_cast<int64_t>(n_kv_heads) * a.subgroups;
+  const int64_t items = n_kv_heads * a.subgroups;
   const double most = (static_cast<double>(n_cols) * page_size / kUnit + n_rows) * items;
   int ctas = sm_count(guard.target) * choice.ctas_per_sm;
   if (most < ctas) ctas = most < 1 ? 1 : static_cast<int>(most);
   const size_t records = static_cast<size_t>(ctas) * 2 * choice.gt;
-  ASG_REQUIRE(workspace_bytes >= workspace_bytes_for(ctas, choice.gt, head_dim), ASG_EWORKSPACE,
+  ASG_REQUIRE(args->workspace_bytes >= workspace_bytes_for(ctas, choice.gt, a.dim), ASG_EWORKSPACE,
               "workspace is smaller than asg_paged_attention_workspace_bytes");
-  char* at = static_cast<char*>(workspace);
+  char* at = static_cast<char*>(args->workspace);
   a.pieces = reinterpret_cast<int4*>(at);
   at += align256(static_cast<size_t>(ctas) * sizeof(int4));
   a.stats = reinterpret_cast<float2*>(at);

@@ -95,6 +95,7 @@ struct Share {
   long long pos, end;   // entries of the list, flat
   long long row_begin;  // entry at which the row begins
   long long per_cta;
+  RowSpan span;         // of that row
   int row;
   int start;            // empty units before each item
 };
@@ -104,6 +105,7 @@ template <int WARPS>
 __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
   __shared__ long long warp_units[WARPS], warp_rows[WARPS];
   __shared__ long long found_begin;
+  __shared__ RowSpan found_span;
   __shared__ int found_row;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_thread = (a.n_rows + WARPS * 32 - 1) / (WARPS * 32);
@@ -148,18 +150,21 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
   long long at = (units_before + s.start * rows_before) * items_per_row;
   if (s.pos < s.end && s.pos >= at && s.pos < at + (units + s.start * rows) * items_per_row) {  // exactly one thread
     long long r = r0;
-    for (; r + 1 < a.n_rows; ++r) {
-      const long long n = row_span(a, static_cast<int>(r)).units();
-      const long long here = n > 0 ? (n + s.start) * items_per_row : 0;
+    RowSpan span = row_span(a, static_cast<int>(r));
+    while (r + 1 < a.n_rows) {
+      const long long n = span.units(), here = n > 0 ? (n + s.start) * items_per_row : 0;
       if (s.pos < at + here) break;
       at += here;
+      span = row_span(a, static_cast<int>(++r));
     }
     found_row = static_cast<int>(r);
     found_begin = at;
+    found_span = span;
   }
   __syncthreads();
   s.row = found_row;
   s.row_begin = found_begin;
+  s.span = found_span;
   return s;
 }
 
@@ -298,7 +303,7 @@ struct Walk {
   int item, items_per_row;
   __device__ __forceinline__ Walk(const AttentionArgs& a, int items, const Share& share) : s(share), items_per_row(items) {
     if (s.pos >= s.end) return;
-    span = row_span(a, s.row);
+    span = s.span;
     units = span.units();
     item = static_cast<int>(quotient(s.pos - s.row_begin, units + s.start));
     at = s.pos - s.row_begin - item * (units + s.start);
@@ -365,7 +370,6 @@ struct Source {
     look_up();
   }
   __device__ __forceinline__ void look_up() { id = tile + (lane_id() & (kTile - 1)) < count ? ids[nth] : -1; }
-  __device__ __forceinline__ bool held(const AttentionArgs& a) const { return id >= 0 && id < a.n_pages; }
   __device__ __forceinline__ void advance(const AttentionArgs& a) {
     tile += kUnit;
     nth += step_pages;
@@ -407,8 +411,9 @@ __device__ __forceinline__ float published_max(float m) { return m == kNoScore ?
 
 // The kernel around an Engine, which computes one ring's part of a piece:
 //   Engine(smem)                      once
-//   start(a, piece)                   begins to fetch the piece's tokens; the part of the piece before is still unpublished
-//   query(a, piece)                   takes the query and clears the accumulators
+//   fetch(a, piece)                   loads the piece's query; the part of the piece before is still unpublished
+//   start(a, piece)                   begins to copy the piece's tokens
+//   query(a)                          takes the query and clears the accumulators
 //   run(a)                            the ring's tiles
 //   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + ring * kRingBytes +
 //                                     kPublish, which no copy of a started piece writes before run()
@@ -427,15 +432,19 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
     Engine engine(smem);
     const float* o = reinterpret_cast<const float*>(smem + Engine::kPublish);
     float2* ml = reinterpret_cast<float2*>(smem + kRings * Engine::kRingBytes);
+    engine.fetch(a, now);
     engine.start(a, now);
-    engine.query(a, now);
+    engine.query(a);
     for (bool more = true; more;) {
       engine.run(a);
       Piece next;
       more = walk.next(a, next);
-      if (more) engine.start(a, next);
+      if (more) {
+        engine.fetch(a, next);
+        engine.start(a, next);
+      }
       engine.publish(smem, ml);
-      if (more) engine.query(a, next);
+      if (more) engine.query(a);
       __syncthreads();
       const int slot = now.u0 > 0 ? 0 : now.u1 < now.units ? 1 : -1;  // -1: a whole item
       if (slot == 1)  // the CTA of the item's last unit is the one of its last piece

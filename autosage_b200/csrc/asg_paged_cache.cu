@@ -334,34 +334,32 @@ static int launch_read(const CacheArgs& a, int out_type, cudaStream_t stream) {
   return launch_read<CACHE, F16>(a, stream);
 }
 
-static int fill_args(CacheArgs& a, const int64_t* slots, int64_t n_tokens, const asg_token_rows* key,
-                     const asg_token_rows* value, const asg_page_pool* key_pool, const asg_page_pool* value_pool,
-                     int64_t n_pages, int64_t page_size, int n_heads, int head_dim, int wide_type, int cache_type) {
-  if (int rc = check_pools(key_pool, value_pool, n_pages, page_size, n_heads, head_dim, wide_type, cache_type)) return rc;
-  ASG_REQUIRE(n_tokens >= 0, ASG_EINVAL, "n_tokens must be non-negative");
-  ASG_REQUIRE(n_tokens <= (1ll << 40), ASG_ERANGE, "n_tokens exceeds the kernel index range");
-  ASG_REQUIRE(key != nullptr && value != nullptr, ASG_EINVAL, "key and value must not be null");
-  ASG_REQUIRE(n_tokens == 0 || (slots != nullptr && key->data != nullptr && value->data != nullptr), ASG_EINVAL,
-              "slots, key and value must not be null");
-  a.slots = slots;
-  a.n_tokens = n_tokens;
-  a.n_slots = n_pages * page_size;
-  a.rows[0] = *key;
-  a.rows[1] = *value;
-  a.pools[0] = *key_pool;
-  a.pools[1] = *value_pool;
-  a.page_size = static_cast<int>(page_size);
-  a.n_heads = n_heads;
-  a.dim = head_dim;
-  a.by_heads = divisor_of(static_cast<unsigned>(n_heads));
-  a.by_page = divisor_of(static_cast<unsigned>(page_size));
-  a.small = n_tokens * n_heads < (1ll << 31) && a.n_slots < (1ll << 31);
-  a.same_rows = key->token_stride == value->token_stride && key->head_stride == value->head_stride;
-  a.same_pools = key_pool->page_stride == value_pool->page_stride && key_pool->token_stride == value_pool->token_stride &&
-                 key_pool->head_stride == value_pool->head_stride &&
-                 key_pool->scale_page_stride == value_pool->scale_page_stride &&
-                 key_pool->scale_head_stride == value_pool->scale_head_stride &&
-                 key_pool->scale_token_stride == value_pool->scale_token_stride;
+static int fill_args(CacheArgs& a, const asg_paged_cache_args* args) {
+  ASG_REQUIRE(args != nullptr, ASG_EINVAL, "args must not be null");
+  const asg_page_pool &key = args->key_pool, &value = args->value_pool;
+  if (int rc = check_pools(key, value, args->n_pages, args->page_size, args->n_heads, args->head_dim, args->token_type,
+                           args->cache_type)) return rc;
+  ASG_REQUIRE(args->n_tokens >= 0, ASG_EINVAL, "n_tokens must be non-negative");
+  ASG_REQUIRE(args->n_tokens <= (1ll << 40), ASG_ERANGE, "n_tokens exceeds the kernel index range");
+  ASG_REQUIRE(args->n_tokens == 0 || (args->slots != nullptr && args->key.data != nullptr && args->value.data != nullptr),
+              ASG_EINVAL, "slots, key and value must not be null");
+  a.slots = args->slots;
+  a.n_tokens = args->n_tokens;
+  a.n_slots = args->n_pages * args->page_size;
+  a.rows[0] = args->key;
+  a.rows[1] = args->value;
+  a.pools[0] = key;
+  a.pools[1] = value;
+  a.page_size = static_cast<int>(args->page_size);
+  a.n_heads = static_cast<int>(args->n_heads);
+  a.dim = static_cast<int>(args->head_dim);
+  a.by_heads = divisor_of(static_cast<unsigned>(a.n_heads));
+  a.by_page = divisor_of(static_cast<unsigned>(a.page_size));
+  a.small = a.n_tokens * a.n_heads < (1ll << 31) && a.n_slots < (1ll << 31);
+  a.same_rows = a.rows[0].token_stride == a.rows[1].token_stride && a.rows[0].head_stride == a.rows[1].head_stride;
+  a.same_pools = key.page_stride == value.page_stride && key.token_stride == value.token_stride &&
+                 key.head_stride == value.head_stride && key.scale_page_stride == value.scale_page_stride &&
+                 key.scale_head_stride == value.scale_head_stride && key.scale_token_stride == value.scale_token_stride;
   return ASG_OK;
 }
 
@@ -370,43 +368,39 @@ static int fill_args(CacheArgs& a, const int64_t* slots, int64_t n_tokens, const
 
 extern "C" {
 
-int asg_paged_cache_write(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key, const asg_token_rows* value,
-                          const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
-                          int64_t page_size, int n_heads, int head_dim, int in_type, int cache_type, void* stream_ptr) {
+int asg_paged_cache_write(const asg_paged_cache_args* args) {
   using namespace asg;
   using namespace asg::paged;
   CacheArgs a;
-  if (int rc = fill_args(a, slots, n_tokens, key, value, key_pool, value_pool, n_pages, page_size, n_heads, head_dim,
-                         in_type, cache_type)) return rc;
-  ASG_REQUIRE(is_coded(cache_type) || cache_type == in_type, ASG_EINVAL,
+  if (int rc = fill_args(a, args)) return rc;
+  ASG_REQUIRE(is_coded(args->cache_type) || args->cache_type == args->token_type, ASG_EINVAL,
               "the pages must have the type of the tokens or an 8-bit type");
-  if (n_tokens == 0 || n_pages == 0) return ASG_OK;
+  if (a.n_tokens == 0 || a.n_slots == 0) return ASG_OK;
   DeviceGuard guard(a.pools[0].data);
   ASG_CUDA(guard.status);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (in_type == ASG_TYPE_F32) return launch_write<F32>(a, cache_type, stream);
-  if (in_type == ASG_TYPE_BF16) return launch_write<BF16>(a, cache_type, stream);
+  cudaStream_t stream = static_cast<cudaStream_t>(args->stream);
+  const int cache_type = static_cast<int>(args->cache_type);
+  if (args->token_type == ASG_TYPE_F32) return launch_write<F32>(a, cache_type, stream);
+  if (args->token_type == ASG_TYPE_BF16) return launch_write<BF16>(a, cache_type, stream);
   return launch_write<F16>(a, cache_type, stream);
 }
 
-int asg_paged_cache_read(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key, const asg_token_rows* value,
-                         const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
-                         int64_t page_size, int n_heads, int head_dim, int out_type, int cache_type, void* stream_ptr) {
+int asg_paged_cache_read(const asg_paged_cache_args* args) {
   using namespace asg;
   using namespace asg::paged;
   CacheArgs a;
-  if (int rc = fill_args(a, slots, n_tokens, key, value, key_pool, value_pool, n_pages, page_size, n_heads, head_dim,
-                         out_type, cache_type)) return rc;
-  if (n_tokens == 0) return ASG_OK;
+  if (int rc = fill_args(a, args)) return rc;
+  if (a.n_tokens == 0) return ASG_OK;
   DeviceGuard guard(a.rows[0].data);
   ASG_CUDA(guard.status);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  switch (cache_type) {
-    case ASG_TYPE_F32: return launch_read<F32>(a, out_type, stream);
-    case ASG_TYPE_BF16: return launch_read<BF16>(a, out_type, stream);
-    case ASG_TYPE_F16: return launch_read<F16>(a, out_type, stream);
-    case ASG_TYPE_E4M3: return launch_read<E4M3>(a, out_type, stream);
-    default: return launch_read<INT8>(a, out_type, stream);
+  cudaStream_t stream = static_cast<cudaStream_t>(args->stream);
+  const int token_type = static_cast<int>(args->token_type);
+  switch (args->cache_type) {
+    case ASG_TYPE_F32: return launch_read<F32>(a, token_type, stream);
+    case ASG_TYPE_BF16: return launch_read<BF16>(a, token_type, stream);
+    case ASG_TYPE_F16: return launch_read<F16>(a, token_type, stream);
+    case ASG_TYPE_E4M3: return launch_read<E4M3>(a, token_type, stream);
+    default: return launch_read<INT8>(a, token_type, stream);
   }
 }
 

@@ -45,39 +45,50 @@ struct General {
   int batch;                              // of the tile that is copied next
   bool held;                              // of the lane's token of that tile
   long long key_offset, value_offset;     // in bytes
+  long long scale_id;
+  int scale_place;
 
   __device__ __forceinline__ explicit General(unsigned char* smem)
       : lane(threadIdx.x & 31), ring(threadIdx.x >> 5), region(smem + (threadIdx.x >> 5) * kRingBytes) {}
 
   static __device__ __forceinline__ int feature(int lane, int e) { return VEC ? lane * E + e : e * 32 + lane; }
 
-  __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
+  __device__ __forceinline__ void fetch(const AttentionArgs& a, const Piece& p) {
     const int head = p.kv_head * a.group + p.sub * GT, heads = min(GT, a.group - p.sub * GT);
 #pragma unroll
     for (int g = 0; g < GT; ++g)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int d = feature(lane, e);
-        q[g][e] = g < heads && d < a.dim
-                      ? load_wide(a.q, p.row * a.q_token_stride + (head + g) * a.q_head_stride + d, a.type) * a.scale_log2
-                      : 0.f;
+        q[g][e] = g < heads && d < a.dim ? load_wide(a.q, p.row * a.q_token_stride + (head + g) * a.q_head_stride + d, a.type) : 0.f;
+      }
+  }
+
+  __device__ __forceinline__ void query(const AttentionArgs& a) {
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        q[g][e] *= a.scale_log2;
         o[g][e] = 0.f;
       }
     m = kNoScore;
     l = 0.f;
   }
 
-  // Where the lane's token of the tile lies.
-  __device__ __forceinline__ void locate(const AttentionArgs& a) {
+  // Where the lane's token of a tile lies.
+  __device__ __forceinline__ void locate(const AttentionArgs& a, long long id, int place) {
     constexpr int item = static_cast<int>(sizeof(T));
-    held = s.held(a);
-    key_offset = held ? s.id * s.page_bytes + s.place * s.token_bytes : 0;
-    value_offset = held ? s.id * a.value.page_stride * item + s.place * a.value.token_stride * item : 0;
+    held = id >= 0 && id < a.n_pages;
+    key_offset = held ? id * s.page_bytes + place * s.token_bytes : 0;
+    value_offset = held ? id * a.value.page_stride * item + place * a.value.token_stride * item : 0;
+    scale_id = id;
+    scale_place = place;
   }
 
-  // Copies the next batch to a stage.
-  __device__ __forceinline__ void issue(const AttentionArgs& a, int stage) {
-    if (s.tile + batch * TB < s.count) {
+  // Copies batch `batch` of the tile at token `tile`, located before, to a stage.
+  __device__ __forceinline__ void copy(const AttentionArgs& a, int stage, int tile, int batch) {
+    if (tile + batch * TB < s.count) {
       const unsigned seen = __ballot_sync(kFull, held) >> (batch * TB) & ((1u << TB) - 1u);
       unsigned char* at = region + stage * kStageBytes;
       const int key_low = static_cast<int>(key_offset), key_high = static_cast<int>(key_offset >> 32);
@@ -115,26 +126,33 @@ struct General {
         if (token >= 0 && token < TB) {
           const asg_page_pool& pool = lane < kTile ? a.key : a.value;
           const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
-          if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
+          if (held) from += scale_id * pool.scale_page_stride + scale_place * pool.scale_token_stride;
           copy_async<4>(smem_u32(at + kExtras) + ((lane < kTile ? 0 : TB) + token) * 4, from, held);
         }
       }
       if (lane == 0) *reinterpret_cast<unsigned*>(at + kStageBytes - 4) = seen;
     }
     copy_commit();
-    if (++batch == kBatches) {
-      batch = 0;
-      s.advance(a);
-      locate(a);
-    }
   }
 
   __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
     s.start(a, p, ring, static_cast<int>(sizeof(T)));
-    batch = 0;
-    locate(a);
-#pragma unroll 1
-    for (int i = 0; i < kStages - 1; ++i) issue(a, i);
+    constexpr int kLast = (kStages - 1) / kBatches;  // tile of the batch after the first copies
+    const int first = s.tile;
+    long long id[kLast + 1];  // the page ids of all tiles are asked for before the first is needed
+    int place[kLast + 1];
+#pragma unroll
+    for (int i = 0; i <= kLast; ++i) {
+      id[i] = s.id;
+      place[i] = s.place;
+      if (i < kLast) s.advance(a);
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i % kBatches == 0) locate(a, id[i / kBatches], place[i / kBatches]);
+      copy(a, i, first + i / kBatches * kUnit, i % kBatches);
+    }
+    batch = (kStages - 1) % kBatches;
   }
 
   __device__ __forceinline__ void run(const AttentionArgs& a) {
@@ -145,7 +163,12 @@ struct General {
       const int first = ring * kTile + i / kBatches * kUnit + i % kBatches * TB;
       copy_wait<kStages - 2>();
       __syncwarp();  // the batch has arrived for all lanes, and all have left the stage that is filled next
-      issue(a, fill);
+      if (batch == 0) locate(a, s.id, s.place);  // the id was asked for a batch ago
+      copy(a, fill, s.tile, batch);
+      if (++batch == kBatches) {
+        batch = 0;
+        s.advance(a);
+      }
       if (first < s.count) compute(region + stage * kStageBytes);
       stage = stage + 1 == kStages ? 0 : stage + 1;
       fill = fill + 1 == kStages ? 0 : fill + 1;

@@ -184,7 +184,7 @@ struct Tensor {
     return bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair)) : __half22float2(*reinterpret_cast<const __half2*>(&pair));
   }
 
-  __device__ __forceinline__ void query(const AttentionArgs& a, const Piece& p) {
+  __device__ __forceinline__ void fetch(const AttentionArgs& a, const Piece& p) {
     const int first = p.sub * kHeads + 8 * part, h = lane >> 2;  // of the group's heads
     const uint16_t* from = static_cast<const uint16_t*>(a.q) + p.row * a.q_token_stride +
                            (static_cast<long long>(p.kv_head) * a.group + first + h) * a.q_head_stride;
@@ -194,6 +194,9 @@ struct Tensor {
       q[step][0] = x.x;
       q[step][1] = x.y;
     }
+  }
+
+  __device__ __forceinline__ void query(const AttentionArgs& a) {
     if constexpr (kCoded) {
       const bool bf16 = a.type == ASG_TYPE_BF16;
       float top = 0.f;
@@ -232,12 +235,13 @@ struct Tensor {
     l[0] = l[1] = 0.f;
   }
 
-  // Copies the next tile to a stage; the ring's warps take every SHARE-th of its rows.
-  __device__ __forceinline__ void issue(const AttentionArgs& a, int stage) {
-    if (s.tile < s.count) {
-      const bool held = s.held(a);
+  // Copies the tile at token `tile` to a stage, given where the lane's token lies; the ring's warps take every SHARE-th
+  // of its rows.
+  __device__ __forceinline__ void copy(const AttentionArgs& a, int stage, int tile, long long id, int place) {
+    if (tile < s.count) {
+      const bool held = id >= 0 && id < a.n_pages;
       const unsigned seen = __ballot_sync(kFull, held) & 0xffffu;
-      const long long offset = held ? s.id * s.page_bytes + s.place * s.token_bytes : 0;
+      const long long offset = held ? id * s.page_bytes + place * s.token_bytes : 0;
       const int offset_low = static_cast<int>(offset), offset_high = static_cast<int>(offset >> 32);
       const uint32_t at = base + stage * kStageBytes;
       constexpr int kLines = 32 / kChunks;  // rows that one copy of all lanes covers
@@ -261,20 +265,28 @@ struct Tensor {
         if constexpr (kCoded) {
           const asg_page_pool& pool = lane < kTile ? a.key : a.value;
           const float* from = pool.scales + s.kv_head * pool.scale_head_stride;
-          if (held) from += s.id * pool.scale_page_stride + s.place * pool.scale_token_stride;
+          if (held) from += id * pool.scale_page_stride + place * pool.scale_token_stride;
           copy_async<4>(at + kExtras + lane * 4, from, held);
         }
         if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + kStageBytes - 4), "r"(seen) : "memory");
       }
     }
     copy_commit();
-    s.advance(a);
   }
 
   __device__ __forceinline__ void start(const AttentionArgs& a, const Piece& p) {
     s.start(a, p, ring, static_cast<int>(sizeof(T)));
+    const int first = s.tile;
+    long long id[kStages - 1];  // the page ids of all tiles are asked for before the first is needed
+    int place[kStages - 1];
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(a, i);
+    for (int i = 0; i < kStages - 1; ++i) {
+      id[i] = s.id;
+      place[i] = s.place;
+      s.advance(a);
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy(a, i, first + i * kUnit, id[i], place[i]);
   }
 
   // A tile's products with V are issued together with the next tile's products with K: the two chains hide one
@@ -296,7 +308,8 @@ struct Tensor {
         const uint32_t next = base + stage * kStageBytes;
         copy_wait<kStages - 3>();
         meet();  // the next tile has arrived, and all lanes have left the one before this, whose stage is filled now
-        issue(a, fill);
+        copy(a, fill, s.tile, s.id, s.place);
+        s.advance(a);
         fill = fill + 1 == kStages ? 0 : fill + 1;
         clear_dots();
 #pragma unroll

@@ -156,7 +156,7 @@ def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: 
     slots = _index("slots", slots, device)
     _require_native(device, key_pages, value_pages, key_scales, value_scales)
     tokens = slots.numel()
-    key = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    key = slots.new_empty((tokens, heads, dim), dtype=dtype)
     value = torch.empty_like(key)
     if tokens:
         _native.paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, value_scales)
@@ -215,7 +215,7 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
         raise ValueError("window must be positive")
     _require_native(device, query, key_pages, value_pages, key_scales, value_scales)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = query.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if rows:
         if _checking():
             _debug_check_table(crow, col, lengths, n_pages, page_size)

@@ -363,28 +363,33 @@ typedef struct asg_token_rows {
 } asg_token_rows;
 
 /*
- * Writes the keys and values of n_tokens new tokens into the cache: token t goes to slot slots[t] =
- * page * page_size + place in the page.  A slot below 0 or not below n_pages * page_size is skipped (a
- * padded batch).  The other slots of one call must differ from one another.
- * cache_type is in_type, or one of the 8-bit types: then scale = max|x| / 448 or / 127 over the
- * features of the row, held in float32, and code = x / scale rounded to the nearest code (ties to
- * even; the quotient is not rounded first).  A row with an infinity or a NaN reads back as NaN.
- * head_dim at most 256.
+ * The two calls that move tokens between rows and slots: token t and slot slots[t] = page * page_size + place in the
+ * page.  A slot below 0 or not below n_pages * page_size lies outside the cache.  token_type is one of the three wider
+ * types, head_dim at most 256.
  */
-int asg_paged_cache_write(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key,
-                          const asg_token_rows* value, const asg_page_pool* key_pool,
-                          const asg_page_pool* value_pool, int64_t n_pages, int64_t page_size, int n_heads,
-                          int head_dim, int in_type, int cache_type, void* stream);
+typedef struct asg_paged_cache_args {
+  const int64_t* slots; /* int64[n_tokens], device */
+  int64_t n_tokens;
+  asg_token_rows key, value;
+  asg_page_pool key_pool, value_pool;
+  int64_t n_pages, page_size, n_heads, head_dim;
+  int64_t token_type, cache_type;
+  void* stream;
+} asg_paged_cache_args;
 
 /*
- * Reads tokens back: row t of key and value (type out_type, any of the three wider ones) becomes the
- * token in slot slots[t], code * scale (a float32 product) for the 8-bit types; zeros where the slot
- * lies outside the cache.
+ * Writes tokens into their slots.  A slot outside the cache is skipped (a padded batch); the other slots of one call
+ * must differ from one another.  cache_type is token_type, or one of the 8-bit types: then scale = max|x| / 448 or
+ * / 127 over the features of the row, held in float32, and code = x / scale rounded to the nearest code (ties
+ * to even; the quotient is not rounded first).  A row with an infinity or a NaN reads back as NaN.
  */
-int asg_paged_cache_read(const int64_t* slots, int64_t n_tokens, const asg_token_rows* key,
-                         const asg_token_rows* value, const asg_page_pool* key_pool,
-                         const asg_page_pool* value_pool, int64_t n_pages, int64_t page_size, int n_heads,
-                         int head_dim, int out_type, int cache_type, void* stream);
+int asg_paged_cache_write(const asg_paged_cache_args* args);
+
+/*
+ * Reads tokens back into the rows, in token_type whatever the type of the pages: code * scale (a float32 product)
+ * for the 8-bit types; zeros where the slot lies outside the cache.
+ */
+int asg_paged_cache_read(const asg_paged_cache_args* args);
 
 /* Bytes of workspace of asg_paged_attention (the partial results of rows that several CTAs share). */
 size_t asg_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
@@ -392,25 +397,31 @@ size_t asg_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head
 /*
  * out[r, h, :] = softmax_t(scale * <q[r, h, :], k_t>) v_t over the tokens t of row r, for one query
  * token a row; lse[r, h] = log sum_t exp(scale * <q, k_t>) when lse is not NULL (natural logarithm).
- *   crow[n_rows + 1], col[n_cols]  the page table: row r owns the pages col[crow[r] ... crow[r + 1])
- *   lengths[n_rows]   tokens of the row, the one in place i of the row's page j being token
- *                     j * page_size + i; cut to what the row's pages hold
- *   window            > 0: only the last `window` tokens of a row are seen; 0: all
- *   n_heads           query heads, a multiple of n_kv_heads; query head h uses key head
- *                     h / (n_heads / n_kv_heads)
- *   type, cache_type  of q and out, and of the pages: equal, or cache_type one of the 8-bit types
- * q takes the layout of asg_token_rows, out is [n_rows, n_heads, head_dim] and lse [n_rows, n_heads],
- * both contiguous.  A page id outside [0, n_pages) is a hole: its tokens are not seen.  A row that sees
- * nothing gets out = 0, lse = -inf.  The tokens behind a row's length are never read.  Scores, softmax
- * and sums are held in float32.  head_dim at most 256.  The workspace is 256-byte aligned; its content
- * need not be kept or cleared between calls.
+ * A page id outside [0, n_pages) is a hole: its tokens are not seen.  A row that sees nothing gets out = 0,
+ * lse = -inf.  The tokens behind a row's length are never read.  Scores, softmax and sums are held in float32.
  */
-int asg_paged_attention(const int64_t* crow, const int64_t* col, const int64_t* lengths, int64_t n_rows,
-                        int64_t n_cols, const asg_token_rows* q, void* out, float* lse,
-                        const asg_page_pool* key_pool, const asg_page_pool* value_pool, int64_t n_pages,
-                        int64_t page_size, int n_heads, int n_kv_heads, int head_dim, float scale,
-                        int64_t window, int type, int cache_type, void* workspace, size_t workspace_bytes,
-                        void* stream);
+typedef struct asg_paged_attention_args {
+  const int64_t *crow, *col; /* [n_rows + 1], [n_cols]: row r owns the pages col[crow[r] ... crow[r + 1]) */
+  const int64_t* lengths;    /* [n_rows] tokens of a row, token j * page_size + i in place i of its page j; cut to what
+                                the row's pages hold */
+  int64_t n_rows, n_cols;
+  asg_token_rows q;          /* [n_rows][n_heads][head_dim] */
+  void* out;                 /* the same, contiguous, in the type of q */
+  float* lse;                /* [n_rows, n_heads] or NULL */
+  asg_page_pool key_pool, value_pool;
+  int64_t n_pages, page_size;
+  int64_t n_heads;           /* a multiple of n_kv_heads; query head h uses key head h / (n_heads / n_kv_heads) */
+  int64_t n_kv_heads;
+  int64_t head_dim;          /* at most 256 */
+  int64_t window;            /* > 0: only the last `window` tokens of a row are seen; 0: all */
+  int64_t type, cache_type;  /* of q and out, and of the pages: equal, or cache_type one of the 8-bit types */
+  double scale;
+  void* workspace;           /* 256-byte aligned; its content need not be kept or cleared between calls */
+  size_t workspace_bytes;
+  void* stream;
+} asg_paged_attention_args;
+
+int asg_paged_attention(const asg_paged_attention_args* args);
 
 #ifdef __cplusplus
 }

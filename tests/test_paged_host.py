@@ -1,8 +1,6 @@
 """The paged cache's checks of arguments, on the CPU, and the float64 rounding that its GPU tests compare with."""
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -105,37 +103,67 @@ def test_library_checks_come_before_any_cuda_call(native_library):
     from autosage_b200 import _native
 
     lib = _native.bind(str(native_library))
-    pool, rows = _native.PagePool(), _native.TokenRows()
-    p, r = ctypes.byref(pool), ctypes.byref(rows)
-
-    def attention(n_rows=1, n_cols=0, n_pages=0, page=16, heads=4, kv=2, dim=64, window=0, kind=0, cache=0, q=r, keys=p):
-        return lib.asg_paged_attention(None, None, None, n_rows, n_cols, q, None, None, keys, p, n_pages, page, heads, kv, dim, 1.0,
-                                       window, kind, cache, None, 0, None)
 
     def says(code, wanted, text):
-        assert code == wanted and text in lib.asg_last_error_string()
+        assert code == wanted and text in lib.asg_last_error_string(), lib.asg_last_error_string()
+
+    def attention(n_rows=1, n_cols=0, n_pages=0, page=16, heads=4, kv=2, dim=64, window=0, kind=0, cache=0, data=0):
+        pool = (data, 0, 0, 0, 0, 0, 0, 0)
+        return lib.asg_paged_attention(_native._ATTENTION_ARGS.pack(
+            0, 0, 0, n_rows, n_cols, 0, 0, 0, 0, 0, *pool, *pool, n_pages, page, heads, kv, dim, window, kind, cache, 1.0, 0, 0, 0))
 
     says(attention(dim=257), -4, b"256 features")
     says(attention(page=0), -1, b"page_size")
     says(attention(page=1 << 30), -4, b"index range")
     says(attention(heads=5), -1, b"multiple of n_kv_heads")
+    says(attention(heads=1 << 40), -1, b"multiple of n_kv_heads")
+    says(attention(kv=1 << 40, heads=1 << 40), -4, b"index range")
     says(attention(kind=3), -1, b"type of the tokens")
     says(attention(cache=9), -1, b"type of the pages")
     says(attention(cache=1), -1, b"8-bit type")
     says(attention(window=-1), -1, b"window")
     says(attention(n_cols=1 << 31), -4, b"n_cols")
     says(attention(n_pages=3), -1, b"pages must not be null")
-    says(attention(keys=None), -1, b"key_pool")
+    says(attention(n_pages=3, cache=4, data=256), -1, b"8-bit pages need scales")
     says(attention(), -1, b"must not be null")
     assert attention(n_rows=0) == 0
-    says(lib.asg_paged_cache_write(None, 4, r, r, p, p, 0, 16, 2, 64, 0, 1, None), -1, b"slots, key and value")
-    says(lib.asg_paged_cache_write(None, -1, r, r, p, p, 0, 16, 2, 64, 0, 0, None), -1, b"n_tokens")
-    says(lib.asg_paged_cache_read(None, 4, r, r, p, p, 0, 16, 2, 64, 4, 0, None), -1, b"type of the tokens")
-    assert lib.asg_paged_cache_read(None, 0, r, r, p, p, 0, 16, 2, 64, 0, 0, None) == 0
-    pool.data = 256
-    says(lib.asg_paged_cache_write(None, 0, r, r, p, p, 1, 16, 2, 64, 0, 4, None), -1, b"8-bit pages need scales")
+
+    def cache(entry, n_tokens=4, page=16, kind=0, cache=0, n_pages=0, data=0):
+        pool = (data, 0, 0, 0, 0, 0, 0, 0)
+        return entry(_native._CACHE_ARGS.pack(0, n_tokens, 0, 0, 0, 0, 0, 0, *pool, *pool, n_pages, page, 2, 64, kind, cache, 0))
+
+    for entry in (lib.asg_paged_cache_write, lib.asg_paged_cache_read):
+        says(cache(entry), -1, b"slots, key and value")
+        says(cache(entry, n_tokens=-1), -1, b"n_tokens")
+        says(cache(entry, kind=4), -1, b"type of the tokens")
+        says(cache(entry, n_tokens=0, n_pages=1, cache=3, data=256), -1, b"8-bit pages need scales")
+        says(entry(None), -1, b"args must not be null")
+        assert cache(entry, n_tokens=0) == 0
+    says(cache(lib.asg_paged_cache_write, n_tokens=0, cache=1), -1, b"8-bit type")
+    says(lib.asg_paged_attention(None), -1, b"args must not be null")
     assert lib.asg_paged_attention_workspace_bytes(32, 8, 128) % 256 == 0
     assert lib.asg_paged_attention_workspace_bytes(32, 7, 128) == 0
+
+
+def test_packed_arguments_have_the_layout_of_the_header(tmp_path):
+    """The structs of the header have as many 8-byte fields as the binding packs."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    from autosage_b200 import _native
+
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    source = tmp_path / "sizes.c"
+    source.write_text('#include "autosage_b200.h"\n#include <stdio.h>\nint main(void) {'
+                      ' printf("%zu %zu %zu", sizeof(asg_paged_cache_args), sizeof(asg_paged_attention_args),'
+                      ' offsetof(asg_paged_attention_args, scale)); return 0; }')
+    include = Path(_native.__file__).resolve().parent.parent / "include"
+    subprocess.run([gcc, "-std=c99", "-Wall", "-Werror", f"-I{include}", str(source), "-o", str(tmp_path / "sizes")], check=True)
+    sizes = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(n) for n in sizes] == [_native._CACHE_ARGS.size, _native._ATTENTION_ARGS.size, 34 * 8]
 
 
 @pytest.mark.parametrize("kind", list(LARGEST))
