@@ -31,7 +31,7 @@ namespace paged {
 constexpr int kRings = 4;                  // warps, or groups of warps, of a CTA; each takes every fourth tile of a piece
 constexpr int kUnit = 64;                  // tokens per unit: one 16-token tile for each ring
 constexpr int kTile = kUnit / kRings;
-constexpr int kStart = 2;                  // cost of starting an item, in units (where the GPU has more than a unit a CTA)
+constexpr int kStart = 3;                  // cost of starting an item, in units (where the GPU has more than a unit a CTA)
 constexpr float kSlack = 6.f;
 constexpr float kNoScore = -3.402823466e38f; // m before the first score: every finite score is above it
 constexpr int kMaxCtasPerSm = 4;           // bounds the workspace; no kernel is launched with more

@@ -82,8 +82,15 @@ struct RowPlace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float largest_code(E4M3) { return 448.f; }
-__device__ __forceinline__ float largest_code(INT8) { return 127.f; }
+constexpr float largest_code(E4M3) { return 448.f; }
+constexpr float largest_code(INT8) { return 127.f; }
+
+// 1 / s within one unit in the last place, s in [2^-90, 2^90].
+__device__ __forceinline__ float reciprocal(float s) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  return fmaf(fmaf(-inv, s, 1.f), inv, inv);
+}
 
 // x / s, rounded to odd in float32; inv = 1 / s, s in [2^-90, 2^90].
 __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
@@ -95,9 +102,11 @@ __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
   return __int_as_float(rest != 0.f && (bits & 1) == 0 ? bits + step : bits);
 }
 // The same by way of float64: a quotient of two 24-bit numbers is never nearer to a border between codes than
-// 2^-40 of itself without lying on it, so 53 bits decide; they are rounded to odd too.
-__device__ __noinline__ float quotient_by_double(float x, float s) {
-  const double wide = static_cast<double>(x) / static_cast<double>(s);
+// 2^-40 of itself without lying on it, so 53 bits decide; they are rounded to odd too.  Cut to the largest code (a
+// subnormal scale may be rounded far down); NaN, which the scale carries, becomes 0.
+__device__ __noinline__ float quotient_by_double(float x, float s, float most) {
+  double wide = static_cast<double>(x) / static_cast<double>(s);
+  wide = wide != wide ? 0.0 : fmin(fmax(wide, -static_cast<double>(most)), static_cast<double>(most));
   const float q = static_cast<float>(wide);
   const double rest = wide - static_cast<double>(q);
   const int bits = __float_as_int(q);
@@ -105,44 +114,66 @@ __device__ __noinline__ float quotient_by_double(float x, float s) {
   return __int_as_float(bits + ((rest < 0.0) == (q < 0.f) ? 1 : -1));
 }
 
-// Two quotients to their nearest codes (ties to even, cut to the largest), first in the low byte.
-__device__ __forceinline__ uint32_t nearest_codes(float a, float b, E4M3) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// Four quotients to their nearest codes, ties to even.  (int8: added to 1.5 * 2^23 they are rounded to whole numbers, whose
+// last eight bits are the code; magnitudes are at most 127 and a rounding error.)
+__device__ __forceinline__ uint32_t nearest_codes(float a, float b, float c, float d, E4M3) {
+  const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return __byte_perm(low, high, 0x5410);
 }
-__device__ __forceinline__ uint32_t nearest_codes(float a, float b, INT8) {
-  const int x = max(-127, min(127, __float2int_rn(a))), y = max(-127, min(127, __float2int_rn(b)));
-  return (x & 0xff) | (y & 0xff) << 8;
+__device__ __forceinline__ uint32_t nearest_codes(float a, float b, float c, float d, INT8) {
+  constexpr float middle = 12582912.f;
+  const uint32_t low = __byte_perm(__float_as_uint(a + middle), __float_as_uint(b + middle), 0x0040);
+  const uint32_t high = __byte_perm(__float_as_uint(c + middle), __float_as_uint(d + middle), 0x0040);
+  return __byte_perm(low, high, 0x5410);
 }
 
-// P features a lane, next to one another (whole rows of such packs, aligned); P = 0: eight, one in 32 each, for any
-// alignment and head size.
+// P features a lane, next to one another, as one aligned vector of 32 bytes of the wide type, or (SPLIT) as two of 16 of
+// which the second may lie past the row's end; P = 0: eight, one in 32 each, for any alignment and head size.
 constexpr int lane_features(int p) { return p == 0 ? 8 : p; }
-template <int P>
-__device__ __forceinline__ int feature(int lane, int i) { return P == 0 ? i * 32 + lane : lane * P + i; }
 
-template <int P, typename T>
+template <int P, bool SPLIT, typename T>
 __device__ __forceinline__ void load_row(Pack<T, lane_features(P)>& x, const T* row, int lane, int dim) {
-  if constexpr (P > 0) {
-    if (lane * P < dim) {
-      x.load(row + lane * P);
-      return;
+  constexpr int N = lane_features(P);
+  if constexpr (P == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = i * 32 + lane < dim ? row[i * 32 + lane] : T{};
+  } else {
+    constexpr int kParts = SPLIT ? 2 : 1;
+    using Part = Pack<T, N / kParts>;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      Part part;
+      const int d = lane * P + i * (P / kParts);
+      if (d < dim) {
+        part.load(row + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N / kParts; ++j) part.v[j] = T{};
+      }
+#pragma unroll
+      for (int j = 0; j < N / kParts; ++j) x.v[i * (N / kParts) + j] = part.v[j];
     }
   }
-#pragma unroll
-  for (int i = 0; i < lane_features(P); ++i) {
-    x.v[i] = T{};
-    if (P == 0 && feature<P>(lane, i) < dim) x.v[i] = row[feature<P>(lane, i)];
-  }
 }
 
-template <int P, typename T>
+template <int P, bool SPLIT, typename T>
 __device__ __forceinline__ void store_row(const Pack<T, lane_features(P)>& x, T* row, int lane, int dim) {
-  if constexpr (P > 0) {
-    if (lane * P < dim) x.store(row + lane * P);
-  } else {
+  constexpr int N = lane_features(P);
+  if constexpr (P == 0) {
 #pragma unroll
-    for (int i = 0; i < lane_features(P); ++i)
-      if (feature<P>(lane, i) < dim) row[feature<P>(lane, i)] = x.v[i];
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane < dim) row[i * 32 + lane] = x.v[i];
+  } else {
+    constexpr int kParts = SPLIT ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int d = lane * P + i * (P / kParts);
+      Pack<T, N / kParts> part;
+#pragma unroll
+      for (int j = 0; j < N / kParts; ++j) part.v[j] = x.v[i * (N / kParts) + j];
+      if (d < dim) part.store(row + d);
+    }
   }
 }
 
@@ -169,21 +200,22 @@ __device__ __forceinline__ float largest_of_row(const Pack<IN, N>& x, int group)
 // Codes and scale of a row whose largest magnitude is `top`.
 template <typename IN, typename CACHE, int N>
 __device__ __forceinline__ float quantise(const Pack<IN, N>& x, float top, Pack<CACHE, N>& c) {
-  const float most = largest_code(CACHE{});
-  const float s = top / most;
+  constexpr float most = largest_code(CACHE{});
   float v[N];
   to_floats(x, v);
-  if (s > 0x1p-90f && s < 0x1p90f) {
+  float s;
+  if (top > 0x1p-80f && top < 0x1p90f) {
+    constexpr float share = 1.f / most;
+    s = top * share;
+    s = fmaf(fmaf(-s, most, top), share, s);  // top / most, correctly rounded (checked for every mantissa)
+    const float inv = reciprocal(s);
     if constexpr (sizeof(IN) == 2) {
-      float inv;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within one unit in the last place
-      const float off = fmaf(-s, most, top);                   // exact; its sign is that of e
+      const float off = fmaf(-s, most, top);  // exact; its sign is that of e
       if (off != 0.f) {
         const float w = inv * (off > 0.f ? 1.f + 0x1p-21f : 1.f - 0x1p-21f);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] *= w;
       } else {
-        inv = fmaf(fmaf(-inv, s, 1.f), inv, inv);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float q0 = v[i] * inv;
@@ -191,30 +223,32 @@ __device__ __forceinline__ float quantise(const Pack<IN, N>& x, float top, Pack<
         }
       }
     } else {
-      const float inv = 1.f / s;
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = quotient_to_odd(v[i], s, inv);
     }
-  } else if (s == 0.f) {  // nothing but zeros, or values that a scale above 0 cannot reach
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
   } else {
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {
+    s = top / most;
+    if (s == 0.f) {  // nothing but zeros, or values that no scale above 0 reaches
 #pragma unroll
-      for (int j = 0; j < N; ++j)  // (registers cannot be indexed)
-        if (j == i) v[j] = quotient_by_double(v[j], s);
+      for (int i = 0; i < N; ++i) v[i] = 0.f;
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)  // (registers cannot be indexed)
+          if (j == i) v[j] = quotient_by_double(v[j], s, most);
+      }
     }
   }
   static_assert(N % 4 == 0, "codes are packed four at a time");
 #pragma unroll
   for (int i = 0; i < N / 4; ++i)
-    reinterpret_cast<uint32_t*>(c.v)[i] = nearest_codes(v[4 * i], v[4 * i + 1], CACHE{}) | nearest_codes(v[4 * i + 2], v[4 * i + 3], CACHE{}) << 16;
+    reinterpret_cast<uint32_t*>(c.v)[i] = nearest_codes(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], CACHE{});
   return s;
 }
 
-template <typename IN, typename CACHE, int P>
-__global__ void __launch_bounds__(kThreads) write_kernel(const CacheArgs a, int group) {
+template <typename IN, typename CACHE, int P, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 4) write_kernel(const CacheArgs a, int group) {
   constexpr int N = lane_features(P);
   const int lane = threadIdx.x & (group - 1);
   const long long n_rows = a.n_tokens * a.n_heads;
@@ -228,24 +262,24 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const CacheArgs a, int 
     Pack<IN, N> x[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w)
-      load_row<P>(x[w], static_cast<const IN*>(a.rows[w].data) + at.token_at[w], lane, ok ? a.dim : 0);
+      load_row<P, SPLIT>(x[w], static_cast<const IN*>(a.rows[w].data) + at.token_at[w], lane, ok ? a.dim : 0);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       CACHE* to = static_cast<CACHE*>(a.pools[w].data) + at.page_at[w];
       if constexpr (!TypeOf<CACHE>::coded) {
-        store_row<P>(x[w], to, lane, ok ? a.dim : 0);
+        store_row<P, SPLIT>(x[w], to, lane, ok ? a.dim : 0);
       } else {
         const float top = largest_of_row(x[w], group);
         Pack<CACHE, N> c;
         const float s = quantise(x[w], top, c);
-        store_row<P>(c, to, lane, ok ? a.dim : 0);
+        store_row<P, SPLIT>(c, to, lane, ok ? a.dim : 0);
         if (ok && lane == 0) a.pools[w].scales[at.scale_at[w]] = s;
       }
     }
   }
 }
 
-template <typename CACHE, typename OUT, int P>
+template <typename CACHE, typename OUT, int P, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int group) {
   constexpr int N = lane_features(P);
   const int lane = threadIdx.x & (group - 1);
@@ -258,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int g
     float s[2] = {1.f, 1.f};
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      load_row<P>(c[w], static_cast<const CACHE*>(a.pools[w].data) + at.page_at[w], lane, at.held ? a.dim : 0);
+      load_row<P, SPLIT>(c[w], static_cast<const CACHE*>(a.pools[w].data) + at.page_at[w], lane, at.held ? a.dim : 0);
       if (TypeOf<CACHE>::coded && at.held) s[w] = a.pools[w].scales[at.scale_at[w]];
     }
 #pragma unroll
@@ -268,32 +302,32 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const CacheArgs a, int g
       Pack<OUT, N> x;
 #pragma unroll
       for (int i = 0; i < N; ++i) x.v[i] = from_float<OUT>(TypeOf<CACHE>::coded ? v[i] * s[w] : v[i]);
-      store_row<P>(x, static_cast<OUT*>(a.rows[w].data) + at.token_at[w], lane, a.dim);
+      store_row<P, SPLIT>(x, static_cast<OUT*>(a.rows[w].data) + at.token_at[w], lane, a.dim);
     }
   }
 }
 
-// Features a lane, lanes per row and blocks.  Rows made of whole 32-byte packs of the wide type are moved in those, rows
-// of whole 16-byte packs in those (32768 tokens of 8 x 128 bfloat16 to e4m3: LANE32 against LANE16 us); anything else
-// takes a warp a row, one feature in 32 a lane.
+// Rows made of whole 32-byte packs of the wide type that start on 32 bytes are moved in those, rows of whole 16-byte packs
+// in pairs of these; anything else takes a warp a row, one feature in 32 a lane.
+enum class Form { whole, split, single };
 struct Shape {
-  int features, group;
+  Form form;
+  int group;  // lanes per row
   unsigned blocks;
 };
 
 static Shape shape_of(const CacheArgs& a, int wide_type, int cache_type) {
-  const int wide = type_bytes(wide_type), item = type_bytes(cache_type);
+  const int wide = type_bytes(wide_type), item = type_bytes(cache_type), p = 32 / wide;
+  auto fits = [&](int bytes) {  // vectors of that many bytes of the wide type
+    const int n = bytes / wide, packed = n * item < 32 ? n * item : 32;
+    bool ok = a.dim % n == 0;
+    for (int w = 0; w < 2; ++w) ok = ok && rows_aligned(a.rows[w], wide, bytes) && rows_aligned(a.pools[w], item, packed);
+    return ok;
+  };
   Shape s;
-  s.features = 0;
-  for (int bytes = 32; bytes >= 16 && s.features == 0; bytes /= 2) {
-    const int p = bytes / wide, packed = p * item;
-    bool fits = a.dim % p == 0 && a.dim <= 32 * p;
-    for (int w = 0; w < 2; ++w)
-      fits = fits && rows_aligned(a.rows[w], wide, bytes) && rows_aligned(a.pools[w], item, packed < 32 ? packed : 32);
-    if (fits) s.features = p;
-  }
+  s.form = fits(32) ? Form::whole : fits(16) ? Form::split : Form::single;
   s.group = 32;
-  while (s.features > 0 && s.group > 1 && s.group / 2 * s.features >= a.dim) s.group /= 2;
+  while (s.form != Form::single && s.group > 1 && s.group / 2 * p >= a.dim) s.group /= 2;
   const long long rows_per_block = kThreads / s.group;
   const long long blocks = (a.n_tokens * a.n_heads + rows_per_block - 1) / rows_per_block;
   s.blocks = static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20));
@@ -302,11 +336,11 @@ static Shape shape_of(const CacheArgs& a, int wide_type, int cache_type) {
 
 template <typename IN, typename CACHE>
 static int launch_write(const CacheArgs& a, cudaStream_t stream) {
-  constexpr int most = 32 / static_cast<int>(sizeof(IN));
+  constexpr int p = 32 / static_cast<int>(sizeof(IN));
   const Shape s = shape_of(a, TypeOf<IN>::id, TypeOf<CACHE>::id);
-  if (s.features == most) write_kernel<IN, CACHE, most><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else if (s.features > 0) write_kernel<IN, CACHE, most / 2><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else write_kernel<IN, CACHE, 0><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  if (s.form == Form::whole) write_kernel<IN, CACHE, p, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else if (s.form == Form::split) write_kernel<IN, CACHE, p, true><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else write_kernel<IN, CACHE, 0, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }
@@ -319,11 +353,11 @@ static int launch_write(const CacheArgs& a, int cache_type, cudaStream_t stream)
 
 template <typename CACHE, typename OUT>
 static int launch_read(const CacheArgs& a, cudaStream_t stream) {
-  constexpr int most = 32 / static_cast<int>(sizeof(OUT));
+  constexpr int p = 32 / static_cast<int>(sizeof(OUT));
   const Shape s = shape_of(a, TypeOf<OUT>::id, TypeOf<CACHE>::id);
-  if (s.features == most) read_kernel<CACHE, OUT, most><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else if (s.features > 0) read_kernel<CACHE, OUT, most / 2><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
-  else read_kernel<CACHE, OUT, 0><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  if (s.form == Form::whole) read_kernel<CACHE, OUT, p, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else if (s.form == Form::split) read_kernel<CACHE, OUT, p, true><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
+  else read_kernel<CACHE, OUT, 0, false><<<s.blocks, kThreads, 0, stream>>>(a, s.group);
   ASG_CUDA(cudaGetLastError());
   return ASG_OK;
 }
