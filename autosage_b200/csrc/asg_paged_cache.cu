@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const CacheArgs a, i
     Pack<IN, N> x[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w)
-      load_row<P, SPLIT>(x[w], static_cast<const IN*>(a.rows[w].data) + at.token_at[w], lane, ok ? a.dim : 0);
+      // (a skipped token's row is loaded too: the loads need not wait for its slot)
+      load_row<P, SPLIT>(x[w], static_cast<const IN*>(a.rows[w].data) + at.token_at[w], lane, r < n_rows ? a.dim : 0);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       CACHE* to = static_cast<CACHE*>(a.pools[w].data) + at.page_at[w];
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const CacheArgs a, i
       } else {
         const float top = largest_of_row(x[w], group);
         Pack<CACHE, N> c;
-        const float s = quantise(x[w], top, c);
+        const float s = quantise(x[w], ok ? top : 0.f, c);
         store_row<P, SPLIT>(c, to, lane, ok ? a.dim : 0);
         if (ok && lane == 0) a.pools[w].scales[at.scale_at[w]] = s;
       }
