@@ -1,4 +1,6 @@
 // Paged attention: C entry points and the kernel that joins the pieces of items shared by several CTAs.
+#include <mutex>
+
 #include "asg_paged_attention.cuh"
 
 namespace asg {
@@ -172,6 +174,10 @@ int asg_paged_attention(const asg_paged_attention_args* args) {
   a.partial = reinterpret_cast<float*>(at);
   // an item of at most one unit is never cut, and no row has more tokens than all pages of the table
   a.join = ctas > 1 && n_cols * page_size > kUnit;
+  // the two launches of a call follow one another on the stream also when another host thread calls with the same
+  // stream and workspace
+  static std::mutex launching;
+  std::lock_guard<std::mutex> hold(launching);
   if (int rc = choice.launch(a, ctas, stream)) return rc;
   return !a.join ? ASG_OK : launch_join(a, ctas, choice.gt, items * n_rows, stream);
 }

@@ -113,7 +113,8 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     NaN reads back as NaN.
 
     A slot outside the pages (-1, say) is skipped: padding.  The others must differ from one another: of two tokens
-    with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call)."""
+    with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call).  ``key`` and ``value``
+    do not share memory with the slots that are written."""
     n_pages, page_size, heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
     shape = key.shape
     if len(shape) != 3 or shape != value.shape or shape[1] != heads or shape[2] != dim:
@@ -140,6 +141,9 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
             raise RuntimeError("two tokens have the same slot")
     _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
                               key_scales, value_scales)
+    for written in (key_pages, value_pages, key_scales, value_scales):   # as after any operation in place
+        if written is not None and not written.is_inference():
+            torch.autograd.graph.increment_version(written)
 
 
 def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, *,
@@ -211,8 +215,11 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
         raise ValueError("crow must contain one entry per row and one more")
     if lengths.numel() != rows:
         raise ValueError("lengths must contain one entry per row")
-    if window is not None and window < 1:
-        raise ValueError("window must be positive")
+    if window is not None:
+        if not isinstance(window, int):
+            raise TypeError("window must be a whole number of tokens")
+        if window < 1:
+            raise ValueError("window must be positive")
     _require_native(device, query, key_pages, value_pages, key_scales, value_scales)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     lse = query.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
@@ -220,7 +227,7 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
         if _checking():
             _debug_check_table(crow, col, lengths, n_pages, page_size)
         _native.paged_attention(crow, col, lengths, _contiguous_features(query), out, lse, key_pages, value_pages, key_scales,
-                                value_scales, 1.0 if scale is None else float(scale), 0 if window is None else int(window))
+                                value_scales, 1.0 if scale is None else float(scale), 0 if window is None else min(window, 1 << 62))
     return (out, lse) if return_lse else out
 
 

@@ -200,6 +200,89 @@ def test_rows_may_share_pages(kinds):
 
 
 @pytest.mark.parametrize("kinds", TYPES, ids=str)
+def test_keys_and_values_in_pages_of_different_strides(kinds):
+    case = Case((8, 2, 64, 16), kinds, [33, 0, 257, 64], seed=19)
+    expected = case.expected()
+    turned = case.pages[1].transpose(1, 2).contiguous().transpose(1, 2)
+    case.check(case.run(value_pages=turned), expected)
+    both = torch.stack(case.pages, 1) if case.pages[0].element_size() > 1 else \
+        torch.stack([p.view(torch.uint8) for p in case.pages], 1).view(case.pages[0].dtype)
+    case.check(case.run(key_pages=both[:, 0], value_pages=both[:, 1]), expected)   # [pages, 2, page, heads, dim]
+    case.check(case.run(window=2 ** 70), expected)
+
+
+@pytest.mark.parametrize("kinds", [(F32, E4M3), (BF16, E4M3), (F16, INT8), (BF16, INT8)], ids=str)
+def test_scales_of_either_sign_and_other_sizes(kinds):
+    """Scales are the caller's: negative ones, zeros, keys and values whose tokens differ by 2^8 in size."""
+    case = Case((8, 2, 64, 16), kinds, [200, 33, 700], seed=20)
+    gen = torch.Generator().manual_seed(21)
+    for w in range(2):
+        factor = torch.exp2(torch.randint(-8, 1, case.scales[w].shape, generator=gen).float())
+        factor[torch.rand(factor.shape, generator=gen) < 0.3] *= -1
+        factor[torch.rand(factor.shape, generator=gen) < 0.05] = 0
+        case.scales[w] = case.scales[w] * factor.cuda()
+        case.exact[w] = case.exact[w] * factor.double().transpose(1, 2).unsqueeze(-1)
+    case.check(case.run(), case.expected())
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16], ids=str)
+def test_a_nan_code_is_a_nan(kind):
+    case = Case((4, 2, 64, 16), (kind, E4M3), [100, 70], seed=22)
+    page, place = int(case.col[case.crow[0] + 1]), 3
+    keys = case.pages[0].clone()
+    keys.view(torch.uint8)[page, place, 1, 5] = 0x7F
+    out, lse = case.run(key_pages=keys)
+    assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isnan(lse[0, 2:]).all())
+    assert bool(torch.isfinite(out[0, :2]).all()) and bool(torch.isfinite(out[1]).all())
+    values = case.pages[1].clone()
+    values.view(torch.uint8)[page, place, 0, 9] = 0xFF
+    out, lse = case.run(value_pages=values)
+    assert bool(torch.isnan(out[0, :2, 9]).all()) and int(torch.isnan(out).sum()) == 2 and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("kinds", [(BF16, BF16), (F32, F32)], ids=str)
+def test_two_threads_on_one_stream(kinds):
+    """Calls of two host threads on the same stream share its workspace; their launches do not interleave."""
+    import threading
+
+    cases = [Case((4, 1, 64, 16), kinds, lengths, seed=40 + i) for i, lengths in enumerate(([9000], [100, 7000, 3]))]
+    wanted = [case.run() for case in cases]
+    calls = []
+    for case in cases:
+        fixed = dict(crow=case.crow.cuda(), col=case.col.cuda(), lengths=case.lengths.cuda(), query=case.query.cuda())
+        calls.append(lambda case=case, fixed=fixed: case.run(**fixed))
+    results = [[], []]
+
+    def work(i):
+        with torch.no_grad():
+            for _ in range(200):
+                results[i].append(calls[i]())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for got, exact in zip(results, wanted):
+        assert len(got) == 200 and all(torch.equal(out, exact[0]) and torch.equal(lse, exact[1]) for out, lse in got)
+
+
+def test_writing_counts_as_a_change_in_place():
+    from autosage_b200 import paged
+
+    pages = [torch.zeros(2, 8, 1, 64, device="cuda") for _ in range(2)]
+    before = [p._version for p in pages]
+    x = torch.ones(1, 1, 64, device="cuda")
+    paged.paged_cache_write(torch.tensor([3], device="cuda"), x, x, *pages)
+    assert all(p._version > v for p, v in zip(pages, before))
+    with torch.inference_mode():
+        pages = [torch.zeros(2, 8, 1, 64, device="cuda") for _ in range(2)]
+        paged.paged_cache_write(torch.tensor([3], device="cuda"), x, x, *pages)
+        assert pages[0][0, 3].min().item() == 1
+
+
+@pytest.mark.parametrize("kinds", TYPES, ids=str)
 @pytest.mark.parametrize("shape", [(8, 2, 128, 16), (5, 5, 48, 12)], ids=str)
 def test_layouts(shape, kinds):
     """Heads outside the tokens; a query cut out of a wider projection; 32-bit indices; rows that no vector load fits."""

@@ -59,6 +59,7 @@ def attend(**change):
     (dict(key_scales=scales(), value_scales=scales()), ValueError, "8-bit pages only"),
     (dict(key_pages=pages(dim=16)[..., ::2]), ValueError, "contiguous"),
     (dict(window=0), ValueError, "window must be positive"),
+    (dict(window=1.5), TypeError, "whole number"),
     (dict(), RuntimeError, "needs CUDA"),
 ])
 def test_attention_refuses(change, error, message):
