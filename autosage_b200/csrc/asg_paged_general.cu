@@ -1,10 +1,10 @@
 // Paged attention on the FMA pipe: every type, head size and alignment, float32 products throughout.
 //
-// A warp takes batches of TB tokens; lane l holds E features of the query, key, value and accumulator rows.
-// The TB x GT scores of a batch are partial sums spread over 32 lanes; a reduce-scatter (each step halves
-// the number of values and the lanes they are spread over) leaves one whole score per lane for about one
-// shuffle a score, and exponentials are taken once, by the lane that owns the score.  The weights come back
-// to all lanes by one shuffle each.
+// A warp takes batches of TB tokens, one token with all 32 lanes or (heads of up to 64 features) two side by side with 16
+// lanes each; a lane holds E features of the query, key, value and accumulator rows.  The scores of a batch are
+// partial sums spread over the LANES lanes of a token; a reduce-scatter (each step halves the number of values and
+// the lanes they are spread over) leaves one whole score per lane for about one shuffle a score, and exponentials
+// are taken once, by the lane that owns the score.  The weights come back to their token's lanes by one shuffle each.
 //
 // Every warp has a ring of kStages batches in shared memory.  Where a lane's E features of a row are one aligned
 // vector (VEC), cp.async brings them there, several batches ahead; a lane copies what it will read itself.
@@ -14,7 +14,7 @@
 namespace asg {
 namespace paged {
 
-template <typename T, int E, int GT, bool VEC, int STAGES, int CTAS>
+template <typename T, int E, int LANES, int GT, bool VEC, int STAGES, int CTAS>
 struct General {
   static constexpr int kThreads = kRings * 32;
   static constexpr int kHeads = GT;
@@ -23,13 +23,15 @@ struct General {
   static constexpr bool kCoded = TypeOf<T>::coded;
   static constexpr int TB = E == 8 || GT == 8 ? 4 : 8;  // tokens per batch
   static constexpr int kBatches = kTile / TB;           // of a tile
-  static constexpr int N = TB * GT;                     // scores per batch: 4 ... 32
-  static constexpr int kShift = N == 32 ? 0 : N == 16 ? 1 : N == 8 ? 2 : 3;
-  static_assert(N == 32 || N == 16 || N == 8 || N == 4, "reduce-scatter sizes");
-  static constexpr int kDim = 32 * E;
+  static constexpr int kSide = 32 / LANES;              // tokens side by side
+  static constexpr int kSteps = TB / kSide;
+  static constexpr int N = kSteps * GT;                 // scores per batch and token's lanes: 4 ... LANES
+  static constexpr int kShift = N == LANES ? 0 : 2 * N == LANES ? 1 : 4 * N == LANES ? 2 : 3;
+  static_assert(N << kShift == LANES && (LANES == 32 || LANES == 16), "reduce-scatter sizes");
+  static constexpr int kDim = LANES * E;
   static constexpr int kPitch = kDim;
   static constexpr int kLaneBytes = E * static_cast<int>(sizeof(T));
-  static constexpr int kRowBytes = 32 * kLaneBytes;
+  static constexpr int kRowBytes = LANES * kLaneBytes;
   static constexpr int kValues = TB * kRowBytes;
   static constexpr int kExtras = 2 * TB * kRowBytes;  // the scales of a batch (key, value), then the mask of its seen tokens
   static constexpr int kStageBytes = (kExtras + (kCoded ? 2 * TB * 4 : 0) + 4 + 15) / 16 * 16;
@@ -38,8 +40,8 @@ struct General {
   static constexpr int kRingBytes = (kNeed + 127) / 128 * 128;
 
   float q[GT][E], o[GT][E];
-  float m, l;  // of the head that this lane owns scores of: head (lane >> kShift) % GT
-  int lane, ring;
+  float m, l;  // of the head that this lane owns scores of: head (place >> kShift) % GT
+  int lane, place, side, ring;  // lane of the warp, of its token; which of the tokens side by side
   unsigned char* region;
   Source s;
   int batch;                              // of the tile that is copied next
@@ -49,9 +51,10 @@ struct General {
   int scale_place;
 
   __device__ __forceinline__ explicit General(unsigned char* smem)
-      : lane(threadIdx.x & 31), ring(threadIdx.x >> 5), region(smem + (threadIdx.x >> 5) * kRingBytes) {}
+      : lane(threadIdx.x & 31), place(threadIdx.x % LANES), side((threadIdx.x & 31) / LANES), ring(threadIdx.x >> 5),
+        region(smem + (threadIdx.x >> 5) * kRingBytes) {}
 
-  static __device__ __forceinline__ int feature(int lane, int e) { return VEC ? lane * E + e : e * 32 + lane; }
+  __device__ __forceinline__ int feature(int e) const { return VEC ? place * E + e : e * LANES + place; }
 
   __device__ __forceinline__ void fetch(const AttentionArgs& a, const Piece& p) {
     const int head = p.kv_head * a.group + p.sub * GT, heads = min(GT, a.group - p.sub * GT);
@@ -59,7 +62,7 @@ struct General {
     for (int g = 0; g < GT; ++g)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int d = feature(lane, e);
+        const int d = feature(e);
         q[g][e] = g < heads && d < a.dim ? load_wide(a.q, p.row * a.q_token_stride + (head + g) * a.q_head_stride + d, a.type) : 0.f;
       }
   }
@@ -94,29 +97,29 @@ struct General {
       const int key_low = static_cast<int>(key_offset), key_high = static_cast<int>(key_offset >> 32);
       const int value_low = static_cast<int>(value_offset), value_high = static_cast<int>(value_offset >> 32);
 #pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const int from = batch * TB + t;
+      for (int i = 0; i < kSteps; ++i) {
+        const int t = i * kSide + side, from = batch * TB + t;
         const long long k = static_cast<long long>(__shfl_sync(kFull, key_high, from)) << 32 |
                             static_cast<unsigned>(__shfl_sync(kFull, key_low, from));
         const long long v = a.same_strides ? k : static_cast<long long>(__shfl_sync(kFull, value_high, from)) << 32 |
                                                      static_cast<unsigned>(__shfl_sync(kFull, value_low, from));
         const bool ok = (seen >> t & 1u) != 0;
-        unsigned char* to = at + t * kRowBytes + lane * kLaneBytes;
+        unsigned char* to = at + i * 32 * kLaneBytes + lane * kLaneBytes;  // token t, this lane's features
         if constexpr (VEC) {
           constexpr int kStep = kLaneBytes < 16 ? kLaneBytes : 16;
 #pragma unroll
           for (int b = 0; b < kLaneBytes; b += kStep) {
-            copy_async<kStep>(smem_u32(to) + b, s.keys + k + lane * kLaneBytes + b, ok && lane * E < a.dim);
-            copy_async<kStep>(smem_u32(to) + kValues + b, s.values + v + lane * kLaneBytes + b, ok && lane * E < a.dim);
+            copy_async<kStep>(smem_u32(to) + b, s.keys + k + place * kLaneBytes + b, ok && place * E < a.dim);
+            copy_async<kStep>(smem_u32(to) + kValues + b, s.values + v + place * kLaneBytes + b, ok && place * E < a.dim);
           }
         } else {
           const T* keys = reinterpret_cast<const T*>(s.keys + k);
           const T* values = reinterpret_cast<const T*>(s.values + v);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const bool in = ok && feature(lane, e) < a.dim;
-            reinterpret_cast<T*>(to)[e] = in ? keys[feature(lane, e)] : T{};
-            reinterpret_cast<T*>(to + kValues)[e] = in ? values[feature(lane, e)] : T{};
+            const bool in = ok && feature(e) < a.dim;
+            reinterpret_cast<T*>(to)[e] = in ? keys[feature(e)] : T{};
+            reinterpret_cast<T*>(to + kValues)[e] = in ? values[feature(e)] : T{};
           }
         }
       }
@@ -189,24 +192,33 @@ struct General {
     to_floats(p, x);
   }
 
+  // f over the lanes that own scores of one head (of different tokens).
+  template <typename F>
+  static __device__ __forceinline__ float over_tokens(float v, F f) {
+#pragma unroll
+    for (int step = 16; step >= 1; step >>= 1)
+      if (step >= LANES || step >= GT << kShift) v = f(v, __shfl_xor_sync(kFull, v, step));
+    return v;
+  }
+
   __device__ __forceinline__ void compute(const unsigned char* at) {
     float x[N];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
+    for (int i = 0; i < kSteps; ++i) {
       float k[E];
-      row_of(k, at + t * kRowBytes);
+      row_of(k, at + i * 32 * kLaneBytes);
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum = fmaf(q[g][e], k[e], sum);
-        x[t * GT + g] = sum;
+        x[i * GT + g] = sum;
       }
     }
-    // reduce-scatter: afterwards lane L holds the whole score of index L >> kShift
+    // reduce-scatter: afterwards the lane at place P of its token's lanes holds the whole score of index P >> kShift
     int n = N;
 #pragma unroll
-    for (int step = 16; step >= 1; step >>= 1) {
+    for (int step = LANES / 2; step >= 1; step >>= 1) {
       if (n > 1) {
         n >>= 1;
 #pragma unroll
@@ -222,7 +234,7 @@ struct General {
         x[0] += __shfl_xor_sync(kFull, x[0], step);
       }
     }
-    const int token = (lane >> kShift) / GT;  // and head (lane >> kShift) % GT
+    const int token = (place >> kShift) / GT * kSide + side;  // and head (place >> kShift) % GT
     const unsigned seen = *reinterpret_cast<const unsigned*>(at + kStageBytes - 4);
     const bool in = (seen >> token & 1u) != 0;
     float weight_scale = 1.f;
@@ -232,10 +244,7 @@ struct General {
     }
     const float score = in ? x[0] : -CUDART_INF_F;
     if (__any_sync(kFull, score > m + kSlack)) {
-      float top = score;
-#pragma unroll
-      for (int step = 16; step >= GT << kShift; step >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, step));
-      top = fmaxf(top, m);
+      const float top = fmaxf(over_tokens(score, [](float a, float b) { return fmaxf(a, b); }), m);
       const float shrink = exp2f(m - top);
       m = top;
       l *= shrink;
@@ -250,12 +259,12 @@ struct General {
     l += w;
     w = in ? w * weight_scale : 0.f;
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
+    for (int i = 0; i < kSteps; ++i) {
       float v[E];
-      row_of(v, at + kValues + t * kRowBytes);
+      row_of(v, at + kValues + i * 32 * kLaneBytes);
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
-        const float f = __shfl_sync(kFull, w, (t * GT + g) << kShift);
+        const float f = __shfl_sync(kFull, w, side * LANES + ((i * GT + g) << kShift));
 #pragma unroll
         for (int e = 0; e < E; ++e) o[g][e] = fmaf(f, v[e], o[g][e]);
       }
@@ -264,47 +273,46 @@ struct General {
 
   __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
     float* buffer = reinterpret_cast<float*>(smem + ring * kRingBytes + kPublish);
-    // the sum of a head is spread over the lanes that own its scores of different tokens
-#pragma unroll
-    for (int step = 16; step >= GT << kShift; step >>= 1) l += __shfl_xor_sync(kFull, l, step);
+    l = over_tokens(l, [](float a, float b) { return a + b; });
     const int mine = lane >> kShift;
     if (mine < GT && (lane & ((1 << kShift) - 1)) == 0) ml[ring * GT + mine] = make_float2(published_max(m), l);
 #pragma unroll
     for (int g = 0; g < GT; ++g)
 #pragma unroll
-      for (int e = 0; e < E; ++e) buffer[g * kPitch + feature(lane, e)] = o[g][e];
+      for (int e = 0; e < E; ++e) {
+        float sum = o[g][e];
+        if constexpr (kSide == 2) sum += __shfl_xor_sync(kFull, sum, 16);
+        if (side == 0) buffer[g * kPitch + feature(e)] = sum;
+      }
   }
 };
 
 // Stages: about 100 KB per SM in flight for float32 rows.  CTAs: q and o take 2 GT E registers.
-template <typename T, int E, int GT, bool VEC>
+template <typename T, int E, int LANES, int GT, bool VEC>
 static Choice pick() {
-  constexpr int batch = (E == 8 || GT == 8 ? 4 : 8) * 64 * E * static_cast<int>(sizeof(T));  // bytes of a stage
+  constexpr int batch = (E == 8 || GT == 8 ? 4 : 8) * 2 * LANES * E * static_cast<int>(sizeof(T));  // bytes of a stage
   constexpr int ctas = GT * E >= 32 || batch >= 8192 ? 2 : 3;
   constexpr int stages = !VEC ? 2 : batch >= 8192 ? 3 : batch >= 4096 ? 4 : 6;
-  return made<General<T, E, GT, VEC, stages, ctas>>();
+  return made<General<T, E, LANES, GT, VEC, stages, ctas>>();
 }
 
 // Heads per item: the group if it is small; a group of more takes several items, whose second reading of
 // the keys and values comes from L2.  Features wider than 128 leave room for four heads in registers.
 template <typename T, bool VEC>
 static Choice choose(const AttentionArgs& a) {
-  if (a.dim > 128) return a.group == 1 ? pick<T, 8, 1, VEC>() : pick<T, 8, 4, VEC>();
-  if (a.dim > 64 || sizeof(T) == 1) {  // (the smallest asynchronous copy is 4 bytes)
-    if (a.group == 1) return pick<T, 4, 1, VEC>();
-    return a.group <= 4 ? pick<T, 4, 4, VEC>() : pick<T, 4, 8, VEC>();
+  if (a.dim > 128) return a.group == 1 ? pick<T, 8, 32, 1, VEC>() : pick<T, 8, 32, 4, VEC>();
+  if (a.dim > 64) {
+    if (a.group == 1) return pick<T, 4, 32, 1, VEC>();
+    return a.group <= 4 ? pick<T, 4, 32, 4, VEC>() : pick<T, 4, 32, 8, VEC>();
   }
-  if constexpr (sizeof(T) > 1) {
-    if (a.group == 1) return pick<T, 2, 1, VEC>();
-    return a.group <= 4 ? pick<T, 2, 4, VEC>() : pick<T, 2, 8, VEC>();
-  }
-  return Choice{};
+  if (a.group == 1) return pick<T, 4, 16, 1, VEC>();
+  return a.group <= 4 ? pick<T, 4, 16, 4, VEC>() : pick<T, 4, 16, 8, VEC>();
 }
 
 template <typename T>
 static Choice choose(const AttentionArgs& a) {
   const int item = static_cast<int>(sizeof(T));
-  const int lane_features = a.dim > 128 ? 8 : a.dim > 64 || item == 1 ? 4 : 2;
+  const int lane_features = a.dim > 128 ? 8 : 4;
   const int bytes = lane_features * item < 16 ? lane_features * item : 16;
   if (a.dim % lane_features == 0 && rows_aligned(a.key, item, bytes) && rows_aligned(a.value, item, bytes))
     return choose<T, true>(a);
