@@ -148,12 +148,12 @@ int asg_paged_attention(const asg_paged_attention_args* args) {
   a.group = static_cast<int>(n_heads / n_kv_heads);
   a.type = static_cast<int>(type);
   a.scale_log2 = static_cast<float>(args->scale * 1.4426950408889634);
-  a.q_pairs = rows_aligned(args->q, type_bytes(type), 8);
+  a.q_fours = rows_aligned(args->q, type_bytes(type), 4 * type_bytes(type));
   a.same_strides = a.key.page_stride == a.value.page_stride && a.key.token_stride == a.value.token_stride;
   a.out_vector = head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
   a.partial_pitch = static_cast<int>((head_dim + 3) / 4 * 4);
-  // 16-bit queries run on the tensor cores wherever 16-byte copies can fetch the rows; float32 queries, whose
-  // products have to keep 24 bits, and everything else on the FMA pipe
+  // Tensor cores wherever 16-byte copies can fetch the rows, save for float32 pages, whose products have to keep 24 bits
+  // on both sides; everything else on the FMA pipe
   const int pages_type = static_cast<int>(cache_type);
   Choice choice = is_coded(cache_type) ? choose_tensor8(a, pages_type) : choose_tensor16(a, pages_type);
   if (choice.launch == nullptr) choice = choose_general(a, pages_type);

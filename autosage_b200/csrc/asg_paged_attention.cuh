@@ -51,7 +51,7 @@ struct AttentionArgs {
   int subgroups;    // items per key head: ceil(group / GT)
   int type;         // of q and out
   float scale_log2; // scale * log2(e)
-  bool q_pairs;     // the query's rows start on 8 bytes
+  bool q_fours;     // the query's rows start on four features' bytes
   bool join;        // the join kernel follows
   bool same_strides;  // of the pages of keys and values: one offset serves both
   bool out_vector;  // four neighbours of out can be stored at once

@@ -1,4 +1,4 @@
-// Paged attention on the tensor cores: 16-bit queries, 16-bit or 8-bit pages.
+// Paged attention on the tensor cores: 16-bit queries with 16-bit pages, any query with 8-bit pages.
 //
 // A decoding step multiplies each key with the few query heads of its group, so it is bound by the bytes of
 // the cache; what the kernel has to do is keep enough of them in flight and stay out of their way.  The
@@ -25,10 +25,15 @@
 // is free, so Q and O are simply laid out to match.  f16 holds codes whole but not every scale, so
 //   - a query head is multiplied by the power of two that brings its largest feature into [1, 2) (features
 //     below 2^-14 of that lose what lies below 2^-24 of it), undone in the factor of its scores;
-//   - the accumulator has a running reference of its own: with value scales c_t it holds
-//     sum_t 2^(s_t - r) c_t code_t, r about the largest s_t + log2 |c_t| so far, so its weights are small numbers
-//     whatever the scales are (the weight 2^(s_t - m) of the sum, times c_t 2^(m - r)); 2^(r - m) brings it to the
-//     common maximum m in the end.
+//   - the accumulator is held 2^-d times its value, 2^d about the largest 2^(s_t - m) |c_t| so far with value scales
+//     c_t: its weights, 2^(s_t - m) of the sum times c_t 2^-d, are small numbers whatever the scales are.  d is
+//     a whole number, so that taking 2^-d back in the end rounds nothing.
+//
+// float32 queries with 8-bit pages (WIDE).  Codes are exact in f16, so only the query and the weights need their 24
+// bits: a feature x enters as h1 + 2^-12 h2, h1 = f16(x), h2 = f16(2^12 (x - h1)), which is x to 2^-24, each with
+// sums of its own; weights are hi + lo as before (2^-23 of a weight, 2^-33 of the largest).  The tensor core cuts its sums
+// off rather than rounding them, so nothing is added up in it over more than two steps: its results are added
+// in float32 by the FMA pipe.  Two thirds of the time that the FMA pipe alone takes go (LANE).
 #pragma once
 
 #include "asg_paged_attention.cuh"
@@ -102,8 +107,9 @@ __device__ __forceinline__ void decode_alternate(uint32_t x, uint32_t& a, uint32
   decode_neighbours(__byte_perm(x, 0u, 0x3120), a, b, type);
 }
 
-// T: type of the pages; DP: features, padded; SHARE: warps that share a ring's tiles, each with 8 query heads of its own.
-template <typename T, int DP, int SHARE, int STAGES, int CTAS>
+// T: type of the pages; DP: features, padded; SHARE: warps that share a ring's tiles, each with 8 query heads of its own;
+// WIDE: the query is float32.
+template <typename T, int DP, int SHARE, int STAGES, int CTAS, bool WIDE = false>
 struct Tensor {
   static constexpr int kThreads = kRings * SHARE * 32;
   static constexpr int kHeads = 8 * SHARE;
@@ -132,13 +138,18 @@ struct Tensor {
   static constexpr float kLift = std::is_same<H, F16>::value ? 8.f : 0.f;
   static_assert(kSlack + 8.f <= 15.f, "weights in f16");
 
+  static_assert(!WIDE || kCoded, "float32 queries go with 8-bit pages");
+  static constexpr float kMostD = 120.f;  // |d|: larger scales overflow anyway, smaller ones count little
+  static __device__ __forceinline__ float power_of_two(float n) { return __int_as_float((127 + static_cast<int>(n)) << 23); }
+
   uint32_t q[kSteps][2];
+  uint32_t q2[WIDE ? kSteps : 1][2];  // second pieces
   float o[kSteps][4];
-  float dots[2][4];         // the next tile's scores, in two chains of products
+  float dots[2][4];         // the next tile's scores: two sums to be added (WIDE: of the first and of the second pieces)
   uint32_t high[2], low[2]; // this tile's weights
   float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1} of the warp's eight
-  float ref[2];      // 8-bit pages: the accumulator's own reference r, 2^(m - r), ...
-  float to_ref[2];
+  float d[2];        // 8-bit pages: the accumulator's power of two, 2^-d, ...
+  float held[2];
   float unit[2];     // ... and what undoes the query's power of two
   int lane, ring, part;
   uint32_t base;     // shared address of the ring's region
@@ -167,7 +178,7 @@ struct Tensor {
   static __device__ __forceinline__ uint2 load_query(const AttentionArgs& a, const uint16_t* row, bool ok, int step, int lane) {
     const int d0 = query_feature(step, lane, 0, 0), d1 = query_feature(step, lane, 1, 0);
     uint2 x = make_uint2(0u, 0u);
-    if (a.q_pairs) {  // whole pairs lie inside or outside the head
+    if (a.q_fours) {  // whole pairs lie inside or outside the head
       if constexpr (kCoded) {
         if (ok && d0 < a.dim) x = *reinterpret_cast<const uint2*>(row + d0);
       } else {
@@ -186,14 +197,37 @@ struct Tensor {
 
   __device__ __forceinline__ void fetch(const AttentionArgs& a, const Piece& p) {
     const int first = p.sub * kHeads + 8 * part, h = lane >> 2;  // of the group's heads
-    const uint16_t* from = static_cast<const uint16_t*>(a.q) + p.row * a.q_token_stride +
-                           (static_cast<long long>(p.kv_head) * a.group + first + h) * a.q_head_stride;
+    const bool ok = first + h < a.group;
+    const long long from = p.row * a.q_token_stride + (static_cast<long long>(p.kv_head) * a.group + first + h) * a.q_head_stride;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const uint2 x = load_query(a, from, first + h < a.group, step, lane);
-      q[step][0] = x.x;
-      q[step][1] = x.y;
+      if constexpr (WIDE) {  // four neighbours, held in the registers of both pieces until query()
+        const float* row = static_cast<const float*>(a.q) + from;
+        const int d = query_feature(step, lane, 0, 0);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (ok && d < a.dim) {
+          if (a.q_fours) x = *reinterpret_cast<const uint4*>(row + d);
+          else x = make_uint4(__float_as_uint(row[d]), __float_as_uint(row[d + 1]), __float_as_uint(row[d + 2]), __float_as_uint(row[d + 3]));
+        }
+        q[step][0] = x.x;
+        q[step][1] = x.y;
+        q2[step][0] = x.z;
+        q2[step][1] = x.w;
+      } else {
+        const uint2 x = load_query(a, static_cast<const uint16_t*>(a.q) + from, ok, step, lane);
+        q[step][0] = x.x;
+        q[step][1] = x.y;
+      }
     }
+  }
+
+  // The fetched features of pair `half` of a step as floats.
+  __device__ __forceinline__ float2 fetched(int step, int half, bool bf16) const {
+    if constexpr (WIDE)
+      return half == 0 ? make_float2(__uint_as_float(q[step][0]), __uint_as_float(q[step][1]))
+                       : make_float2(__uint_as_float(q2[step][0]), __uint_as_float(q2[step][1]));
+    else
+      return widen(q[step][half], bf16);
   }
 
   __device__ __forceinline__ void query(const AttentionArgs& a) {
@@ -204,7 +238,7 @@ struct Tensor {
       for (int step = 0; step < kSteps; ++step)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const float2 x = widen(q[step][half], bf16);
+          const float2 x = fetched(step, half, bf16);
           top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
         }
       top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
@@ -213,18 +247,21 @@ struct Tensor {
       power = power < -126 || power > 126 ? 0 : power;
       const float down = __int_as_float((127 - power) << 23), up = __int_as_float((127 + power) << 23);
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float2 x = widen(q[step][half], bf16);
-          float none0, none1;
-          q[step][half] = pack2<F16>(x.x * down, x.y * down, none0, none1);
+      for (int step = 0; step < kSteps; ++step) {
+        const float2 x = fetched(step, 0, bf16), y = fetched(step, 1, bf16);
+        float rest[4], none0, none1;
+        q[step][0] = pack2<F16>(x.x * down, x.y * down, rest[0], rest[1]);
+        q[step][1] = pack2<F16>(y.x * down, y.y * down, rest[2], rest[3]);
+        if constexpr (WIDE) {
+          q2[step][0] = pack2<F16>(rest[0] * 4096.f, rest[1] * 4096.f, none0, none1);
+          q2[step][1] = pack2<F16>(rest[2] * 4096.f, rest[3] * 4096.f, none0, none1);
         }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         unit[i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
-        ref[i] = kNoScore;
-        to_ref[i] = 0.f;
+        d[i] = -kMostD;
+        held[i] = power_of_two(kMostD);
       }
     }
 #pragma unroll
@@ -364,12 +401,22 @@ struct Tensor {
     } else {
       uint32_t c[4];
       ldmatrix_x4(c, further(line, step * 16));
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t k[4];
         decode_neighbours(c[2 * i], k[0], k[2], T{});
         decode_neighbours(c[2 * i + 1], k[1], k[3], T{});
-        mma16816<H>(dots[i], k, q[step + i][0], q[step + i][1]);
+        if constexpr (WIDE) {
+          mma16816<H>(sum, k, q[step + i][0], q[step + i][1]);
+          mma16816<H>(dots[1], k, q2[step + i][0], q2[step + i][1]);
+        } else {
+          mma16816<H>(dots[i], k, q[step + i][0], q[step + i][1]);
+        }
+      }
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dots[0][i] += sum[i];
       }
     }
   }
@@ -394,8 +441,16 @@ struct Tensor {
         uint32_t v[4];
         decode_alternate(c[2 * i], v[0], v[1], T{});
         decode_alternate(c[2 * i + 1], v[2], v[3], T{});
-        mma16816<H>(o[step + i], v, high[0], high[1]);
-        mma16816<H>(o[step + i], v, low[0], low[1]);
+        if constexpr (WIDE) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816<H>(sum, v, low[0], low[1]);
+          mma16816<H>(sum, v, high[0], high[1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[step + i][j] += sum[j];
+        } else {
+          mma16816<H>(o[step + i], v, high[0], high[1]);
+          mma16816<H>(o[step + i], v, low[0], low[1]);
+        }
       }
     }
   }
@@ -418,7 +473,7 @@ struct Tensor {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) x[t][h] = (dots[0][2 * t + h] + dots[1][2 * t + h]) * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
+      for (int h = 0; h < 2; ++h) x[t][h] = (dots[0][2 * t + h] + (WIDE ? dots[1][2 * t + h] * 0x1p-12f : dots[1][2 * t + h])) * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
     if (seen != 0xffffu) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -430,7 +485,7 @@ struct Tensor {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           w[t][h] = fast_exp2(x[t][h] - (m[h] - kLift));
-          u[t][h] = kCoded ? w[t][h] * (value_scale[t] * to_ref[h]) : w[t][h];
+          u[t][h] = kCoded ? w[t][h] * (value_scale[t] * held[h]) : w[t][h];
         }
     };
     powers();
@@ -445,14 +500,17 @@ struct Tensor {
       float shrink[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const float before = m[h];
         shrink[h] = raise(x[0][h], x[1][h], m[h]);
         l[h] *= shrink[h];
         if constexpr (kCoded) {
-          const float before = ref[h];
-          raise(x[0][h] + fast_log2(fabsf(value_scale[0])), x[1][h] + fast_log2(fabsf(value_scale[1])), ref[h]);
-          ref[h] = fmaxf(ref[h], m[h] - 120.f);  // 2^(m - r) stays a number; scales below 2^-120 count little
-          shrink[h] = fast_exp2(before - ref[h]);
-          to_ref[h] = fast_exp2(m[h] - ref[h]);
+          float largest = kNoScore;  // log2 of the tile's largest weight of the accumulator, against the new m
+          raise(x[0][h] + fast_log2(fabsf(value_scale[0])), x[1][h] + fast_log2(fabsf(value_scale[1])), largest);
+          const float faded = d[h] - (m[h] - before);
+          const float next = fminf(fmaxf(ceilf(fmaxf(largest - m[h], faded)), -kMostD), kMostD);
+          shrink[h] *= fast_exp2(fminf(d[h] - next, 126.f));
+          d[h] = next;
+          held[h] = power_of_two(-next);
         }
       }
 #pragma unroll
@@ -486,8 +544,7 @@ struct Tensor {
       sum += __shfl_xor_sync(kFull, sum, 8);
       sum += __shfl_xor_sync(kFull, sum, 16);
       if (lane < 4) ml[ring * kHeads + head] = make_float2(published_max(m[h]), sum * undo);
-      float back = undo;  // of the accumulator, to the maximum m
-      if (kCoded && ref[h] != kNoScore) back *= exp2f(ref[h] - m[h]);
+      const float back = kCoded ? undo * power_of_two(d[h]) : undo;
 #pragma unroll
       for (int step = 0; step < kSteps; ++step)
 #pragma unroll
@@ -499,9 +556,13 @@ struct Tensor {
 // Stages of a ring and CTAs per SM: one tile is being used with the next, the others are in flight.  16-bit pages want
 // few bytes in flight (64 x 8192 float16 of 8 x 128 take 174 us with one tile of each ring under way, 183 with two:
 // more requests from more rows spoil the order in which HBM serves them), 8-bit pages want the warps for their decoding.
-template <typename T, int SHARE>
+template <typename T, int SHARE, bool WIDE>
 inline Choice choose_padded(const AttentionArgs& a) {
-  if constexpr (sizeof(T) == 1) {
+  if constexpr (WIDE) {
+    if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 4, SHARE == 1 ? 3 : 2, true>>();
+    if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 4, SHARE == 1 ? 2 : 1, true>>();
+    return made<Tensor<T, 256, SHARE, 3, 1, true>>();
+  } else if constexpr (sizeof(T) == 1) {
     if (a.dim <= 64) return made<Tensor<T, 64, SHARE, 4, SHARE == 1 ? 4 : 2>>();
     if (a.dim <= 128) return made<Tensor<T, 128, SHARE, 4, SHARE == 1 ? 3 : 2>>();
     return made<Tensor<T, 256, SHARE, 3, SHARE == 1 ? 2 : 1>>();
@@ -511,12 +572,12 @@ inline Choice choose_padded(const AttentionArgs& a) {
     return made<Tensor<T, 256, SHARE, 3, 1>>();
   }
 }
-template <typename T>
+template <typename T, bool WIDE = false>
 inline Choice choose_tensor(const AttentionArgs& a) {
   const int item = static_cast<int>(sizeof(T));
   if (a.dim * item % 16 != 0 || !rows_aligned(a.key, item, 16) || !rows_aligned(a.value, item, 16)) return Choice{};
   if (!a.same_strides) return Choice{};
-  return a.group <= 8 ? choose_padded<T, 1>(a) : choose_padded<T, 2>(a);
+  return a.group <= 8 ? choose_padded<T, 1, WIDE>(a) : choose_padded<T, 2, WIDE>(a);
 }
 
 #endif  // __CUDACC__

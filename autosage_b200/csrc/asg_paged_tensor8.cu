@@ -5,7 +5,7 @@ namespace asg {
 namespace paged {
 
 Choice choose_tensor8(const AttentionArgs& a, int cache_type) {
-  if (a.type == ASG_TYPE_F32) return Choice{};
+  if (a.type == ASG_TYPE_F32) return cache_type == ASG_TYPE_E4M3 ? choose_tensor<E4M3, true>(a) : choose_tensor<INT8, true>(a);
   return cache_type == ASG_TYPE_E4M3 ? choose_tensor<E4M3>(a) : choose_tensor<INT8>(a);
 }
 
