@@ -161,6 +161,8 @@ int asg_paged_attention(const asg_paged_attention_args* args) {
   // no more CTAs than units there can be (every row may end in a partly filled one)
   const int64_t items = n_kv_heads * a.subgroups;
   const double most = (static_cast<double>(n_cols) * page_size / kUnit + n_rows) * items;
+  ASG_REQUIRE(most + static_cast<double>(n_rows) * kStart * items < 2e9, ASG_ERANGE,
+              "the page table lists more than 2^37 tokens and heads");
   int ctas = sm_count(guard.target) * choice.ctas_per_sm;
   if (most < ctas) ctas = most < 1 ? 1 : static_cast<int>(most);
   const size_t records = static_cast<size_t>(ctas) * 2 * choice.gt;

@@ -76,7 +76,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 // nothing outside them is addressed: crow is cut to [0, n_cols], lengths to what the pages hold.
 struct RowSpan {
   long long first, last, pages_begin;
-  __device__ __forceinline__ long long units() const { return (last - first + kUnit - 1) / kUnit; }
+  __device__ __forceinline__ int units() const { return static_cast<int>((last - first + kUnit - 1) / kUnit); }
 };
 __device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
   const long long n_cols = a.n_cols;
@@ -90,36 +90,36 @@ __device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
   return s;
 }
 
-// Where a CTA's share begins.
+// Where a CTA's share begins.  The host has seen to it that entries have 31-bit numbers (where crow is what it should be;
+// with any other nothing is addressed that should not be, and what is computed is nobody's).
 struct Share {
-  long long pos, end;   // entries of the list, flat
-  long long row_begin;  // entry at which the row begins
-  long long per_cta;
-  RowSpan span;         // of that row
+  int pos, end;   // entries of the list
+  int row_begin;  // entry at which the row begins
+  int per_cta;
   int row;
-  int start;            // empty units before each item
+  int start;      // empty units before each item
+  RowSpan span;   // of the row
 };
 
 // Every thread sums the units of its rows, a block scan finds the row that holds the share's first entry.
 template <int WARPS>
 __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
-  __shared__ long long warp_units[WARPS], warp_rows[WARPS];
-  __shared__ long long found_begin;
+  __shared__ int warp_units[WARPS], warp_rows[WARPS];
   __shared__ RowSpan found_span;
-  __shared__ int found_row;
+  __shared__ int found_row, found_begin;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_thread = (a.n_rows + WARPS * 32 - 1) / (WARPS * 32);
   const long long r0 = static_cast<long long>(tid) * per_thread;
-  long long units = 0, rows = 0;
+  int units = 0, rows = 0;
   for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) {
-    const long long here = row_span(a, static_cast<int>(r)).units();
+    const int here = row_span(a, static_cast<int>(r)).units();
     units += here;
     rows += here > 0;
   }
-  long long units_scan = units, rows_scan = rows;
+  int units_scan = units, rows_scan = rows;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(kFull, units_scan, o), r = __shfl_up_sync(kFull, rows_scan, o);
+    const int u = __shfl_up_sync(kFull, units_scan, o), r = __shfl_up_sync(kFull, rows_scan, o);
     if (lane >= o) {
       units_scan += u;
       rows_scan += r;
@@ -131,7 +131,7 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
   }
   if (tid == 0) found_row = -1;
   __syncthreads();
-  long long units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
+  int units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w < warp) {
@@ -142,17 +142,17 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
     all_rows += warp_rows[w];
   }
   Share s;
-  s.start = all_units * items_per_row > gridDim.x ? kStart : 0;
-  const long long total = (all_units + s.start * all_rows) * items_per_row;
-  s.per_cta = quotient(total + gridDim.x - 1, gridDim.x);
-  s.pos = s.per_cta * blockIdx.x;
-  s.end = s.pos + s.per_cta < total ? s.pos + s.per_cta : total;
-  long long at = (units_before + s.start * rows_before) * items_per_row;
+  s.start = all_units * items_per_row > static_cast<int>(gridDim.x) ? kStart : 0;
+  const int total = (all_units + s.start * all_rows) * items_per_row;
+  s.per_cta = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
+  s.pos = static_cast<int>(min(static_cast<long long>(s.per_cta) * blockIdx.x, static_cast<long long>(total)));
+  s.end = static_cast<int>(min(static_cast<long long>(s.pos) + s.per_cta, static_cast<long long>(total)));
+  int at = (units_before + s.start * rows_before) * items_per_row;
   if (s.pos < s.end && s.pos >= at && s.pos < at + (units + s.start * rows) * items_per_row) {  // exactly one thread
     long long r = r0;
     RowSpan span = row_span(a, static_cast<int>(r));
     while (r + 1 < a.n_rows) {
-      const long long n = span.units(), here = n > 0 ? (n + s.start) * items_per_row : 0;
+      const int n = span.units(), here = n > 0 ? (n + s.start) * items_per_row : 0;
       if (s.pos < at + here) break;
       at += here;
       span = row_span(a, static_cast<int>(++r));
@@ -289,37 +289,40 @@ __device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a, int blo
 struct Piece {
   RowSpan span;
   int row, item, kv_head, sub;
-  long long entry;          // of the list at which the item's tokens begin
-  long long units, u0, u1;  // of the item; the piece's
-  __device__ __forceinline__ long long first() const { return span.first + u0 * kUnit; }
-  __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + u1 * kUnit; }
+  int entry;          // of the list at which the item's tokens begin
+  int units, u0, u1;  // of the item; the piece's
+  __device__ __forceinline__ long long first() const { return span.first + static_cast<long long>(u0) * kUnit; }
+  __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + static_cast<long long>(u1) * kUnit; }
 };
 
 // Walks through a share.
 struct Walk {
   Share s;
   RowSpan span;
-  long long units, at;  // of the row's items; entry inside the item
+  int units, at;  // of the row's items; entry inside the item
   int item, items_per_row;
   __device__ __forceinline__ Walk(const AttentionArgs& a, int items, const Share& share) : s(share), items_per_row(items) {
     if (s.pos >= s.end) return;
     span = s.span;
-    units = span.units();
-    item = static_cast<int>(quotient(s.pos - s.row_begin, units + s.start));
+    units = s.row < 0 ? 0 : span.units();
+    if (units <= 0) {  // (only if crow is not what it should be)
+      s.pos = s.end;
+      return;
+    }
+    item = (s.pos - s.row_begin) / (units + s.start);
     at = s.pos - s.row_begin - item * (units + s.start);
   }
   // The next piece that has tokens; all threads of the block get the same.
   __device__ __forceinline__ bool next(const AttentionArgs& a, Piece& p) {
     while (s.pos < s.end) {
-      const long long entries = units + s.start, left = s.end - s.pos;
-      const long long to = entries - at <= left ? entries : at + left;
+      const int entries = units + s.start, to = min(entries, at + (s.end - s.pos));
       p.span = span;
       p.row = s.row;
       p.item = item;
       p.units = units;
       p.entry = s.pos - at + s.start;
-      p.u0 = at > s.start ? at - s.start : 0;
-      p.u1 = to > s.start ? to - s.start : 0;
+      p.u0 = max(at - s.start, 0);
+      p.u1 = max(to - s.start, 0);
       s.pos += to - at;
       at = 0;
       if (s.pos < s.end && ++item == items_per_row) {
@@ -448,8 +451,7 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       __syncthreads();
       const int slot = now.u0 > 0 ? 0 : now.u1 < now.units ? 1 : -1;  // -1: a whole item
       if (slot == 1)  // the CTA of the item's last unit is the one of its last piece
-        left_over = make_int4(now.row, now.item,
-                              static_cast<int>(quotient(now.entry + now.units - 1, walk.s.per_cta)) - static_cast<int>(blockIdx.x) + 1, 0);
+        left_over = make_int4(now.row, now.item, (now.entry + now.units - 1) / walk.s.per_cta - static_cast<int>(blockIdx.x) + 1, 0);
       store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o,
                                                                     Engine::kRingBytes / 4, ml);
       __syncthreads();  // the buffers are free again
