@@ -33,7 +33,7 @@
 // bits: a feature x enters as h1 + 2^-12 h2, h1 = f16(x), h2 = f16(2^12 (x - h1)), which is x to 2^-24, each with
 // sums of its own; weights are hi + lo as before (2^-23 of a weight, 2^-33 of the largest).  The tensor core cuts its sums
 // off rather than rounding them, so nothing is added up in it over more than two steps: its results are added
-// in float32 by the FMA pipe.  Two thirds of the time that the FMA pipe alone takes go (LANE).
+// in float32 by the FMA pipe.  (64 rows of up to 8192 tokens of 8 x 128 int8: 132 us, on the FMA pipe alone 308.)
 #pragma once
 
 #include "asg_paged_attention.cuh"

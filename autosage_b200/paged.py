@@ -84,7 +84,7 @@ def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> N
         for tensor in tensors:
             if tensor is not None and tensor.requires_grad:
                 raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
-    if not ops.load_native():
+    if _native._LIB is None and not ops.load_native():
         detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")
 
@@ -141,9 +141,9 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
             raise RuntimeError("two tokens have the same slot")
     _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
                               key_scales, value_scales)
-    for written in (key_pages, value_pages, key_scales, value_scales):   # as after any operation in place
-        if written is not None and not written.is_inference():
-            torch.autograd.graph.increment_version(written)
+    if not key_pages.is_inference():   # as after any operation in place
+        torch.autograd.graph.increment_version(
+            (key_pages, value_pages) if key_scales is None else (key_pages, value_pages, key_scales, value_scales))
 
 
 def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, *,
