@@ -132,7 +132,7 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     for name, tensor in (("key_pages", key_pages), ("value_pages", value_pages), ("key_scales", key_scales),
                          ("value_scales", value_scales)):
         _check_writable(name, tensor)
-    _require_native(device, key, value, key_pages, value_pages)
+    _require_native(device, key, value, key_pages, value_pages, key_scales, value_scales)
     if slots.numel() == 0 or n_pages == 0:
         return
     if _checking():
