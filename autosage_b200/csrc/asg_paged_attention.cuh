@@ -293,6 +293,7 @@ struct Piece {
   int units, u0, u1;  // of the item; the piece's
   __device__ __forceinline__ long long first() const { return span.first + static_cast<long long>(u0) * kUnit; }
   __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + static_cast<long long>(u1) * kUnit; }
+  __device__ __forceinline__ bool any() const { return u0 < u1; }
 };
 
 // Walks through a share.
@@ -301,7 +302,9 @@ struct Walk {
   RowSpan span;
   int units, at;  // of the row's items; entry inside the item
   int item, items_per_row;
-  __device__ __forceinline__ Walk(const AttentionArgs& a, int items, const Share& share) : s(share), items_per_row(items) {
+  __device__ __forceinline__ void begin(int items, const Share& share) {
+    s = share;
+    items_per_row = items;
     if (s.pos >= s.end) return;
     span = s.span;
     units = s.row < 0 ? 0 : span.units();
@@ -312,8 +315,9 @@ struct Walk {
     item = (s.pos - s.row_begin) / (units + s.start);
     at = s.pos - s.row_begin - item * (units + s.start);
   }
-  // The next piece that has tokens; all threads of the block get the same.
-  __device__ __forceinline__ bool next(const AttentionArgs& a, Piece& p) {
+  // The next piece that has tokens, or one without (all lanes of a warp).
+  __device__ __forceinline__ Piece next(const AttentionArgs& a) {
+    Piece p;
     while (s.pos < s.end) {
       const int entries = units + s.start, to = min(entries, at + (s.end - s.pos));
       p.span = span;
@@ -332,13 +336,14 @@ struct Walk {
         else span = row_span(a, s.row);
         units = span.units();
       }
-      if (p.u0 < p.u1) {
+      if (p.any()) {
         p.kv_head = p.item / a.subgroups;
         p.sub = p.item - p.kv_head * a.subgroups;
-        return true;
+        return p;
       }
     }
-    return false;
+    p.u0 = p.u1 = 0;
+    return p;
   }
 };
 
@@ -427,38 +432,63 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_wait_for_primary();  // launched while the kernel before on the stream ends
   pdl_release_dependents();
-  const int items_per_row = a.n_kv_heads * a.subgroups;
-  Walk walk(a, items_per_row, locate_share<Engine::kThreads / 32>(a, items_per_row));
-  int4 left_over = make_int4(0, 0, 0, 0);
-  Piece now;
-  if (walk.next(a, now)) {
+  // The walk and the pieces it finds live in shared memory: the loop over tiles wants the registers.  The first warp looks
+  // two pieces ahead, so that the barriers of a piece are all that the others need to see the next one.
+  __shared__ Walk shared_walk;
+  __shared__ Piece pieces[3];
+  const bool first_warp = threadIdx.x < 32, first_lane = threadIdx.x == 0;
+  {
+    const int items_per_row = a.n_kv_heads * a.subgroups;
+    const Share share = locate_share<Engine::kThreads / 32>(a, items_per_row);
+    if (first_warp) {
+      Walk walk;
+      walk.begin(items_per_row, share);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const Piece p = walk.next(a);
+        if (first_lane) pieces[i] = p;
+      }
+      if (first_lane) shared_walk = walk;
+    }
+    if (a.join && first_lane) a.pieces[blockIdx.x] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  if (pieces[0].any()) {
     Engine engine(smem);
     const float* o = reinterpret_cast<const float*>(smem + Engine::kPublish);
     float2* ml = reinterpret_cast<float2*>(smem + kRings * Engine::kRingBytes);
-    engine.fetch(a, now);
-    engine.start(a, now);
+    engine.fetch(a, pieces[0]);
+    engine.start(a, pieces[0]);
     engine.query(a);
-    for (bool more = true; more;) {
+    for (int now = 0;;) {
+      const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
+      if (first_warp) {
+        Walk walk = shared_walk;
+        const Piece p = walk.next(a);
+        if (first_lane) {
+          pieces[after] = p;
+          shared_walk = walk;
+        }
+      }
       engine.run(a);
-      Piece next;
-      more = walk.next(a, next);
+      const bool more = pieces[next].any();
       if (more) {
-        engine.fetch(a, next);
-        engine.start(a, next);
+        engine.fetch(a, pieces[next]);
+        engine.start(a, pieces[next]);
       }
       engine.publish(smem, ml);
       if (more) engine.query(a);
       __syncthreads();
-      const int slot = now.u0 > 0 ? 0 : now.u1 < now.units ? 1 : -1;  // -1: a whole item
-      if (slot == 1)  // the CTA of the item's last unit is the one of its last piece
-        left_over = make_int4(now.row, now.item, (now.entry + now.units - 1) / walk.s.per_cta - static_cast<int>(blockIdx.x) + 1, 0);
-      store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, now.row, now.kv_head, now.sub, slot, o,
-                                                                    Engine::kRingBytes / 4, ml);
+      const Piece& p = pieces[now];
+      const int slot = p.u0 > 0 ? 0 : p.u1 < p.units ? 1 : -1;  // -1: a whole item
+      if (slot == 1 && first_lane)  // the CTA of the item's last unit is the one of its last piece
+        a.pieces[blockIdx.x] = make_int4(p.row, p.item, (p.entry + p.units - 1) / shared_walk.s.per_cta - static_cast<int>(blockIdx.x) + 1, 0);
+      store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, p.row, p.kv_head, p.sub, slot, o, Engine::kRingBytes / 4, ml);
       __syncthreads();  // the buffers are free again
+      if (!more) break;
       now = next;
     }
   }
-  if (a.join && threadIdx.x == 0) a.pieces[blockIdx.x] = left_over;
   if (!a.join) clear_empty_rows(a, blockIdx.x, gridDim.x);  // otherwise the join kernel does, while this one runs
 }
 
