@@ -451,19 +451,22 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _page_pool(pages: torch.Tensor, scales: Optional[torch.Tensor]) -> tuple:
-    """asg_page_pool: data, scales, strides of pages, tokens and heads, strides of the scales."""
-    page, token, head, _ = pages.stride()
-    if scales is None:
-        return pages.data_ptr(), 0, page, token, head, 0, 0, 0
-    return (pages.data_ptr(), scales.data_ptr(), page, token, head, *scales.stride())
+def _page_pools(key_pages, value_pages, key_scales, value_scales) -> tuple:
+    """Two asg_page_pool: data, scales, strides of pages, tokens and heads, strides of the scales."""
+    k_page, k_token, k_head, _ = key_pages.stride()
+    v_page, v_token, v_head, _ = value_pages.stride()
+    if key_scales is None:
+        return (key_pages.data_ptr(), 0, k_page, k_token, k_head, 0, 0, 0,
+                value_pages.data_ptr(), 0, v_page, v_token, v_head, 0, 0, 0)
+    return (key_pages.data_ptr(), key_scales.data_ptr(), k_page, k_token, k_head, *key_scales.stride(),
+            value_pages.data_ptr(), value_scales.data_ptr(), v_page, v_token, v_head, *value_scales.stride())
 
 
 def _paged_cache_args(slots, key, value, key_pages, value_pages, key_scales, value_scales) -> bytes:
     key_token, key_head, _ = key.stride()
     value_token, value_head, _ = value.stride()
     return _CACHE_ARGS.pack(slots.data_ptr(), slots.numel(), key.data_ptr(), key_token, key_head, value.data_ptr(), value_token,
-                            value_head, *_page_pool(key_pages, key_scales), *_page_pool(value_pages, value_scales),
+                            value_head, *_page_pools(key_pages, value_pages, key_scales, value_scales),
                             *key_pages.shape, TYPES[key.dtype], TYPES[key_pages.dtype], _raw_stream(key_pages.device.index))
 
 
@@ -497,8 +500,7 @@ def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages,
     workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(n_heads, n_kv_heads, head_dim))
     code = library().asg_paged_attention(_ATTENTION_ARGS.pack(
         crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), query.data_ptr(), q_token, q_head,
-        out.data_ptr(), 0 if lse is None else lse.data_ptr(), *_page_pool(key_pages, key_scales),
-        *_page_pool(value_pages, value_scales), n_pages, page_size, n_heads, n_kv_heads, head_dim, window,
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), *_page_pools(key_pages, value_pages, key_scales, value_scales), n_pages, page_size, n_heads, n_kv_heads, head_dim, window,
         TYPES[query.dtype], TYPES[key_pages.dtype], scale, workspace.data_ptr(), workspace.numel(), stream))
     if code:
         check(code)

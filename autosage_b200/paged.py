@@ -44,37 +44,53 @@ def _index(name: str, tensor: torch.Tensor, device: torch.device) -> torch.Tenso
     return tensor if tensor.is_contiguous() else tensor.contiguous()
 
 
-def _check_pages(key_pages, value_pages, key_scales, value_scales) -> tuple:
-    """Checks the pages and returns (n_pages, page_size, heads, dim)."""
-    shape = key_pages.shape
-    if len(shape) != 4 or shape != value_pages.shape:
+def _refuse_pages(key_pages, value_pages, key_scales, value_scales) -> None:
+    """Says what is wrong with the pages."""
+    if key_pages.ndim != 4 or key_pages.shape != value_pages.shape:
         raise ValueError("key_pages and value_pages must have the same [n_pages, page_size, n_kv_heads, head_dim] shape")
-    n_pages, page_size, heads, dim = shape
-    if page_size < 1 or heads < 1 or dim < 1:
+    n_pages, page_size, heads, dim = key_pages.shape
+    if min(page_size, heads, dim) < 1:
         raise ValueError("page_size, n_kv_heads and head_dim must be positive")
     if dim > MAX_HEAD_DIM:
         raise ValueError(f"head_dim is at most {MAX_HEAD_DIM}")
-    dtype = key_pages.dtype
-    if dtype != value_pages.dtype or (dtype not in _WIDE and dtype not in _CODED):
+    dtype, device = key_pages.dtype, key_pages.device
+    if dtype != value_pages.dtype or dtype not in _native.TYPES:
         raise TypeError("the pages must both be float32, bfloat16, float16, float8_e4m3fn or int8")
     if dim > 1 and (key_pages.stride(3) != 1 or value_pages.stride(3) != 1):
         raise ValueError("the features of a page row must be contiguous")
-    device = key_pages.device
     if value_pages.device != device:
         raise ValueError("key_pages and value_pages must be on the same device")
-    if dtype in _CODED:
-        for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
-            if scales is None:
-                raise ValueError(f"8-bit pages need {name}")
-            if scales.dtype is not torch.float32:
-                raise TypeError(f"{name} must be float32")
-            if scales.shape != (n_pages, heads, page_size):
-                raise ValueError(f"{name} must have shape [n_pages, n_kv_heads, page_size]")
-            if scales.device != device:
-                raise ValueError(f"{name} must be on the device of the pages")
-    elif key_scales is not None or value_scales is not None:
+    if dtype not in _CODED:
         raise ValueError("scales go with 8-bit pages only")
-    return n_pages, page_size, heads, dim
+    for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
+        if scales is None:
+            raise ValueError(f"8-bit pages need {name}")
+        if scales.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        if scales.shape != (n_pages, heads, page_size):
+            raise ValueError(f"{name} must have shape [n_pages, n_kv_heads, page_size]")
+        if scales.device != device:
+            raise ValueError(f"{name} must be on the device of the pages")
+    raise AssertionError("pages refused for no reason")
+
+
+def _check_pages(key_pages, value_pages, key_scales, value_scales) -> torch.Size:
+    """Checks the pages and returns their shape (n_pages, page_size, heads, dim)."""
+    shape, dtype, device = key_pages.shape, key_pages.dtype, key_pages.device
+    fine = (len(shape) == 4 and shape == value_pages.shape and shape[1] > 0 and shape[2] > 0 and 0 < shape[3] <= MAX_HEAD_DIM
+            and value_pages.dtype is dtype and value_pages.device == device
+            and ((key_pages.stride(3) == 1 and value_pages.stride(3) == 1) or shape[3] == 1))
+    if fine and _native.TYPES.get(dtype, 9) <= 2:
+        fine = key_scales is None and value_scales is None
+    elif fine:
+        wanted = (shape[0], shape[2], shape[1])
+        fine = (dtype in _CODED and key_scales is not None and value_scales is not None
+                and key_scales.dtype is torch.float32 and value_scales.dtype is torch.float32
+                and key_scales.shape == wanted and value_scales.shape == wanted
+                and key_scales.device == device and value_scales.device == device)
+    if not fine:
+        _refuse_pages(key_pages, value_pages, key_scales, value_scales)
+    return shape
 
 
 def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
