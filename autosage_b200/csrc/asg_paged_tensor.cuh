@@ -139,7 +139,9 @@ struct Tensor {
   static_assert(kSlack + 8.f <= 15.f, "weights in f16");
 
   static_assert(!WIDE || kCoded, "float32 queries go with 8-bit pages");
-  static constexpr float kMostD = 120.f;  // |d|: larger scales overflow anyway, smaller ones count little
+  // d stays in range of float32 exponents: larger scales overflow anyway, smaller ones count little, and a weight (2^14 at
+  // most) times 2^-d is finite, so that a weight of 0 makes 0 of every value scale
+  static constexpr float kLeastD = -112.f, kMostD = 120.f;
   static __device__ __forceinline__ float power_of_two(float n) { return __int_as_float((127 + static_cast<int>(n)) << 23); }
 
   uint32_t q[kSteps][2];
@@ -260,8 +262,8 @@ struct Tensor {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         unit[i] = a.scale_log2 * __shfl_sync(kFull, up, 4 * (2 * (lane & 3) + i));
-        d[i] = -kMostD;
-        held[i] = power_of_two(kMostD);
+        d[i] = kLeastD;
+        held[i] = power_of_two(-kLeastD);
       }
     }
 #pragma unroll
@@ -485,7 +487,7 @@ struct Tensor {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           w[t][h] = fast_exp2(x[t][h] - (m[h] - kLift));
-          u[t][h] = kCoded ? w[t][h] * (value_scale[t] * held[h]) : w[t][h];
+          u[t][h] = kCoded ? w[t][h] * held[h] * value_scale[t] : w[t][h];
         }
     };
     powers();
@@ -507,7 +509,7 @@ struct Tensor {
           float largest = kNoScore;  // log2 of the tile's largest weight of the accumulator, against the new m
           raise(x[0][h] + fast_log2(fabsf(value_scale[0])), x[1][h] + fast_log2(fabsf(value_scale[1])), largest);
           const float faded = d[h] - (m[h] - before);
-          const float next = fminf(fmaxf(ceilf(fmaxf(largest - m[h], faded)), -kMostD), kMostD);
+          const float next = fminf(fmaxf(ceilf(fmaxf(largest - m[h], faded)), kLeastD), kMostD);
           shrink[h] *= fast_exp2(fminf(d[h] - next, 126.f));
           d[h] = next;
           held[h] = power_of_two(-next);

@@ -225,6 +225,25 @@ def test_scales_of_either_sign_and_other_sizes(kinds):
     case.check(case.run(), case.expected())
 
 
+@pytest.mark.parametrize("kinds", [(F32, E4M3), (BF16, E4M3), (F16, INT8), (BF16, INT8), (F32, INT8)], ids=str)
+def test_a_zero_value_takes_all_the_weight_of_large_ones(kinds):
+    """The first token of a row has a value scale of 0 and outweighs the others, whose values are large, by some 2^900."""
+    case = Case((8, 2, 64, 16), kinds, [200, 33, 700], seed=23)
+    case.query = case.query.abs()
+    first = case.col[case.crow[:-1]]
+    codes = case.pages[0].view(torch.uint8)
+    codes[first, 0] = codes[first, 0] & 0x7F if case.cache == E4M3 else case.pages[0][first, 0].abs().view(torch.uint8)
+    case.scales[0][first, :, 0] *= 128
+    case.scales[1] *= 2.0 ** 17
+    case.scales[1][first, :, 0] = 0
+    case.exact[0][first, 0] = case.exact[0][first, 0].abs() * 128
+    case.exact[1] *= 2.0 ** 17
+    case.exact[1][first, 0] = 0
+    expected = case.expected()
+    assert expected[0].abs().max() < 1e-60                        # (float64 holds what float32 cannot)
+    case.check(case.run(), expected)
+
+
 @pytest.mark.parametrize("kind", [F32, BF16, F16], ids=str)
 def test_a_nan_code_is_a_nan(kind):
     case = Case((4, 2, 64, 16), (kind, E4M3), [100, 70], seed=22)
