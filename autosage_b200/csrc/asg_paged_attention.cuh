@@ -10,7 +10,7 @@
 // per CTA (the piece it begins with and the piece it ends with), and join_kernel puts them together in the
 // order of the tokens, so results do not depend on timing.  Nothing waits on another CTA.
 //
-// Softmax: scores are kept in units of log2 (scale * log2(e) is folded into q), each warp keeps a running
+// Softmax: scores are kept in units of log2 (scale * log2(e) is a factor of q or of the score), each warp keeps a running
 // maximum m, sum l and accumulator o of its tokens:
 //   m' = max(m, s),  o' = o 2^(m - m') + 2^(s - m') v,  l' = l 2^(m - m') + 2^(s - m').
 // m moves only when a score exceeds it by more than kSlack: weights up to 2^kSlack do no harm in float32, and most
@@ -308,12 +308,15 @@ struct Walk {
     if (s.pos >= s.end) return;
     span = s.span;
     units = s.row < 0 ? 0 : span.units();
-    if (units <= 0) {  // (only if crow is not what it should be)
+    const unsigned into = static_cast<unsigned>(s.pos) - static_cast<unsigned>(s.row_begin);
+    const unsigned entries = static_cast<unsigned>(units + s.start);
+    // crow is not what it should be: rows that overlap can list more than 2^31 entries, whose numbers are then wrong
+    if (units <= 0 || into / entries >= static_cast<unsigned>(items)) {
       s.pos = s.end;
       return;
     }
-    item = (s.pos - s.row_begin) / (units + s.start);
-    at = s.pos - s.row_begin - item * (units + s.start);
+    item = static_cast<int>(into / entries);
+    at = static_cast<int>(into - item * entries);
   }
   // The next piece that has tokens, or one without (all lanes of a warp).
   __device__ __forceinline__ Piece next(const AttentionArgs& a) {

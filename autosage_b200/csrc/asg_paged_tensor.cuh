@@ -13,9 +13,10 @@
 // The weights enter as two 16-bit pieces (p = hi + lo, 2^-17 of p lost at most), so that the result is as
 // good as one with float32 weights: the second product costs nothing while the kernel waits for memory.
 //
-// Each warp works alone: 16-token tiles, a ring of kStages tiles of its own in shared memory filled by
-// cp.async 16 bytes at a time (rows padded by 16 bytes, so ldmatrix is free of bank conflicts), page ids
-// fetched one tile ahead of the copies that need them.  The warps of a CTA meet only at the end of a piece.
+// Each warp works alone (with more than 8 heads, two warps share a ring): 16-token tiles, a ring of kStages tiles in
+// shared memory filled by cp.async 16 bytes at a time (rows swizzled or padded, so ldmatrix is free of bank
+// conflicts), page ids fetched one tile ahead of the copies that need them.  The warps of a CTA meet only at the end
+// of a piece.
 //
 // 8-bit pages.  Codes stay codes in shared memory and become f16 numbers in registers, exactly:
 //   int8   0x6400 | (c + 128) is the number 1024 + c + 128; subtract 1152
