@@ -146,9 +146,10 @@ def _stream(device: torch.device) -> int:
 # --------------------------------------------------------------------------------------------
 # Workspaces.  The C ABI never allocates; scratch comes from torch's caching allocator so it
 # follows torch's stream semantics.  One scratch buffer per (device, stream) is kept for calls that
-# rebuild the plan, and a small LRU of buffers holding finished plans is keyed by the crow tensor.
+# rebuild the plan, another for the paged attention, and a small LRU of buffers holding finished plans
+# is keyed by the crow tensor.
 # --------------------------------------------------------------------------------------------
-_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+_SCRATCH: dict[tuple, torch.Tensor] = {}
 _PLANS: "OrderedDict[tuple, list]" = OrderedDict()   # key -> [crow weakref, crow version, buffer, plan built?]
 _UNBUILT: dict[int, list] = {}                       # buffer address -> entry whose plan no kernel has built yet
 PLAN_CACHE_ENTRIES = 16
@@ -167,12 +168,13 @@ def scratch(device: torch.device, n_rows: int, extra_bytes: int = 0) -> torch.Te
     return _scratch_on(device, index, _stream(device), workspace_bytes(n_rows) + int(extra_bytes))
 
 
-def _scratch_on(device: torch.device, index: int, stream: int, need: int) -> torch.Tensor:
+def _scratch_on(device: torch.device, index: int, stream: int, need: int, *owner: str) -> torch.Tensor:
+    """The buffer of (device, stream), or the one of its own that an ``owner`` has there."""
     if _capturing():
         # a captured launch keeps the raw pointer: the buffer has to come from the graph's own pool
         # (and so live as long as the graph), not from a cache that may replace it later
         return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
-    key = (index, stream)
+    key = (index, stream, *owner)
     buffer = _SCRATCH.get(key)
     if buffer is None or buffer.numel() < need:
         buffer = torch.empty(max(need, 1 << 16), dtype=torch.uint8, device=device)
@@ -497,7 +499,9 @@ def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages,
     q_token, q_head, _ = query.stride()
     device = query.device
     stream = _raw_stream(device.index)
-    workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(n_heads, n_kv_heads, head_dim))
+    # a buffer of its own: the launches of a call are kept together among calls of this operator only, so another
+    # host thread's SpMM on the same stream may come between the kernel that fills the workspace and the one that reads it
+    workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(n_heads, n_kv_heads, head_dim), "paged_attention")
     code = library().asg_paged_attention(_ATTENTION_ARGS.pack(
         crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), query.data_ptr(), q_token, q_head,
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), *_page_pools(key_pages, value_pages, key_scales, value_scales), n_pages, page_size, n_heads, n_kv_heads, head_dim, window,

@@ -26,7 +26,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
   pdl_wait_for_primary();
   const int4 piece = a.pieces[c];
   const int n = min(piece.z, ctas - c);  // of its pieces; 0: none starts here
-  if (n <= 0) return;
+  // (the workspace is the caller's: should anything else have written to it, no row is addressed that is not there)
+  if (n <= 0 || static_cast<unsigned>(piece.x) >= static_cast<unsigned>(a.n_rows) ||
+      static_cast<unsigned>(piece.y) >= static_cast<unsigned>(a.n_kv_heads * a.subgroups)) return;
   const int kv_head = piece.y / a.subgroups, sub = piece.y - kv_head * a.subgroups;
   const int heads = min(gt, a.group - sub * gt);
   const int fours = (a.dim + 3) / 4;

@@ -1,0 +1,66 @@
+"""What the paged operators pass to the library, on the CPU with a library that only records it."""
+from __future__ import annotations
+
+import struct
+
+import pytest
+import torch
+
+from autosage_b200 import _native
+
+WORKSPACE = 35            # field of asg_paged_attention_args, counted in eights of bytes
+
+
+class Recorder:
+    """Stands in for the shared library."""
+
+    def __init__(self):
+        self.attention, self.written, self.sizes = [], [], []
+
+    def asg_paged_attention(self, args):
+        self.attention.append(struct.unpack("=38q", args))
+        return 0
+
+    def asg_paged_cache_write(self, args):
+        self.written.append(struct.unpack("=31q", args))
+        return 0
+
+    def asg_paged_attention_workspace_bytes(self, n_heads, n_kv_heads, head_dim):
+        self.sizes.append((n_heads, n_kv_heads, head_dim))
+        return 4096
+
+    def asg_workspace_bytes(self, n_rows):
+        return 4096
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    library = Recorder()
+    monkeypatch.setattr(_native, "_LIB", library)
+    monkeypatch.setattr(_native, "_SCRATCH", {})
+    monkeypatch.setattr(_native, "_capturing", lambda *index: False)
+    monkeypatch.setattr(_native, "_stream", lambda device: 7)
+    monkeypatch.setattr(_native, "_raw_stream", lambda index: 7)
+    _native._paged_attention_bytes.cache_clear()
+    yield library
+    _native._paged_attention_bytes.cache_clear()
+
+
+def attend():
+    """One call below the checks of arguments."""
+    pages, query = torch.zeros(3, 4, 2, 8), torch.zeros(2, 4, 8)
+    crow, col, lengths = torch.tensor([0, 1, 3]), torch.tensor([2, 0, 1]), torch.tensor([3, 5])
+    _native.paged_attention(crow, col, lengths, query, torch.empty_like(query), None, pages, pages.clone(), None, None, 1.0, 0)
+
+
+def test_the_attention_has_a_workspace_of_its_own(recorder):
+    """Another operator's launches, by another host thread on the same stream, may lie between the two of a call."""
+    def other():
+        return _native._scratch_on(torch.device("cpu"), None, 7, 4096)
+
+    shared = other()
+    attend()
+    assert recorder.attention[0][WORKSPACE] != shared.data_ptr()
+    attend()
+    assert recorder.attention[1][WORKSPACE] == recorder.attention[0][WORKSPACE]     # kept between calls
+    assert other().data_ptr() == shared.data_ptr()
