@@ -467,6 +467,7 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
       if (first_warp) {
         Walk walk = shared_walk;
+        __syncwarp();  // all lanes have their copy before the first one replaces it
         const Piece p = walk.next(a);
         if (first_lane) {
           pieces[after] = p;

@@ -1,0 +1,86 @@
+"""Paged attention where every token's share of the answer is known exactly."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from paged_reference import HALF_STEP, LARGEST
+from test_gpu_paged import BF16, E4M3, F16, F32, INT8, TYPES, Case, loaded  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def counted(shape, kinds, lengths, block=16, **options):
+    """A case whose query is 0, so that all weights are 1, and whose value rows are 1 in feature (position // block) % dim and
+    0 elsewhere: output feature f is the share of the row's tokens that belong to f, the log-sum-exp log n."""
+    case = Case(shape, kinds, lengths, **options)
+    case.query = torch.zeros_like(case.query)
+    place, feature = [], []
+    for r, n in enumerate(lengths):
+        t = torch.arange(n)
+        place.append(case.col[case.crow[r] + t // case.page] * case.page + t % case.page)
+        feature.append(t // block % case.dim)
+    place, feature = torch.cat(place), torch.cat(feature)
+    one = 64.0 if case.cache in LARGEST else 1.0                 # a code that both 8-bit types hold, with a scale of 2^-6
+    rows = torch.zeros(place.numel(), case.kv, case.dim)
+    rows[torch.arange(place.numel()), :, feature] = one
+    values = case.pages[1].cpu()
+    flat = values.reshape(-1, case.kv, case.dim)
+    if values.element_size() == 1:
+        flat.view(torch.uint8)[place] = rows.to(values.dtype).view(torch.uint8)
+    else:
+        flat[place] = rows.to(values.dtype)
+    case.pages[1] = flat.view(values.shape).cuda()
+    if case.scales[1] is not None:
+        case.scales[1] = torch.full_like(case.scales[1], 2.0 ** -6)
+    case.block = block
+    return case
+
+
+def shares(case, window=None):
+    out = torch.zeros(len(case.lengths), case.dim, dtype=torch.float64)
+    n = case.lengths.clone()
+    for r, length in enumerate(case.lengths.tolist()):
+        t = torch.arange(max(0, length - window) if window else 0, length)
+        n[r] = t.numel()
+        if t.numel():
+            out[r] = torch.bincount(t // case.block % case.dim, minlength=case.dim).double() / t.numel()
+    return out, torch.log(n.double())
+
+
+def check(case, got, window=None):
+    exact, exact_lse = shares(case, window)
+    out, lse = got[0].double().cpu(), got[1].double().cpu()
+    # weights of 1 and their sums are whole numbers below 2^24, whatever pieces they are joined from: what is left is the
+    # rounding of 1 / n, of the product with it, and of the answer to its type
+    limit = (2.0 ** -23 + HALF_STEP[case.kind] * (1 + 2.0 ** -22)) * exact
+    assert bool(((out - exact.unsqueeze(1)).abs() <= limit.unsqueeze(1)).all())
+    # log2 (one unit in the last place), the factor ln 2 and its product
+    assert torch.equal(lse == float("-inf"), (exact_lse == float("-inf")).unsqueeze(1).expand_as(lse))
+    fine = torch.isfinite(exact_lse)
+    assert bool(((lse - exact_lse.unsqueeze(1)).abs()[fine] <= 2.0 ** -22 * exact_lse.unsqueeze(1)[fine]).all())
+
+
+@pytest.mark.parametrize("kinds", TYPES, ids=str)
+@pytest.mark.parametrize("lengths", [[1, 60001, 1], [40000], [5000] * 10, [4000, 3000, 1, 0, 2500, 7001] * 3, [300] * 200,
+                                     [2000 + 37 * r for r in range(24)], [64] * 7, list(range(130))], ids=lambda n: f"{len(n)}x{max(n)}")
+def test_every_token_counts_once(lengths, kinds):
+    """Wherever shares end and pieces are joined, no tile is lost or taken twice."""
+    case = counted((4, 2, 64, 16), kinds, lengths, seed=50)
+    check(case, case.run())
+    check(case, case.run(window=777), window=777)
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, E4M3), (F32, INT8)], ids=str)
+@pytest.mark.parametrize("shape", [(24, 1, 128, 24), (16, 1, 256, 64), (3, 3, 100, 7)], ids=str)
+def test_every_token_counts_once_in_other_heads(shape, kinds):
+    case = counted(shape, kinds, [30011, 900, 0, 17], seed=51)
+    check(case, case.run())
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, INT8)], ids=str)
+def test_more_items_than_ctas_on_one_walk(kinds):
+    """Each CTA walks through many whole items, some with rows that see nothing between them."""
+    lengths = [17 * (r % 13) for r in range(3000)]
+    case = counted((6, 3, 64, 16), kinds, lengths, seed=52)
+    check(case, case.run())
