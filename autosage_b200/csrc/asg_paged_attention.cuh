@@ -90,8 +90,10 @@ __device__ __forceinline__ RowSpan row_span(const AttentionArgs& a, int row) {
   return s;
 }
 
-// Where a CTA's share begins.  The host has seen to it that entries have 31-bit numbers (where crow is what it should be;
-// with any other nothing is addressed that should not be, and what is computed is nobody's).
+// Where a CTA's share begins.  The host has seen to it that entries have 31-bit numbers where crow is what it should be.
+// Rows of any other crow may overlap and list more than 2^32 entries; sums of entries are unsigned and wrap then, several
+// threads may find the share's first entry among their rows, and one of them is chosen: the span that all go by is
+// one that row_span has cut, so nothing is addressed that should not be, and what is computed is nobody's.
 struct Share {
   int pos, end;   // entries of the list
   int row_begin;  // entry at which the row begins
@@ -104,22 +106,23 @@ struct Share {
 // Every thread sums the units of its rows, a block scan finds the row that holds the share's first entry.
 template <int WARPS>
 __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_per_row) {
-  __shared__ int warp_units[WARPS], warp_rows[WARPS];
+  __shared__ unsigned warp_units[WARPS], warp_rows[WARPS];
   __shared__ RowSpan found_span;
-  __shared__ int found_row, found_begin;
+  __shared__ int found_row;
+  __shared__ unsigned found_begin, claimed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_thread = (a.n_rows + WARPS * 32 - 1) / (WARPS * 32);
   const long long r0 = static_cast<long long>(tid) * per_thread;
-  int units = 0, rows = 0;
+  unsigned units = 0, rows = 0;
   for (long long r = r0; r < r0 + per_thread && r < a.n_rows; ++r) {
     const int here = row_span(a, static_cast<int>(r)).units();
     units += here;
     rows += here > 0;
   }
-  int units_scan = units, rows_scan = rows;
+  unsigned units_scan = units, rows_scan = rows;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(kFull, units_scan, o), r = __shfl_up_sync(kFull, rows_scan, o);
+    const unsigned u = __shfl_up_sync(kFull, units_scan, o), r = __shfl_up_sync(kFull, rows_scan, o);
     if (lane >= o) {
       units_scan += u;
       rows_scan += r;
@@ -129,9 +132,12 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
     warp_units[warp] = units_scan;
     warp_rows[warp] = rows_scan;
   }
-  if (tid == 0) found_row = -1;
+  if (tid == 0) {
+    found_row = -1;
+    claimed = 0;
+  }
   __syncthreads();
-  int units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
+  unsigned units_before = units_scan - units, rows_before = rows_scan - rows, all_units = 0, all_rows = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w < warp) {
@@ -142,18 +148,21 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
     all_rows += warp_rows[w];
   }
   Share s;
-  s.start = all_units * items_per_row > static_cast<int>(gridDim.x) ? kStart : 0;
-  const int total = (all_units + s.start * all_rows) * items_per_row;
-  s.per_cta = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
+  const unsigned items = static_cast<unsigned>(items_per_row);
+  s.start = all_units * items > gridDim.x ? kStart : 0;
+  const unsigned total = min((all_units + s.start * all_rows) * items, 0x7fffffffu);
+  s.per_cta = static_cast<int>((total + gridDim.x - 1) / gridDim.x);
   s.pos = static_cast<int>(min(static_cast<long long>(s.per_cta) * blockIdx.x, static_cast<long long>(total)));
   s.end = static_cast<int>(min(static_cast<long long>(s.pos) + s.per_cta, static_cast<long long>(total)));
-  int at = (units_before + s.start * rows_before) * items_per_row;
-  if (s.pos < s.end && s.pos >= at && s.pos < at + (units + s.start * rows) * items_per_row) {  // exactly one thread
+  const unsigned pos = static_cast<unsigned>(s.pos);
+  unsigned at = (units_before + s.start * rows_before) * items;
+  // one thread has the entry among its rows
+  if (s.pos < s.end && pos - at < (units + s.start * rows) * items && atomicExch(&claimed, 1u) == 0) {
     long long r = r0;
     RowSpan span = row_span(a, static_cast<int>(r));
     while (r + 1 < a.n_rows) {
-      const int n = span.units(), here = n > 0 ? (n + s.start) * items_per_row : 0;
-      if (s.pos < at + here) break;
+      const unsigned n = span.units(), here = n > 0 ? (n + s.start) * items : 0;
+      if (pos - at < here) break;
       at += here;
       span = row_span(a, static_cast<int>(++r));
     }
@@ -163,7 +172,7 @@ __device__ __forceinline__ Share locate_share(const AttentionArgs& a, int items_
   }
   __syncthreads();
   s.row = found_row;
-  s.row_begin = found_begin;
+  s.row_begin = static_cast<int>(found_begin);
   s.span = found_span;
   return s;
 }

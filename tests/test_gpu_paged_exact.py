@@ -84,3 +84,25 @@ def test_more_items_than_ctas_on_one_walk(kinds):
     lengths = [17 * (r % 13) for r in range(3000)]
     case = counted((6, 3, 64, 16), kinds, lengths, seed=52)
     check(case, case.run())
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, INT8)], ids=str)
+def test_a_crow_whose_rows_overlap_past_2_to_the_32_entries(kinds):
+    """No table, and no answer: every second row lists all columns, 2^32 entries and some 65,000 of the list together.  The call ends,
+    and the next one is right."""
+    from autosage_b200 import paged
+
+    rows, n, page = 65534, 4096, 1024
+    assert (rows // 2 * (n * page // 64 + 3) * 2) % 2 ** 32 < 2 ** 17 < 2 ** 32 < rows // 2 * (n * page // 64 + 3) * 2
+    case = counted((4, 2, 64, 16), kinds, [700, 3], seed=53)
+    pools = dict(key_pages=torch.zeros(4, page, 2, 64, device="cuda").to(case.cache),
+                 value_pages=torch.zeros(4, page, 2, 64, device="cuda").to(case.cache))
+    if case.cache in LARGEST:
+        pools.update(key_scales=torch.ones(4, 2, page, device="cuda"), value_scales=torch.ones(4, 2, page, device="cuda"))
+    crow = torch.tensor([0, n], device="cuda").repeat(rows // 2 + 1)[:rows + 1]
+    lengths = torch.full((rows,), n * page, device="cuda")
+    out = paged.csr_paged_attention(crow, torch.arange(n, device="cuda") % 4, lengths,
+                                    torch.zeros(rows, 4, 64, device="cuda").to(case.kind), **pools)
+    torch.cuda.synchronize()
+    assert out.shape == (rows, 4, 64)
+    check(case, case.run())
