@@ -435,6 +435,8 @@ __device__ __forceinline__ float published_max(float m) { return m == kNoScore ?
 //   start(a, piece)                   begins to copy the piece's tokens
 //   query(a)                          takes the query and clears the accumulators
 //   run(a)                            the ring's tiles
+//   unsound(a, piece)                 whether a sum that run() has left cannot stand (the same for all lanes of a ring)
+//   run_carefully(a)                  the ring's tiles once more, however long it takes
 //   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + ring * kRingBytes +
 //                                     kPublish, which no copy of a started piece writes before run()
 // kRingBytes * kRings bytes of shared memory belong to the engine, the (m, l) pairs lie behind them.
@@ -484,6 +486,12 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
         }
       }
       engine.run(a);
+      if (engine.unsound(a, pieces[now])) {
+        engine.fetch(a, pieces[now]);
+        engine.start(a, pieces[now]);
+        engine.query(a);
+        engine.run_carefully(a);
+      }
       const bool more = pieces[next].any();
       if (more) {
         engine.fetch(a, pieces[next]);

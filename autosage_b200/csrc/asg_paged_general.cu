@@ -180,6 +180,10 @@ struct General {
     __syncwarp();
   }
 
+  // (float32 weights, one product a value: what is not finite is the answer)
+  __device__ __forceinline__ bool unsound(const AttentionArgs&, const Piece&) const { return false; }
+  __device__ __forceinline__ void run_carefully(const AttentionArgs& a) { run(a); }
+
   __device__ __forceinline__ void row_of(float (&x)[E], const unsigned char* at) const {
     const T* from = reinterpret_cast<const T*>(at + lane * kLaneBytes);
     Pack<T, E> p;

@@ -12,6 +12,9 @@
 //                                         packed to 16 bits and transposed by movmatrix, no trip to memory
 // The weights enter as two 16-bit pieces (p = hi + lo, 2^-17 of p lost at most), so that the result is as
 // good as one with float32 weights: the second product costs nothing while the kernel waits for memory.
+// An infinite value times two pieces is not what it is times their sum (lo may be 0 or negative, and so may a weight's hi
+// be 0).  Such a value leaves a sum that is not finite; a ring that ends a piece with one goes through it again and
+// multiplies float32 weights with single values on the FMA pipe (run_carefully), which costs nothing where all is finite.
 //
 // Each warp works alone (with more than 8 heads, two warps share a ring): 16-token tiles, a ring of kStages tiles in
 // shared memory filled by cp.async 16 bytes at a time (rows swizzled or padded, so ldmatrix is free of bank
@@ -367,6 +370,85 @@ struct Tensor {
     meet();
   }
 
+  // Whether a sum of the piece's heads is not finite: 0 times it is not 0.
+  __device__ __forceinline__ bool unsound(const AttentionArgs& a, const Piece& p) const {
+    bool any = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float zero = 0.f;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) zero = fmaf(o[step][h], 0.f, fmaf(o[step][2 + h], 0.f, zero));
+      any = any || (p.sub * kHeads + 8 * part + 2 * (lane & 3) + h < a.group && zero != 0.f);
+    }
+    if constexpr (SHARE == 1) {
+      any = __any_sync(kFull, any);
+    } else {
+      int ring_any;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                   : "=r"(ring_any) : "r"(static_cast<int>(any)), "r"(1 + ring), "n"(SHARE * 32) : "memory");
+      any = ring_any != 0;
+    }
+    return any;
+  }
+
+  __device__ __forceinline__ void run_carefully(const AttentionArgs& a) {
+    const int tiles = s.count <= ring * kTile ? 0 : (s.count - ring * kTile + kUnit - 1) / kUnit;
+    int stage = 0, fill = kStages - 1;
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+      copy_wait<kStages - 2>();
+      meet();  // the tile has arrived, and all lanes have left the one before it, whose stage is filled now
+      copy(a, fill, s.tile, s.id, s.place);
+      s.advance(a);
+      const uint32_t at = base + stage * kStageBytes;
+      clear_dots();
+#pragma unroll
+      for (int step = 0; step < kSteps; step += 2) score_steps(at, step);
+      weigh<true>(a, at);
+      add_values(at);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      fill = fill + 1 == kStages ? 0 : fill + 1;
+    }
+    copy_wait<0>();
+    meet();
+  }
+
+  // The tile's products with V one by one: `high` and `low` hold the weights of heads 2 (lane % 4) and the next one, of tokens
+  // lane / 4 and lane / 4 + 8, as floats.
+  __device__ __forceinline__ void add_values(uint32_t at) {
+    unsigned seen;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(seen) : "r"(at + kStageBytes - 4));
+#pragma unroll 1
+    for (int t = 0; t < kTile; ++t) {
+      const int owner = (t & 7) * 4 + (lane & 3);
+      const float w0 = __uint_as_float(__shfl_sync(kFull, t < 8 ? high[0] : high[1], owner));
+      const float w1 = __uint_as_float(__shfl_sync(kFull, t < 8 ? low[0] : low[1], owner));
+      if ((seen >> t & 1u) == 0) continue;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int byte = output_feature(step, lane, half) * static_cast<int>(sizeof(T));
+          const uint32_t from = place_of(at + kValues, t, 0);
+          const float v = load_value((kSwizzled ? from ^ (byte & ~15) : from + (byte & ~15)) + (byte & 15));
+          o[step][2 * half] = fmaf(w0, v, o[step][2 * half]);
+          o[step][2 * half + 1] = fmaf(w1, v, o[step][2 * half + 1]);
+        }
+    }
+  }
+  static __device__ __forceinline__ float load_value(uint32_t from) {
+    uint16_t bits;
+    if constexpr (sizeof(T) == 1) {
+      asm volatile("{\n\t.reg .b32 x;\n\tld.shared.u8 x, [%1];\n\tcvt.u16.u32 %0, x;\n\t}" : "=h"(bits) : "r"(from));
+      T code;
+      code.code = static_cast<decltype(code.code)>(bits);
+      return to_float(code);
+    } else {
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(from));
+      return to_float(*reinterpret_cast<const T*>(&bits));
+    }
+  }
+
   // Raises `before` to the largest score of a head in the tile (the lanes of equal lane % 4 hold its tokens) and
   // returns the factor of what has been added up so far.
   static __device__ __forceinline__ float raise(float x0, float x1, float& before) {
@@ -458,7 +540,8 @@ struct Tensor {
     }
   }
 
-  // Scores to weights.
+  // Scores to weights, in two pieces or (WHOLE) as they are.
+  template <bool WHOLE = false>
   __device__ __forceinline__ void weigh(const AttentionArgs& a, uint32_t at) {
     // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) + {0, 1}
     unsigned seen;
@@ -529,6 +612,11 @@ struct Tensor {
     l[1] += w[0][1] + w[1][1];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      if constexpr (WHOLE) {
+        high[t] = __float_as_uint(u[t][0]);
+        low[t] = __float_as_uint(u[t][1]);
+        continue;
+      }
       float rest0, rest1, none0, none1;
       high[t] = transpose_8x8(pack2<H>(u[t][0], u[t][1], rest0, rest1));
       low[t] = transpose_8x8(pack2<H>(rest0, rest1, none0, none1));

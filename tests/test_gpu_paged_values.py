@@ -1,0 +1,79 @@
+"""Paged attention over values at the ends of their range: infinite ones, and finite ones that a weight above 1 would make
+infinite on the way."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_paged import BF16, E4M3, F16, F32, INT8, TYPES, Case, loaded  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def weights(case):
+    """log2 of the smallest softmax weight of the case, by float64."""
+    least = 0.0
+    for r, n in enumerate(case.lengths.tolist()):
+        t = torch.arange(n)
+        k = case.exact[0][case.col[case.crow[r] + t // case.page], t % case.page]
+        q = case.query[r].double().view(case.kv, -1, case.dim)
+        s = torch.log_softmax(torch.einsum("hgd,thd->hgt", q, k) * case.scale, -1)
+        least = min(least, s.min().item() / 0.6931471805599453)
+    return least
+
+
+def place(case, row, token):
+    return int(case.col[case.crow[row] + token // case.page]), token % case.page
+
+
+@pytest.mark.parametrize("spread", [1.0, 8.0])
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, F16)], ids=str)
+@pytest.mark.parametrize("shape", [(4, 2, 64, 16), (32, 2, 128, 16), (12, 1, 256, 24), (4, 2, 100, 16)], ids=str)
+def test_an_infinite_value_makes_its_feature_infinite(shape, kinds, spread):
+    """Every weight is above 0, so a feature with an infinity is that infinity, with both of them NaN, and the others are what
+    they were, in every head of the group and nowhere else; whatever the tile of the token and the rounding of its weight."""
+    case = Case(shape, kinds, [130, 90, 1, 5000], seed=60, spread=spread)
+    assert weights(case) > -126                                    # float32 holds them all
+    exact, exact_lse, slack, lse_slack, total = case.expected()
+    values = case.pages[1].clone()
+    group = case.heads // case.kv
+    wanted = {}
+    for row, token, head, feature, value in [(0, 0, 0, 5, INF), (0, 77, case.kv - 1, 6, -INF), (0, 129, 0, 7, INF),
+                                             (1, 3, 0, 0, INF), (1, 60, 0, 0, INF), (1, 61, 0, 1, INF), (1, 62, 0, 1, -INF),
+                                             (1, 89, 0, 2, float("nan")), (2, 0, 0, 9, -INF),
+                                             *[(3, 611 * i, 0, i, INF if i % 2 else -INF) for i in range(8)], (3, 4999, 0, 20, INF)]:
+        values[(*place(case, row, token), head, feature)] = value
+        for h in range(head * group, (head + 1) * group):
+            wanted[row, h, feature] = wanted.get((row, h, feature), 0.0) + value
+    out, lse = case.run(value_pages=values)
+    for at, value in wanted.items():
+        got = out[at].item()
+        assert got == value or (value != value and got != got), (at, value, got)
+        exact[at] = 0.0
+        out[at] = 0.0
+    case.check((out, lse), (exact, exact_lse, slack, lse_slack, total))
+
+
+@pytest.mark.parametrize("kinds", [k for k in TYPES if k[1] in (E4M3, INT8)], ids=str)
+@pytest.mark.parametrize("shape", [(4, 2, 64, 16), (24, 2, 128, 16)], ids=str)
+def test_an_infinite_value_scale(shape, kinds):
+    """value = code * scale: infinite by the sign of the code, NaN for a code of 0; the other head and the other rows are what they were."""
+    case = Case(shape, kinds, [130, 90, 1, 5000], seed=61)
+    exact, exact_lse, slack, lse_slack, total = case.expected()
+    group = case.heads // case.kv
+    scales = case.scales[1].clone()
+    codes = case.pages[1].float().cpu()
+    out = {}
+    for row, token in ((0, 33), (3, 4321)):
+        page, at = place(case, row, token)
+        scales[page, 0, at] = INF
+        exact[row, :group] = codes[page, at, 0].double() * INF
+        slack[row, :group] = total[row, :group] = 0.0
+    out, lse = case.run(value_scales=scales)
+    special = ~torch.isfinite(exact)
+    assert torch.equal(out.cpu().double()[special].nan_to_num(nan=7.0), exact[special].nan_to_num(nan=7.0))
+    exact[special] = 0.0
+    out[special.cuda()] = 0.0
+    case.check((out, lse), (exact, exact_lse, slack, lse_slack, total))
