@@ -10,6 +10,11 @@
 // per CTA (the piece it begins with and the piece it ends with), and join_kernel puts them together in the
 // order of the tokens, so results do not depend on timing.  Nothing waits on another CTA.
 //
+// Long sums.  A piece of more than an engine's kLeg units is computed in legs of that many; each ends like a piece, and what it
+// has summed is added to what the legs before it left in the CTA's record.  Added up in one accumulator, the rounding
+// of one sum after the other builds up: 2^20 tokens of equal weight and value in one piece were off by 1.5e-3 in float16
+// (the tensor core cuts its sums off) and by 5e-4 in float32.
+//
 // Softmax: scores are kept in units of log2 (scale * log2(e) is a factor of q or of the score), each warp keeps a running
 // maximum m, sum l and accumulator o of its tokens:
 //   m' = max(m, s),  o' = o 2^(m - m') + 2^(s - m') v,  l' = l 2^(m - m') + 2^(s - m').
@@ -234,12 +239,14 @@ __device__ __forceinline__ void store_four(const AttentionArgs& a, long long row
 }
 
 // The rings' parts of one piece lie in shared memory: ring w's accumulators o[w * ring_stride + g * PITCH + d] and
-// ml[w * GT + g] = (m, l).  Puts them together and stores the result (whole item) or a partial record.  All threads
-// call it between barriers.
+// ml[w * GT + g] = (m, l).  Puts them together with the record of the legs before (`more`) and stores the result (`whole`: the
+// item is complete) or a partial record.  A thread writes and reads the same parts of a record.  All threads call it
+// between barriers.
 template <int THREADS, int GT, int DIM, int PITCH>
-__device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot,
+__device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int kv_head, int sub, int slot, bool more, bool whole,
                                             const float* o, int ring_stride, const float2* ml) {
   __shared__ float4 factors[GT];
+  __shared__ float factors_before[GT];
   static_assert(kRings == 4, "one float4 of factors per head");
   const int heads = min(GT, a.group - sub * GT);
   const long long first_row = static_cast<long long>(row) * a.n_heads + kv_head * a.group + sub * GT;
@@ -253,19 +260,25 @@ __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int
       part[w] = ml[w * GT + tid];
       top = fmaxf(top, part[w].x);
     }
+    float2 before = make_float2(-CUDART_INF_F, 0.f);
+    if (more) before = a.stats[first_record + tid];
+    top = fmaxf(top, before.x);
+    const float f_before = part_factor(before.x, before.y, top);
+    sum = f_before * before.y;
 #pragma unroll
     for (int w = 0; w < kRings; ++w) {
       f[w] = part_factor(part[w].x, part[w].y, top);
       sum += f[w] * part[w].y;
     }
     float scale = 1.f;
-    if (slot < 0) {
+    if (whole) {
       scale = sum == 0.f ? 0.f : 1.f / sum;
       if (a.lse != nullptr) a.lse[first_row + tid] = log_sum(top, sum);
     } else {
       a.stats[first_record + tid] = make_float2(top, sum);
     }
     factors[tid] = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
+    factors_before[tid] = f_before * scale;
   }
   __syncthreads();
   constexpr int kFours = DIM / 4;
@@ -276,10 +289,16 @@ __device__ __forceinline__ void store_piece(const AttentionArgs& a, int row, int
     const float* at = o + g * PITCH + d;
     const float4 x0 = *reinterpret_cast<const float4*>(at), x1 = *reinterpret_cast<const float4*>(at + ring_stride),
                  x2 = *reinterpret_cast<const float4*>(at + 2 * ring_stride), x3 = *reinterpret_cast<const float4*>(at + 3 * ring_stride);
-    const float4 v = make_float4(f.x * x0.x + f.y * x1.x + f.z * x2.x + f.w * x3.x, f.x * x0.y + f.y * x1.y + f.z * x2.y + f.w * x3.y,
+    float4 v = make_float4(f.x * x0.x + f.y * x1.x + f.z * x2.x + f.w * x3.x, f.x * x0.y + f.y * x1.y + f.z * x2.y + f.w * x3.y,
                                  f.x * x0.z + f.y * x1.z + f.z * x2.z + f.w * x3.z, f.x * x0.w + f.y * x1.w + f.z * x2.w + f.w * x3.w);
-    if (slot < 0) store_four(a, first_row + g, d, v);
-    else *reinterpret_cast<float4*>(a.partial + (first_record + g) * a.partial_pitch + d) = v;
+    float4* record = reinterpret_cast<float4*>(a.partial + (first_record + g) * a.partial_pitch + d);
+    if (more) {
+      const float4 x = *record;
+      const float fb = factors_before[g];
+      v = make_float4(v.x + fb * x.x, v.y + fb * x.y, v.z + fb * x.z, v.w + fb * x.w);
+    }
+    if (whole) store_four(a, first_row + g, d, v);
+    else *record = v;
   }
 }
 
@@ -294,12 +313,13 @@ __device__ __forceinline__ void clear_empty_rows(const AttentionArgs& a, int blo
   }
 }
 
-// One piece of a CTA's share.
+// One piece of a CTA's share, or a leg of it.
 struct Piece {
   RowSpan span;
   int row, item, kv_head, sub;
   int entry;          // of the list at which the item's tokens begin
-  int units, u0, u1;  // of the item; the piece's
+  int units, u0, u1;  // of the item; the leg's
+  int from, to;       // the piece's
   __device__ __forceinline__ long long first() const { return span.first + static_cast<long long>(u0) * kUnit; }
   __device__ __forceinline__ long long last() const { return u1 == units ? span.last : span.first + static_cast<long long>(u1) * kUnit; }
   __device__ __forceinline__ bool any() const { return u0 < u1; }
@@ -310,6 +330,7 @@ struct Walk {
   Share s;
   RowSpan span;
   int units, at;  // of the row's items; entry inside the item
+  int began;      // entry inside the item at which the piece begins
   int item, items_per_row;
   __device__ __forceinline__ void begin(int items, const Share& share) {
     s = share;
@@ -325,10 +346,10 @@ struct Walk {
       return;
     }
     item = static_cast<int>(into / entries);
-    at = static_cast<int>(into - item * entries);
+    at = began = static_cast<int>(into - item * entries);
   }
-  // The next piece that has tokens, or one without (all lanes of a warp).
-  __device__ __forceinline__ Piece next(const AttentionArgs& a) {
+  // The next leg, of at most `leg` units, that has tokens, or one without (all lanes of a warp).
+  __device__ __forceinline__ Piece next(const AttentionArgs& a, int leg) {
     Piece p;
     while (s.pos < s.end) {
       const int entries = units + s.start, to = min(entries, at + (s.end - s.pos));
@@ -337,16 +358,22 @@ struct Walk {
       p.item = item;
       p.units = units;
       p.entry = s.pos - at + s.start;
+      const int stop = min(to, max(at, s.start) + leg);
       p.u0 = max(at - s.start, 0);
-      p.u1 = max(to - s.start, 0);
-      s.pos += to - at;
-      at = 0;
-      if (s.pos < s.end && ++item == items_per_row) {
-        item = 0;
-        s.row = next_row(a, s.row);
-        if (s.row >= a.n_rows) s.pos = s.end;
-        else span = row_span(a, s.row);
-        units = span.units();
+      p.u1 = max(stop - s.start, 0);
+      p.from = max(began - s.start, 0);
+      p.to = max(to - s.start, 0);
+      s.pos += stop - at;
+      at = stop;
+      if (stop == to) {
+        at = began = 0;
+        if (s.pos < s.end && ++item == items_per_row) {
+          item = 0;
+          s.row = next_row(a, s.row);
+          if (s.row >= a.n_rows) s.pos = s.end;
+          else span = row_span(a, s.row);
+          units = span.units();
+        }
       }
       if (p.any()) {
         p.kv_head = p.item / a.subgroups;
@@ -430,6 +457,7 @@ __device__ __forceinline__ float fast_log2(float x) {
 __device__ __forceinline__ float published_max(float m) { return m == kNoScore ? -CUDART_INF_F : m; }
 
 // The kernel around an Engine, which computes one ring's part of a piece:
+//   kLeg                              units after which sums are put away
 //   Engine(smem)                      once
 //   fetch(a, piece)                   loads the piece's query; the part of the piece before is still unpublished
 //   start(a, piece)                   begins to copy the piece's tokens
@@ -459,7 +487,7 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       walk.begin(items_per_row, share);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        const Piece p = walk.next(a);
+        const Piece p = walk.next(a, Engine::kLeg);
         if (first_lane) pieces[i] = p;
       }
       if (first_lane) shared_walk = walk;
@@ -479,7 +507,7 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       if (first_warp) {
         Walk walk = shared_walk;
         __syncwarp();  // all lanes have their copy before the first one replaces it
-        const Piece p = walk.next(a);
+        const Piece p = walk.next(a, Engine::kLeg);
         if (first_lane) {
           pieces[after] = p;
           shared_walk = walk;
@@ -501,10 +529,12 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
       if (more) engine.query(a);
       __syncthreads();
       const Piece& p = pieces[now];
-      const int slot = p.u0 > 0 ? 0 : p.u1 < p.units ? 1 : -1;  // -1: a whole item
-      if (slot == 1 && first_lane)  // the CTA of the item's last unit is the one of its last piece
+      const bool ends = p.u1 == p.to, whole = p.from == 0 && p.to == p.units;
+      const int slot = p.from > 0 ? 0 : 1;  // (legs of a whole item: the record of the item that the CTA does not finish is still free)
+      if (slot == 1 && ends && !whole && first_lane)  // the CTA of the item's last unit is the one of its last piece
         a.pieces[blockIdx.x] = make_int4(p.row, p.item, (p.entry + p.units - 1) / shared_walk.s.per_cta - static_cast<int>(blockIdx.x) + 1, 0);
-      store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, p.row, p.kv_head, p.sub, slot, o, Engine::kRingBytes / 4, ml);
+      store_piece<Engine::kThreads, GT, Engine::kDim, Engine::kPitch>(a, p.row, p.kv_head, p.sub, slot, p.u0 > p.from, whole && ends, o,
+                                                                                 Engine::kRingBytes / 4, ml);
       __syncthreads();  // the buffers are free again
       if (!more) break;
       now = next;

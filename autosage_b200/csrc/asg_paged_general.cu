@@ -20,6 +20,9 @@ struct General {
   static constexpr int kHeads = GT;
   static constexpr int kCtasPerSm = CTAS;
   static constexpr int kStages = STAGES;
+  // 1024 sums rounded by 2^-24 at most: 6e-5, one-sided only where all values are alike.  (Legs of 32 units: 2.6 % on 64 rows of up
+  // to 8192 tokens of 4 x 128 with 32 query heads, whose shares are then two legs.)
+  static constexpr int kLeg = 64;
   static constexpr bool kCoded = TypeOf<T>::coded;
   static constexpr int TB = E == 8 || GT == 8 ? 4 : 8;  // tokens per batch
   static constexpr int kBatches = kTile / TB;           // of a tile

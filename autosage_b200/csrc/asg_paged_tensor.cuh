@@ -119,6 +119,7 @@ struct Tensor {
   static constexpr int kHeads = 8 * SHARE;
   static constexpr int kCtasPerSm = CTAS;
   static constexpr int kStages = STAGES;
+  static constexpr int kLeg = 128;  // 2 x 128 sums cut off by 2^-23 at most (mean 2^-24): 3e-5
   static constexpr bool kCoded = TypeOf<T>::coded;
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
   // Rows of 128 bytes: the 16-byte piece c of row r lies at place c ^ (r mod 8); other rows are padded by 16 bytes.

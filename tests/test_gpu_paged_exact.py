@@ -106,3 +106,60 @@ def test_a_crow_whose_rows_overlap_past_2_to_the_32_entries(kinds):
     torch.cuda.synchronize()
     assert out.shape == (rows, 4, 64)
     check(case, case.run())
+
+
+def on_four_pages(kinds, lengths, rows_of_values, dim=64, page=1024, kv=2):
+    """A call whose rows list the same four pages over and over: long rows from little memory.  Queries and keys are such that
+    all weights are 1.  rows_of_values: [4 * page, dim], of values that the type of the pages holds times 2^-6."""
+    from autosage_b200 import paged
+
+    kind, cache = kinds
+    counts = torch.tensor([-(-n // page) for n in lengths])
+    crow = torch.zeros(len(lengths) + 1, dtype=torch.long)
+    torch.cumsum(counts, 0, out=crow[1:])
+    col = torch.cat([torch.arange(int(c)) % 4 for c in counts])
+    values = rows_of_values.view(4, page, 1, dim).expand(4, page, kv, dim)
+    scales = {}
+    if cache in LARGEST:
+        scales = dict(key_scales=torch.ones(4, kv, page, device="cuda"), value_scales=torch.full((4, kv, page), 2.0 ** -6, device="cuda"))
+        values = values * 64
+    values = values.to(cache).contiguous().cuda()
+    keys = torch.ones(4, page, kv, dim, device="cuda").to(cache)
+    out, lse = paged.csr_paged_attention(crow.cuda(), col.cuda(), torch.tensor(lengths).cuda(),
+                                         torch.zeros(len(lengths), 2 * kv, dim, device="cuda", dtype=kind), keys, values,
+                                         return_lse=True, **scales)
+    return out.double().cpu(), lse.double().cpu()
+
+
+@pytest.mark.parametrize("kinds", TYPES, ids=str)
+@pytest.mark.parametrize("lengths", [[2 ** 20 + 77] * 40 + [5, 0, 9000] + [700001] * 3, [3 * 2 ** 20 + 1, 1, 2 ** 21],
+                                     [70000 + 1111 * (r % 13) for r in range(900)]], ids=lambda n: f"{len(n)}x{max(n)}")
+def test_pieces_of_many_legs(lengths, kinds):
+    """Items of many legs, whole in a CTA, cut once or running through several: every token counts once."""
+    marks = torch.zeros(4096, 64)
+    marks[torch.arange(4096), torch.arange(4096) // 16 % 64] = 1
+    out, lse = on_four_pages(kinds, lengths, marks)
+    n = torch.tensor(lengths)
+    whole = torch.bincount(torch.arange(4096) // 16 % 64, minlength=64)
+    exact = torch.stack([(whole * (m // 4096) + torch.bincount(torch.arange(m % 4096) // 16 % 64, minlength=64)).double() / max(m, 1)
+                         for m in lengths])
+    limit = (2.0 ** -23 + HALF_STEP[kinds[0]] * (1 + 2.0 ** -22)) * exact     # as in check()
+    assert bool(((out - exact.unsqueeze(1)).abs() <= limit.unsqueeze(1)).all())
+    some = n > 0
+    assert bool(((lse - torch.log(n.double()).unsqueeze(1))[some].abs() <= 2.0 ** -22 * torch.log(n.double())[some].unsqueeze(1)).all())
+
+
+@pytest.mark.parametrize("kinds", TYPES, ids=str)
+def test_a_million_equal_tokens(kinds):
+    """The mean of equal values is the value, however many there are in one accumulator's way: 1200 rows of 2^20 tokens, more items
+    than CTAs, so that each CTA adds up whole rows."""
+    value = 85 / 64 if kinds[1] != E4M3 else 88 / 64                 # held by every type (with the scale of 2^-6 by the 8-bit ones)
+    out, lse = on_four_pages(kinds, [2 ** 20] * 1200, torch.full((4096, 64), value), kv=1)
+    # sums of a leg, cut off on the tensor cores (2 x 128 of 2^-23 of them) or rounded on the FMA pipe (1024 of 2^-24), one rounding a
+    # leg when it is added to those before (128 legs of 8192 tokens, 256 of 4096), then 1 / n, the product and the type's rounding
+    error = 2.0 ** -14 + 2.0 ** -16 + 2.0 ** -23 if kinds[1] == F32 else 2.0 ** -15 + 2.0 ** -17 + 2.0 ** -23
+    if kinds[0] == F32:
+        assert bool(((out - value).abs() <= (error + 2.0 ** -24) * value).all())
+    else:
+        assert error < HALF_STEP[kinds[0]] / 2 and bool((out == value).all())    # nothing else lies as near
+    assert bool(((lse - torch.log(torch.tensor(2.0 ** 20).double())).abs() <= 2.0 ** -22 * 14).all())
