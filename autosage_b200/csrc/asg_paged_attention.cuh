@@ -19,7 +19,8 @@
 // maximum m, sum l and accumulator o of its tokens:
 //   m' = max(m, s),  o' = o 2^(m - m') + 2^(s - m') v,  l' = l 2^(m - m') + 2^(s - m').
 // m moves only when a score exceeds it by more than kSlack: weights up to 2^kSlack do no harm in float32, and most
-// tiles then need neither the maximum over their lanes nor the rescaling (each of them a third of a tile's work).
+// tiles then need neither the maximum over their lanes nor the rescaling (each of them a third of a tile's work).  Where such a
+// weight makes a sum of very large values infinite, the piece is computed once more without slack (unsound()).
 // With 8-bit pages the key scale multiplies the score and the value scale the weight; codes are never
 // multiplied out in memory.
 #pragma once
@@ -464,6 +465,7 @@ __device__ __forceinline__ float published_max(float m) { return m == kNoScore ?
 //   query(a)                          takes the query and clears the accumulators
 //   run(a)                            the ring's tiles
 //   unsound(a, piece)                 whether a sum that run() has left cannot stand (the same for all lanes of a ring)
+//   drain()                           waits for the copies that were started
 //   run_carefully(a)                  the ring's tiles once more, however long it takes
 //   publish(smem, ml)                 its part into shared memory: float o[kHeads][kPitch] at smem + ring * kRingBytes +
 //                                     kPublish, which no copy of a started piece writes before run()
@@ -514,16 +516,21 @@ __global__ void __launch_bounds__(Engine::kThreads, Engine::kCtasPerSm) attentio
         }
       }
       engine.run(a);
-      if (engine.unsound(a, pieces[now])) {
-        engine.fetch(a, pieces[now]);
-        engine.start(a, pieces[now]);
-        engine.query(a);
-        engine.run_carefully(a);
-      }
       const bool more = pieces[next].any();
       if (more) {
         engine.fetch(a, pieces[next]);
         engine.start(a, pieces[next]);
+      }
+      if (engine.unsound(a, pieces[now])) {  // (looked at while the copies are under way)
+        engine.drain();
+        engine.fetch(a, pieces[now]);
+        engine.start(a, pieces[now]);
+        engine.query(a);
+        engine.run_carefully(a);
+        if (more) {
+          engine.fetch(a, pieces[next]);
+          engine.start(a, pieces[next]);
+        }
       }
       engine.publish(smem, ml);
       if (more) engine.query(a);

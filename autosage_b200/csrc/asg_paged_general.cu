@@ -47,6 +47,7 @@ struct General {
   int lane, place, side, ring;  // lane of the warp, of its token; which of the tokens side by side
   unsigned char* region;
   Source s;
+  float slack = kSlack;
   int batch;                              // of the tile that is copied next
   bool held;                              // of the lane's token of that tile
   long long key_offset, value_offset;     // in bytes
@@ -183,9 +184,27 @@ struct General {
     __syncwarp();
   }
 
-  // (float32 weights, one product a value: what is not finite is the answer)
-  __device__ __forceinline__ bool unsound(const AttentionArgs&, const Piece&) const { return false; }
-  __device__ __forceinline__ void run_carefully(const AttentionArgs& a) { run(a); }
+  // A sum that is not finite may be a large value times a weight above 1: the second time no weight is.
+  __device__ __forceinline__ bool unsound(const AttentionArgs& a, const Piece& p) const {
+    bool any = false;
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+      float zero = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) zero = fmaf(o[g][e], 0.f, zero);
+      any = any || (p.sub * GT + g < a.group && zero != 0.f);
+    }
+    return __any_sync(kFull, any);
+  }
+  __device__ __forceinline__ void drain() const {
+    copy_wait<0>();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void run_carefully(const AttentionArgs& a) {
+    slack = 0.f;
+    run(a);
+    slack = kSlack;
+  }
 
   __device__ __forceinline__ void row_of(float (&x)[E], const unsigned char* at) const {
     const T* from = reinterpret_cast<const T*>(at + lane * kLaneBytes);
@@ -250,7 +269,7 @@ struct General {
       weight_scale = reinterpret_cast<const float*>(at + kExtras)[TB + token];
     }
     const float score = in ? x[0] : -CUDART_INF_F;
-    if (__any_sync(kFull, score > m + kSlack)) {
+    if (__any_sync(kFull, score > m + slack)) {
       const float top = fmaxf(over_tokens(score, [](float a, float b) { return fmaxf(a, b); }), m);
       const float shrink = exp2f(m - top);
       m = top;

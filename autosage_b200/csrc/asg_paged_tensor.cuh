@@ -13,8 +13,9 @@
 // The weights enter as two 16-bit pieces (p = hi + lo, 2^-17 of p lost at most), so that the result is as
 // good as one with float32 weights: the second product costs nothing while the kernel waits for memory.
 // An infinite value times two pieces is not what it is times their sum (lo may be 0 or negative, and so may a weight's hi
-// be 0).  Such a value leaves a sum that is not finite; a ring that ends a piece with one goes through it again and
-// multiplies float32 weights with single values on the FMA pipe (run_carefully), which costs nothing where all is finite.
+// be 0).  Such a value leaves a sum that is not finite, and so may a large one times a weight above 1 (kSlack); a ring
+// that ends a piece with such a sum goes through it again, holds weights to 1 and multiplies them in float32 with single
+// values on the FMA pipe (run_carefully), which costs nothing where all is finite.
 //
 // Each warp works alone (with more than 8 heads, two warps share a ring): 16-token tiles, a ring of kStages tiles in
 // shared memory filled by cp.async 16 bytes at a time (rows swizzled or padded, so ldmatrix is free of bank
@@ -371,15 +372,26 @@ struct Tensor {
     meet();
   }
 
+  // What the accumulators of head h are multiplied with in the end.
+  __device__ __forceinline__ float undo(int h) const {
+    constexpr float lower = kLift == 0.f ? 1.f : 1.f / 256.f;
+    static_assert(kLift == 0.f || kLift == 8.f, "2^-kLift");
+    return kCoded ? lower * power_of_two(d[h]) : lower;
+  }
+
   // Whether a sum of the piece's heads is not finite: 0 times it is not 0.
   __device__ __forceinline__ bool unsound(const AttentionArgs& a, const Piece& p) const {
     bool any = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float zero = 0.f;
+      const float back = undo(h);
+      float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) zero = fmaf(o[step][h], 0.f, fmaf(o[step][2 + h], 0.f, zero));
-      any = any || (p.sub * kHeads + 8 * part + 2 * (lane & 3) + h < a.group && zero != 0.f);
+      for (int step = 0; step < kSteps; ++step) {
+        zero[step & 1] = fmaf(kCoded ? o[step][h] * back : o[step][h], 0.f, zero[step & 1]);
+        zero[2 + (step & 1)] = fmaf(kCoded ? o[step][2 + h] * back : o[step][2 + h], 0.f, zero[2 + (step & 1)]);
+      }
+      any = any || (p.sub * kHeads + 8 * part + 2 * (lane & 3) + h < a.group && (zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.f);
     }
     if constexpr (SHARE == 1) {
       any = __any_sync(kFull, any);
@@ -390,6 +402,11 @@ struct Tensor {
       any = ring_any != 0;
     }
     return any;
+  }
+
+  __device__ __forceinline__ void drain() const {
+    copy_wait<0>();
+    meet();
   }
 
   __device__ __forceinline__ void run_carefully(const AttentionArgs& a) {
@@ -541,7 +558,7 @@ struct Tensor {
     }
   }
 
-  // Scores to weights, in two pieces or (WHOLE) as they are.
+  // Scores to weights, in two pieces or (WHOLE) as they are and at most 1.
   template <bool WHOLE = false>
   __device__ __forceinline__ void weigh(const AttentionArgs& a, uint32_t at) {
     // this lane's scores: tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) + {0, 1}
@@ -577,12 +594,13 @@ struct Tensor {
     };
     powers();
     float largest = fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[1][0], w[1][1]));
+    if constexpr (WHOLE) largest *= 64.f;  // (no slack)
     if constexpr (kCoded) {
       const float other = fmaxf(fmaxf(fabsf(u[0][0]), fabsf(u[0][1])), fmaxf(fabsf(u[1][0]), fabsf(u[1][1])));
       largest = fmaxf(largest, other);
     }
     constexpr float limit = kLift == 0.f ? 64.f : 16384.f;
-    static_assert(kSlack == 6.f, "2^(kSlack + kLift)");
+    static_assert(kSlack == 6.f, "2^kSlack, 2^(kSlack + kLift)");
     if (__any_sync(kFull, largest > limit)) {
       float shrink[2];
 #pragma unroll
@@ -626,8 +644,7 @@ struct Tensor {
 
   __device__ __forceinline__ void publish(unsigned char* smem, float2* ml) {
     float* to = reinterpret_cast<float*>(smem + ring * kRingBytes + kPublish);
-    constexpr float undo = kLift == 0.f ? 1.f : 1.f / 256.f;
-    static_assert(kLift == 0.f || kLift == 8.f, "2^-kLift");
+    constexpr float lower = kLift == 0.f ? 1.f : 1.f / 256.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int head = 8 * part + 2 * (lane & 3) + h;
@@ -635,8 +652,8 @@ struct Tensor {
       sum += __shfl_xor_sync(kFull, sum, 4);
       sum += __shfl_xor_sync(kFull, sum, 8);
       sum += __shfl_xor_sync(kFull, sum, 16);
-      if (lane < 4) ml[ring * kHeads + head] = make_float2(published_max(m[h]), sum * undo);
-      const float back = kCoded ? undo * power_of_two(d[h]) : undo;
+      if (lane < 4) ml[ring * kHeads + head] = make_float2(published_max(m[h]), sum * lower);
+      const float back = undo(h);
 #pragma unroll
       for (int step = 0; step < kSteps; ++step)
 #pragma unroll

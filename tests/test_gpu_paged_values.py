@@ -77,3 +77,39 @@ def test_an_infinite_value_scale(shape, kinds):
     exact[special] = 0.0
     out[special.cuda()] = 0.0
     case.check((out, lse), (exact, exact_lse, slack, lse_slack, total))
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F32, E4M3), (BF16, E4M3), (BF16, INT8), (F32, INT8)], ids=str)
+@pytest.mark.parametrize("shape", [(4, 2, 64, 16), (24, 2, 128, 16), (4, 2, 100, 16), (6, 1, 256, 7)], ids=str)
+def test_large_values_whose_scores_rise(shape, kinds):
+    """The value of the highest score is near the largest number, and scores have risen by less than a factor of 2^6 before: no weight
+    above 1 may make it infinite."""
+    case = Case(shape, kinds, [65, 200, 700, 1, 9000], seed=62)
+    case.query = torch.zeros_like(case.query)
+    case.query[:, :, 0] = 1
+    case.scale = 1.0
+    gen = torch.Generator().manual_seed(63)
+    scores = -30 * torch.rand(case.pages[0].shape[:3], generator=gen) - 20
+    size = torch.ones(scores.shape)
+    for row, n in enumerate(case.lengths.tolist()):
+        for t, score in ((0, 0.0), (64, 3.4), (128, 6.9), (8000, 7.1)):   # every fourth tile is of the same ring
+            if t < n:
+                scores[place(case, row, t)] = score
+        size[place(case, row, next(t for t in (8000, 128, 64, 0) if t < n))] = 2.0 ** 123
+    if case.scales[0] is None:
+        keys, values = torch.zeros(case.pages[0].shape), case.pages[1].cpu().float().nan_to_num(0.0).clamp(-4, 4)
+        keys[..., 0] = scores
+        pools = [keys.to(case.cache), (values * size.unsqueeze(-1)).to(case.cache)]
+        case.exact = [x.double() for x in pools]
+    else:
+        keys = torch.zeros(case.pages[0].shape)
+        keys[..., 0] = 64
+        values = case.pages[1].cpu().float().nan_to_num(0.0)
+        pools = [keys.to(case.cache), case.pages[1].cpu()]
+        scales = [scores / 64, size * (2.0 ** -6 if kinds[1] == E4M3 else 2.0 ** -4)]
+        case.scales = [s.transpose(1, 2).contiguous().cuda() for s in scales]
+        case.exact = [k.double() * s.double().unsqueeze(-1) for k, s in zip((keys, values), scales)]
+    case.pages = [x.cuda() for x in pools]
+    expected = case.expected()
+    assert bool((expected[0].abs().amax(-1) < 2.0 ** 127).all()) and expected[0].abs().max() > 2.0 ** 122
+    case.check(case.run(), expected)
