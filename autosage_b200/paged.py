@@ -14,7 +14,8 @@ bfloat16, float16, ``float8_e4m3fn`` or int8, with any strides whose features ar
 go with float32 scales ``[n_pages, n_kv_heads, page_size]``, one for each row of ``head_dim`` features: value =
 code * scale.  A slot is ``page * page_size + place in the page``.
 
-These are operators of inference: there is no backward, and a call that would need one is refused.  The reference
+These are operators of inference: they have no backward and no forward-mode derivative, and a call that would need one is
+refused.  The reference
 has no counterpart (its attention, ``autosage/_auto.py:762-780``, is the whole-pattern form).
 """
 from __future__ import annotations
@@ -23,6 +24,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native, ops
 
@@ -93,13 +95,21 @@ def _check_pages(key_pages, value_pages, key_scales, value_scales) -> torch.Size
     return shape
 
 
-def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    if device.type != "cuda":
-        raise RuntimeError("the paged cache needs CUDA tensors")
+def _refuse_derivatives(*tensors: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled():
         for tensor in tensors:
             if tensor is not None and tensor.requires_grad:
                 raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:   # (no_grad() does not end forward mode)
+        for tensor in tensors:
+            if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+                raise RuntimeError("the paged cache has no forward-mode derivative; call it with the primal parts of its inputs")
+
+
+def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    _refuse_derivatives(*tensors)
+    if device.type != "cuda":
+        raise RuntimeError("the paged cache needs CUDA tensors")
     if _native._LIB is None and not ops.load_native():
         detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")
