@@ -24,6 +24,7 @@ import os
 from typing import Optional
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 from torch.autograd import forward_ad
 
 from . import _native, ops
@@ -110,6 +111,9 @@ def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> N
     _refuse_derivatives(*tensors)
     if device.type != "cuda":
         raise RuntimeError("the paged cache needs CUDA tensors")
+    for tensor in tensors:
+        if isinstance(tensor, FakeTensor):   # its address is 0, and a workspace made beside it would be one too
+            raise RuntimeError("the paged cache needs tensors with memory, not fake ones")
     if _native._LIB is None and not ops.load_native():
         detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")

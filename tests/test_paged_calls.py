@@ -6,7 +6,7 @@ import struct
 import pytest
 import torch
 
-from autosage_b200 import _native
+from autosage_b200 import _native, paged
 
 WORKSPACE = 35            # field of asg_paged_attention_args, counted in eights of bytes
 
@@ -64,3 +64,19 @@ def test_the_attention_has_a_workspace_of_its_own(recorder):
     attend()
     assert recorder.attention[1][WORKSPACE] == recorder.attention[0][WORKSPACE]     # kept between calls
     assert other().data_ptr() == shared.data_ptr()
+
+
+def test_fake_tensors_are_refused_and_leave_no_workspace(recorder):
+    """A fake tensor's address is 0; a workspace allocated among them would be fake too and serve the calls after it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        pages = [torch.zeros(3, 4, 2, 8, device="cuda") for _ in range(2)]
+        crow, col, lengths = (torch.zeros(n, dtype=torch.long, device="cuda") for n in (3, 3, 2))
+        rows = torch.zeros(2, 2, 8, device="cuda")
+        for call in (lambda: paged.csr_paged_attention(crow, col, lengths, rows, *pages),
+                     lambda: paged.paged_cache_write(lengths, rows, rows, *pages),
+                     lambda: paged.paged_cache_read(lengths, *pages)):
+            with pytest.raises(RuntimeError, match="not fake ones"):
+                call()
+    assert recorder.attention == recorder.written == [] and _native._SCRATCH == {}
