@@ -159,8 +159,12 @@ def workspace_bytes(n_rows: int) -> int:
     return int(library().asg_workspace_bytes(int(n_rows)))
 
 
-def _capturing() -> bool:
-    return torch.cuda.is_current_stream_capturing()
+def _capturing(index: Optional[int] = None) -> bool:
+    """Whether the stream that a launch on GPU ``index`` (the current one) goes to is being captured."""
+    if index is None or index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def scratch(device: torch.device, n_rows: int, extra_bytes: int = 0) -> torch.Tensor:
@@ -170,7 +174,7 @@ def scratch(device: torch.device, n_rows: int, extra_bytes: int = 0) -> torch.Te
 
 def _scratch_on(device: torch.device, index: int, stream: int, need: int, *owner: str) -> torch.Tensor:
     """The buffer of (device, stream), or the one of its own that an ``owner`` has there."""
-    if _capturing():
+    if _capturing(index):
         # a captured launch keeps the raw pointer: the buffer has to come from the graph's own pool
         # (and so live as long as the graph), not from a cache that may replace it later
         return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
@@ -487,8 +491,9 @@ def paged_cache_read(slots, key, value, key_pages, value_pages, key_scales, valu
 
 
 @functools.lru_cache(maxsize=None)
-def _paged_attention_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
-    return int(library().asg_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim))
+def _paged_attention_bytes(index: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    with torch.cuda.device(index):   # the library goes by the SMs of the current GPU
+        return int(library().asg_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim))
 
 
 def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages, key_scales, value_scales, scale: float,
@@ -501,7 +506,8 @@ def paged_attention(crow, col, lengths, query, out, lse, key_pages, value_pages,
     stream = _raw_stream(device.index)
     # a buffer of its own: the launches of a call are kept together among calls of this operator only, so another
     # host thread's SpMM on the same stream may come between the kernel that fills the workspace and the one that reads it
-    workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(n_heads, n_kv_heads, head_dim), "paged_attention")
+    workspace = _scratch_on(device, device.index, stream, _paged_attention_bytes(device.index, n_heads, n_kv_heads, head_dim),
+                            "paged_attention")
     code = library().asg_paged_attention(_ATTENTION_ARGS.pack(
         crow.data_ptr(), col.data_ptr(), lengths.data_ptr(), n_rows, col.numel(), query.data_ptr(), q_token, q_head,
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), *_page_pools(key_pages, value_pages, key_scales, value_scales), n_pages, page_size, n_heads, n_kv_heads, head_dim, window,

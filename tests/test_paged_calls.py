@@ -26,11 +26,26 @@ class Recorder:
         return 0
 
     def asg_paged_attention_workspace_bytes(self, n_heads, n_kv_heads, head_dim):
-        self.sizes.append((n_heads, n_kv_heads, head_dim))
-        return 4096
+        self.sizes.append((torch.cuda.current_device(), n_heads, n_kv_heads, head_dim))
+        return 4096 * (1 + torch.cuda.current_device())
 
     def asg_workspace_bytes(self, n_rows):
         return 4096
+
+
+class Current:
+    """Stands in for torch.cuda.device: two GPUs, the first of them current."""
+
+    index, capturing = 0, set()
+
+    def __init__(self, index):
+        self.wanted = 0 if index is None else index
+
+    def __enter__(self):
+        self.before, Current.index = Current.index, self.wanted
+
+    def __exit__(self, *_):
+        Current.index = self.before
 
 
 @pytest.fixture
@@ -38,8 +53,10 @@ def recorder(monkeypatch):
     library = Recorder()
     monkeypatch.setattr(_native, "_LIB", library)
     monkeypatch.setattr(_native, "_SCRATCH", {})
-    monkeypatch.setattr(_native, "_capturing", lambda *index: False)
-    monkeypatch.setattr(_native, "_stream", lambda device: 7)
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: Current.index)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: Current.index in Current.capturing)
+    monkeypatch.setattr(Current, "capturing", set())
     monkeypatch.setattr(_native, "_raw_stream", lambda index: 7)
     _native._paged_attention_bytes.cache_clear()
     yield library
@@ -64,6 +81,42 @@ def test_the_attention_has_a_workspace_of_its_own(recorder):
     attend()
     assert recorder.attention[1][WORKSPACE] == recorder.attention[0][WORKSPACE]     # kept between calls
     assert other().data_ptr() == shared.data_ptr()
+
+
+def on_gpu(index):
+    """The arguments of a call whose tensors say that they lie on GPU `index`."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        pages = [torch.zeros(3, 4, 2, 8, device=f"cuda:{index}") for _ in range(2)]
+        crow, col, lengths = (torch.zeros(n, dtype=torch.long, device=f"cuda:{index}") for n in (3, 3, 2))
+        query, out = (torch.zeros(2, 4, 8, device=f"cuda:{index}") for _ in range(2))
+    return crow, col, lengths, query, out, None, *pages, None, None, 1.0, 0
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_the_workspace_is_sized_for_the_gpu_of_the_tensors(recorder, monkeypatch):
+    """Not for the current one, nor for the one that the first call went to."""
+    asked = []
+
+    def scratch_on(device, index, stream, need, *owner):
+        asked.append((index, need))
+        return torch.zeros(8192, dtype=torch.uint8)
+
+    monkeypatch.setattr(_native, "_scratch_on", scratch_on)
+    for index in (0, 1, 0, 1):
+        _native.paged_attention(*on_gpu(index))
+    assert asked == [(0, 4096), (1, 8192), (0, 4096), (1, 8192)] and Current.index == 0
+    assert recorder.sizes == [(0, 4, 2, 8), (1, 4, 2, 8)]           # asked of the library once a GPU
+
+
+def test_capture_is_asked_of_the_gpu_that_is_launched_on(recorder):
+    Current.capturing.add(1)
+    kept = _native._scratch_on(torch.device("cpu"), 0, 7, 100, "paged_attention")
+    assert _native._scratch_on(torch.device("cpu"), 0, 7, 100, "paged_attention") is kept
+    # what is captured on the other GPU comes from the graph's pool, whatever GPU is current
+    first, second = (_native._scratch_on(torch.device("cpu"), 1, 7, 100, "paged_attention") for _ in range(2))
+    assert first is not second and list(_native._SCRATCH) == [(0, 7, "paged_attention")]
 
 
 def test_fake_tensors_are_refused_and_leave_no_workspace(recorder):
