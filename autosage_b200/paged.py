@@ -171,9 +171,9 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
             raise RuntimeError("two tokens have the same slot")
     _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
                               key_scales, value_scales)
-    if not key_pages.is_inference():   # as after any operation in place
-        torch.autograd.graph.increment_version(
-            (key_pages, value_pages) if key_scales is None else (key_pages, value_pages, key_scales, value_scales))
+    # as after any operation in place; tensors made in inference mode keep no count
+    torch.autograd.graph.increment_version([tensor for tensor in (key_pages, value_pages, key_scales, value_scales)
+                                            if tensor is not None and not tensor.is_inference()])
 
 
 def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, *,

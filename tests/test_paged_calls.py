@@ -133,3 +133,21 @@ def test_fake_tensors_are_refused_and_leave_no_workspace(recorder):
             with pytest.raises(RuntimeError, match="not fake ones"):
                 call()
     assert recorder.attention == recorder.written == [] and _native._SCRATCH == {}
+
+
+@pytest.mark.parametrize("made_in_inference", [(0,), (1,), (2,), (3,), (0, 2), (1, 3), (0, 1, 2, 3), ()], ids=str)
+@pytest.mark.parametrize("later", [False, True], ids=["outside", "in inference mode"])
+def test_a_write_counts_on_each_tensor_that_counts(recorder, monkeypatch, made_in_inference, later):
+    """Tensors made in inference mode and others may be mixed: the write is made, and the others' versions rise."""
+    monkeypatch.setattr(paged, "_require_native", lambda *_: None)
+    monkeypatch.setattr(_native, "_page_pools", lambda *_: (0,) * 16)
+    tensors = []
+    for i, make in enumerate([lambda: torch.zeros(3, 4, 2, 8, dtype=torch.int8)] * 2 + [lambda: torch.zeros(3, 2, 4)] * 2):
+        with torch.inference_mode(i in made_in_inference):
+            tensors.append(make())
+    before = {i: t._version for i, t in enumerate(tensors) if i not in made_in_inference}
+    rows = torch.zeros(2, 2, 8)
+    with torch.inference_mode(later):
+        paged.paged_cache_write(torch.tensor([1, 2]), rows, rows, *tensors[:2], key_scales=tensors[2], value_scales=tensors[3])
+    assert len(recorder.written) == 1
+    assert all(tensors[i]._version == version + 1 for i, version in before.items())
