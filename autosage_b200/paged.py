@@ -143,8 +143,8 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     NaN reads back as NaN.
 
     A slot outside the pages (-1, say) is skipped: padding.  The others must differ from one another: of two tokens
-    with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call).  ``key`` and ``value``
-    do not share memory with the slots that are written."""
+    with the same slot, what is kept is a mixture (``AUTOSAGE_CHECK_INDICES=1`` refuses such a call).  Neither ``key`` and
+    ``value`` nor other pages or scales of the call share memory with the slots that are written."""
     n_pages, page_size, heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
     shape = key.shape
     if len(shape) != 3 or shape != value.shape or shape[1] != heads or shape[2] != dim:
@@ -163,6 +163,10 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
                          ("value_scales", value_scales)):
         _check_writable(name, tensor)
     _require_native(device, key, value, key_pages, value_pages, key_scales, value_scales)
+    if n_pages and (key_pages.data_ptr() == value_pages.data_ptr()
+                    or (key_scales is not None and key_scales.data_ptr() == value_scales.data_ptr())):
+        if key.data_ptr() != value.data_ptr() or key.stride() != value.stride():   # one tensor for both is written twice alike
+            raise ValueError("different keys and values cannot be written to the same pages or scales")
     if slots.numel() == 0 or n_pages == 0:
         return
     if _checking():

@@ -151,3 +151,21 @@ def test_a_write_counts_on_each_tensor_that_counts(recorder, monkeypatch, made_i
         paged.paged_cache_write(torch.tensor([1, 2]), rows, rows, *tensors[:2], key_scales=tensors[2], value_scales=tensors[3])
     assert len(recorder.written) == 1
     assert all(tensors[i]._version == version + 1 for i, version in before.items())
+
+
+def test_keys_and_values_are_not_written_to_the_same_memory(recorder, monkeypatch):
+    monkeypatch.setattr(paged, "_require_native", lambda *_: None)
+    one, other = torch.zeros(3, 4, 2, 8), torch.zeros(3, 4, 2, 8)
+    rows, others = torch.zeros(2, 2, 8), torch.zeros(2, 2, 8)
+    slots = torch.tensor([1, 2])
+    with pytest.raises(ValueError, match="to the same pages or scales"):
+        paged.paged_cache_write(slots, rows, others, one, one)
+    codes, scales = [x.to(torch.int8) for x in (one, other)], torch.zeros(3, 2, 4)
+    with pytest.raises(ValueError, match="to the same pages or scales"):
+        paged.paged_cache_write(slots, rows, others, *codes, key_scales=scales, value_scales=scales)
+    assert recorder.written == []
+    both = torch.zeros(3, 2, 4, 2, 8)                      # interleaved, but not the same
+    paged.paged_cache_write(slots, rows, others, both[:, 0], both[:, 1])
+    paged.paged_cache_write(slots, rows, others, one[:0], one[:0])   # no pages: nothing is written
+    paged.paged_cache_write(slots, rows, rows, one, one)             # keys that are the values
+    assert len(recorder.written) == 2
