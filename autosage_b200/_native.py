@@ -159,9 +159,12 @@ def workspace_bytes(n_rows: int) -> int:
     return int(library().asg_workspace_bytes(int(n_rows)))
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _capturing(index: Optional[int] = None) -> bool:
     """Whether the stream that a launch on GPU ``index`` (the current one) goes to is being captured."""
-    if index is None or index == torch.cuda.current_device():
+    if index is None or index == _current_device():
         return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(index):
         return torch.cuda.is_current_stream_capturing()

@@ -16,9 +16,13 @@
 //     product x w with w = (1 / s) (1 + 2^-21 sign(e)) decides every code: its own error, below 2^-22, moves
 //     nothing across a border, and what lies on a border goes where e sends it.  For e = 0 the quotient is
 //     corrected by its remainder instead, which gives a quotient on a border exactly, and the tie rule holds.
-//   float32 x.  The quotient is rounded "to odd": correctly rounded by one multiply with 1/s and two fused
-//     multiply-adds, then its last bit is set towards the sign of the exact remainder x - q s.  Borders have
-//     an even last bit, so rounding that value to a code gives the code nearest to the true quotient.
+//   float32 x.  The quotient is rounded "to odd" (Boldo and Melquiond, Emulation of FMA and correctly rounded sums, IEEE
+//     Trans. Computers 2008: a value so rounded can be rounded again as if it were exact).  With y = 1 / s correctly rounded,
+//     q0 = x y is within a unit in the last place of the quotient, and q = q0 + y (x - q0 s), the inner term by a fused
+//     multiply-add, is the correctly rounded one (Markstein, Computation of elementary functions on the IBM RISC System/6000,
+//     IBM J. Res. Dev. 1990).  All that is needed of it here is that the quotient lies between q and a neighbour: the
+//     remainder x - q s is then exact, its sign names that neighbour, and of the two the one with an odd last bit is taken.
+//     Borders have an even last bit, so rounding that value to a code gives the code nearest to the true quotient.
 //   Scales so small or large that 1/s or a remainder would leave float32's range: division in float64.
 #include "asg_paged.cuh"
 
@@ -85,14 +89,7 @@ constexpr int kThreads = 256;
 constexpr float largest_code(E4M3) { return 448.f; }
 constexpr float largest_code(INT8) { return 127.f; }
 
-// 1 / s within one unit in the last place, s in [2^-90, 2^90].
-__device__ __forceinline__ float reciprocal(float s) {
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  return fmaf(fmaf(-inv, s, 1.f), inv, inv);
-}
-
-// x / s, rounded to odd in float32; inv = 1 / s, s in [2^-90, 2^90].
+// x / s, rounded to odd in float32; inv = 1 / s, correctly rounded, s in [2^-90, 2^90].
 __device__ __forceinline__ float quotient_to_odd(float x, float s, float inv) {
   const float q0 = x * inv;
   const float q = fmaf(fmaf(-q0, s, x), inv, q0);
@@ -205,10 +202,10 @@ __device__ __forceinline__ float quantise(const Pack<IN, N>& x, float top, Pack<
   to_floats(x, v);
   float s;
   if (top > 0x1p-80f && top < 0x1p90f) {
-    constexpr float share = 1.f / most;
+    constexpr float share = 1.f / most;  // correctly rounded, so that the same theorem gives the scale
     s = top * share;
-    s = fmaf(fmaf(-s, most, top), share, s);  // top / most, correctly rounded (checked for every mantissa)
-    const float inv = reciprocal(s);
+    s = fmaf(fmaf(-s, most, top), share, s);
+    const float inv = __frcp_rn(s);
     if constexpr (sizeof(IN) == 2) {
       const float off = fmaf(-s, most, top);  // exact; its sign is that of e
       if (off != 0.f) {
@@ -411,6 +408,11 @@ int asg_paged_cache_write(const asg_paged_cache_args* args) {
   ASG_REQUIRE(is_coded(args->cache_type) || args->cache_type == args->token_type, ASG_EINVAL,
               "the pages must have the type of the tokens or an 8-bit type");
   if (a.n_tokens == 0 || a.n_slots == 0) return ASG_OK;
+  // one tensor for keys and values is written twice alike
+  const bool same_tokens = a.same_rows && a.rows[0].data == a.rows[1].data;
+  ASG_REQUIRE(same_tokens || (a.pools[0].data != a.pools[1].data &&
+                              (!is_coded(args->cache_type) || a.pools[0].scales != a.pools[1].scales)), ASG_EINVAL,
+              "different keys and values cannot be written to the same pages or scales");
   DeviceGuard guard(a.pools[0].data);
   ASG_CUDA(guard.status);
   cudaStream_t stream = static_cast<cudaStream_t>(args->stream);

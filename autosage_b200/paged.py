@@ -31,18 +31,18 @@ from . import _native, ops
 
 _WIDE = (torch.float32, torch.bfloat16, torch.float16)
 _CODED = (torch.float8_e4m3fn, torch.int8)
-_INDEX_DTYPES = (torch.int32, torch.int64)
 MAX_HEAD_DIM = 256
 
 
 def _index(name: str, tensor: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if tensor.dtype not in _INDEX_DTYPES:
+    dtype = tensor.dtype
+    if dtype is not torch.int64 and dtype is not torch.int32:
         raise TypeError(f"{name} must use integer indices")
     if tensor.dim() != 1:
         raise ValueError(f"{name} must be one-dimensional")
     if tensor.device != device:
         raise ValueError(f"{name} must be on the device of the pages")
-    if tensor.dtype is not torch.int64:
+    if dtype is not torch.int64:
         tensor = tensor.to(torch.int64)
     return tensor if tensor.is_contiguous() else tensor.contiguous()
 
@@ -82,7 +82,7 @@ def _check_pages(key_pages, value_pages, key_scales, value_scales) -> torch.Size
     shape, dtype, device = key_pages.shape, key_pages.dtype, key_pages.device
     fine = (len(shape) == 4 and shape == value_pages.shape and shape[1] > 0 and shape[2] > 0 and 0 < shape[3] <= MAX_HEAD_DIM
             and value_pages.dtype is dtype and value_pages.device == device
-            and ((key_pages.stride(3) == 1 and value_pages.stride(3) == 1) or shape[3] == 1))
+            and ((key_pages.stride()[3] == 1 and value_pages.stride()[3] == 1) or shape[3] == 1))
     if fine and _native.TYPES.get(dtype, 9) <= 2:
         fine = key_scales is None and value_scales is None
     elif fine:
@@ -96,24 +96,21 @@ def _check_pages(key_pages, value_pages, key_scales, value_scales) -> torch.Size
     return shape
 
 
-def _refuse_derivatives(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for tensor in tensors:
-            if tensor is not None and tensor.requires_grad:
-                raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
+def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+    grad = torch.is_grad_enabled()
+    for tensor in tensors:
+        if tensor is None:
+            continue
+        if grad and tensor.requires_grad:
+            raise RuntimeError("the paged cache has no backward; call it under torch.no_grad() or detach its inputs")
+        if type(tensor) is FakeTensor:   # its address is 0, and a workspace made beside it would be one too
+            raise RuntimeError("the paged cache needs tensors with memory, not fake ones")
     if forward_ad._current_level >= 0:   # (no_grad() does not end forward mode)
         for tensor in tensors:
             if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
                 raise RuntimeError("the paged cache has no forward-mode derivative; call it with the primal parts of its inputs")
-
-
-def _require_native(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
-    _refuse_derivatives(*tensors)
     if device.type != "cuda":
         raise RuntimeError("the paged cache needs CUDA tensors")
-    for tensor in tensors:
-        if isinstance(tensor, FakeTensor):   # its address is 0, and a workspace made beside it would be one too
-            raise RuntimeError("the paged cache needs tensors with memory, not fake ones")
     if _native._LIB is None and not ops.load_native():
         detail = f": {ops.native_load_error()}" if ops.native_load_error() else ""
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable{detail}")
@@ -127,10 +124,11 @@ def _checking() -> bool:
     return os.environ.get("AUTOSAGE_CHECK_INDICES") == "1"
 
 
-def _check_writable(name: str, tensor: Optional[torch.Tensor]) -> None:
-    if tensor is not None and 0 in tensor.stride() and any(
-            step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
-        raise ValueError(f"{name} is written and must not repeat memory (it has a stride of 0)")
+def _check_writable(**tensors: Optional[torch.Tensor]) -> None:
+    for name, tensor in tensors.items():
+        if tensor is not None and 0 in tensor.stride() and any(
+                step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
+            raise ValueError(f"{name} is written and must not repeat memory (it has a stride of 0)")
 
 
 def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
@@ -159,14 +157,8 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     slots = _index("slots", slots, device)
     if slots.numel() != shape[0]:
         raise ValueError("slots must contain one slot per token")
-    for name, tensor in (("key_pages", key_pages), ("value_pages", value_pages), ("key_scales", key_scales),
-                         ("value_scales", value_scales)):
-        _check_writable(name, tensor)
+    _check_writable(key_pages=key_pages, value_pages=value_pages, key_scales=key_scales, value_scales=value_scales)
     _require_native(device, key, value, key_pages, value_pages, key_scales, value_scales)
-    if n_pages and (key_pages.data_ptr() == value_pages.data_ptr()
-                    or (key_scales is not None and key_scales.data_ptr() == value_scales.data_ptr())):
-        if key.data_ptr() != value.data_ptr() or key.stride() != value.stride():   # one tensor for both is written twice alike
-            raise ValueError("different keys and values cannot be written to the same pages or scales")
     if slots.numel() == 0 or n_pages == 0:
         return
     if _checking():
@@ -176,8 +168,12 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     _native.paged_cache_write(slots, _contiguous_features(key), _contiguous_features(value), key_pages, value_pages,
                               key_scales, value_scales)
     # as after any operation in place; tensors made in inference mode keep no count
-    torch.autograd.graph.increment_version([tensor for tensor in (key_pages, value_pages, key_scales, value_scales)
-                                            if tensor is not None and not tensor.is_inference()])
+    written = (key_pages, value_pages) if key_scales is None else (key_pages, value_pages, key_scales, value_scales)
+    for tensor in written:
+        if tensor.is_inference():
+            written = [tensor for tensor in written if not tensor.is_inference()]
+            break
+    torch.autograd.graph.increment_version(written)
 
 
 def paged_cache_read(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, *,

@@ -55,6 +55,7 @@ def recorder(monkeypatch):
     monkeypatch.setattr(_native, "_SCRATCH", {})
     monkeypatch.setattr(torch.cuda, "device", Current)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: Current.index)
+    monkeypatch.setattr(_native, "_current_device", lambda: Current.index)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: Current.index in Current.capturing)
     monkeypatch.setattr(Current, "capturing", set())
     monkeypatch.setattr(_native, "_raw_stream", lambda index: 7)
@@ -153,19 +154,18 @@ def test_a_write_counts_on_each_tensor_that_counts(recorder, monkeypatch, made_i
     assert all(tensors[i]._version == version + 1 for i, version in before.items())
 
 
-def test_keys_and_values_are_not_written_to_the_same_memory(recorder, monkeypatch):
-    monkeypatch.setattr(paged, "_require_native", lambda *_: None)
-    one, other = torch.zeros(3, 4, 2, 8), torch.zeros(3, 4, 2, 8)
-    rows, others = torch.zeros(2, 2, 8), torch.zeros(2, 2, 8)
-    slots = torch.tensor([1, 2])
-    with pytest.raises(ValueError, match="to the same pages or scales"):
-        paged.paged_cache_write(slots, rows, others, one, one)
-    codes, scales = [x.to(torch.int8) for x in (one, other)], torch.zeros(3, 2, 4)
-    with pytest.raises(ValueError, match="to the same pages or scales"):
-        paged.paged_cache_write(slots, rows, others, *codes, key_scales=scales, value_scales=scales)
-    assert recorder.written == []
-    both = torch.zeros(3, 2, 4, 2, 8)                      # interleaved, but not the same
-    paged.paged_cache_write(slots, rows, others, both[:, 0], both[:, 1])
-    paged.paged_cache_write(slots, rows, others, one[:0], one[:0])   # no pages: nothing is written
-    paged.paged_cache_write(slots, rows, rows, one, one)             # keys that are the values
-    assert len(recorder.written) == 2
+def test_keys_and_values_are_not_written_to_the_same_memory(native_library):
+    """The library says so before any CUDA call."""
+    lib = _native.bind(str(native_library))
+
+    def write(key=256, value=512, key_pages=1024, value_pages=2048, key_scales=0, value_scales=0, cache=0, n_tokens=2):
+        pools = (key_pages, key_scales, 64, 16, 8, 0, 0, 0, value_pages, value_scales, 64, 16, 8, 0, 0, 0)
+        code = lib.asg_paged_cache_write(_native._CACHE_ARGS.pack(128, n_tokens, key, 16, 8, value, 16, 8, *pools, 3, 4, 2, 8, 0, cache, 0))
+        return code == -1 and b"to the same pages or scales" in lib.asg_last_error_string()
+
+    assert write(value_pages=1024)
+    assert write(cache=4, key_scales=4096, value_scales=4096)
+    assert write(cache=4, key_scales=4096, value_scales=8192, value_pages=1024)
+    assert not write(value_pages=1024, n_tokens=0)
+    if not torch.cuda.is_available():                      # (with a GPU these would be launched)
+        assert not write() and not write(value=256, value_pages=1024)
