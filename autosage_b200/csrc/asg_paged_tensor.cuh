@@ -251,8 +251,8 @@ struct Tensor {
         }
       top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
       top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-      int power = (__float_as_int(top) >> 23) - 127;  // top in [2^power, 2^(power + 1)); 0 and infinity: as they are
-      power = power < -126 || power > 126 ? 0 : power;
+      // top in [2^power, 2^(power + 1)), cut to powers whose inverse is a normal number: 2^127 becomes 2, an infinity stays one
+      const int power = min(max((__float_as_int(top) >> 23) - 127, -126), 126);
       const float down = __int_as_float((127 - power) << 23), up = __int_as_float((127 + power) << 23);
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
@@ -577,7 +577,10 @@ struct Tensor {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) x[t][h] = (dots[0][2 * t + h] + (WIDE ? dots[1][2 * t + h] * 0x1p-12f : dots[1][2 * t + h])) * (kCoded ? key_scale[t] * unit[h] : a.scale_log2);
+      for (int h = 0; h < 2; ++h) {
+        x[t][h] = dots[0][2 * t + h] + (WIDE ? dots[1][2 * t + h] * 0x1p-12f : dots[1][2 * t + h]);
+        x[t][h] = kCoded ? x[t][h] * key_scale[t] * unit[h] : x[t][h] * a.scale_log2;  // (a key of zeros scores 0 whatever its scale)
+      }
     if (seen != 0xffffu) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)

@@ -113,3 +113,34 @@ def test_large_values_whose_scores_rise(shape, kinds):
     expected = case.expected()
     assert bool((expected[0].abs().amax(-1) < 2.0 ** 127).all()) and expected[0].abs().max() > 2.0 ** 122
     case.check(case.run(), expected)
+
+
+@pytest.mark.parametrize("kinds", [k for k in TYPES if k[1] in (E4M3, INT8)], ids=str)
+@pytest.mark.parametrize("power, key_power, rest", [(127, -110, 17), (126, -110, 16), (-126, 110, -16), (-14, 12, 0), (60, -61, 0)], ids=str)
+def test_queries_at_the_ends_of_their_range(kinds, power, key_power, rest):
+    """Query features of 2^power or more beside key scales that bring the scores back to where they always are."""
+    if kinds[0] == F16 and abs(power) > 15:
+        power, key_power, rest = (15, -16, 0) if power > 0 else (-14, 12, 0)
+    case = Case((8, 2, 64, 16), kinds, [200, 33, 700], seed=64)
+    size = case.query.double().abs().amax(-1, keepdim=True)
+    unit = torch.full_like(size, 1.9 * 2.0 ** power)
+    case.query = (case.query.double() / size * unit).to(kinds[0])
+    assert bool(torch.isfinite(case.query).all())
+    case.scales[0] = case.scales[0] * 2.0 ** key_power
+    case.exact[0] = case.exact[0] * 2.0 ** key_power
+    case.scale = 2.0 ** -rest
+    case.check(case.run(), case.expected())
+
+
+@pytest.mark.parametrize("kinds", [k for k in TYPES if k[1] in (E4M3, INT8)], ids=str)
+def test_a_key_of_zeros_scores_0_whatever_its_scale(kinds):
+    case = Case((8, 2, 64, 16), kinds, [40], seed=65)
+    page, at = place(case, 0, 17)
+    if kinds[0] != F16:
+        case.query = case.query * 2.0 ** 70
+        case.scales[0] = case.scales[0] * 2.0 ** -70
+        case.exact[0] = case.exact[0] * 2.0 ** -70
+    case.pages[0].view(torch.uint8)[page, at] = 0
+    case.exact[0][page, at] = 0
+    case.scales[0][page, :, at] = 2.0 ** 100
+    case.check(case.run(), case.expected())
