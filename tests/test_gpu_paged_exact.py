@@ -163,3 +163,20 @@ def test_a_million_equal_tokens(kinds):
     else:
         assert error < HALF_STEP[kinds[0]] / 2 and bool((out == value).all())    # nothing else lies as near
     assert bool(((lse - torch.log(torch.tensor(2.0 ** 20).double())).abs() <= 2.0 ** -22 * 14).all())
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16), (F16, INT8)], ids=str)
+def test_a_workspace_that_is_too_small_is_refused(kinds, monkeypatch):
+    """By the library, before anything is launched; the next call is right."""
+    from autosage_b200 import _native
+
+    case = counted((4, 2, 64, 16), kinds, [3000, 5], seed=54)
+    check(case, case.run())
+    whole = _native._scratch_on
+    for cut, message in ((lambda w: w[:4096], "smaller than"), (lambda w: w[128:], "256-byte aligned"),
+                         (lambda w: w[:0], "null")):
+        monkeypatch.setattr(_native, "_scratch_on", lambda *of: cut(whole(*of)))
+        with pytest.raises(RuntimeError, match=message):
+            case.run()
+    monkeypatch.setattr(_native, "_scratch_on", whole)
+    check(case, case.run())
