@@ -15,8 +15,7 @@ go with float32 scales ``[n_pages, n_kv_heads, page_size]``, one for each row of
 code * scale.  A slot is ``page * page_size + place in the page``.
 
 These are operators of inference: they have no backward and no forward-mode derivative, and a call that would need one is
-refused.  The reference
-has no counterpart (its attention, ``autosage/_auto.py:762-780``, is the whole-pattern form).
+refused.  The reference has no counterpart (its attention, ``autosage/_auto.py:762-780``, is the whole-pattern form).
 """
 from __future__ import annotations
 
@@ -124,10 +123,11 @@ def _checking() -> bool:
     return os.environ.get("AUTOSAGE_CHECK_INDICES") == "1"
 
 
-def _check_writable(**tensors: Optional[torch.Tensor]) -> None:
-    for name, tensor in tensors.items():
+def _check_writable(*tensors: Optional[torch.Tensor]) -> None:
+    for i, tensor in enumerate(tensors):
         if tensor is not None and 0 in tensor.stride() and any(
                 step == 0 and size > 1 for step, size in zip(tensor.stride(), tensor.shape)):
+            name = ("key_pages", "value_pages", "key_scales", "value_scales")[i]
             raise ValueError(f"{name} is written and must not repeat memory (it has a stride of 0)")
 
 
@@ -157,7 +157,7 @@ def paged_cache_write(slots: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     slots = _index("slots", slots, device)
     if slots.numel() != shape[0]:
         raise ValueError("slots must contain one slot per token")
-    _check_writable(key_pages=key_pages, value_pages=value_pages, key_scales=key_scales, value_scales=value_scales)
+    _check_writable(key_pages, value_pages, key_scales, value_scales)
     _require_native(device, key, value, key_pages, value_pages, key_scales, value_scales)
     if slots.numel() == 0 or n_pages == 0:
         return
@@ -225,7 +225,9 @@ def csr_paged_attention(crow: torch.Tensor, col: torch.Tensor, lengths: torch.Te
     Returns ``[B, n_heads, head_dim]`` in the type of the query and, with ``return_lse=True``, the natural
     logarithm of each softmax's denominator as float32 ``[B, n_heads]`` (parts computed over different pages can be
     joined with it).  A row that sees nothing gives 0 and ``-inf``.  A page id outside the pages is a hole whose
-    tokens are not seen; whatever lies behind a row's length in its last pages is not read."""
+    tokens are not seen (``AUTOSAGE_CHECK_INDICES=1`` takes only negative ids for one); whatever lies behind a row's length
+    in its last pages is not read.  An infinity among the values that are seen makes its feature infinite, unless its weight is
+    one that float32 calls 0: then NaN, as 0 times infinity."""
     n_pages, page_size, kv_heads, dim = _check_pages(key_pages, value_pages, key_scales, value_scales)
     device = key_pages.device
     shape = query.shape
