@@ -219,7 +219,8 @@ __device__ __forceinline__ void bulk_g2s(void* dst_smem, const void* src_gmem, u
 // still running (as soon as every CTA of that kernel has executed pdl_release_dependents() or has
 // exited).  It must call pdl_wait_for_primary() before it ends, so that whatever follows on the
 // stream still sees both kernels complete.  Used for the short-row kernels, which touch rows the main
-// kernel never touches: they fill the SMs the main kernel's last long rows leave idle.
+// kernel never touches (they fill the SMs the main kernel's last long rows leave idle), and for the
+// paged attention, whose kernels wait before they touch what a kernel before them may still write.
 __device__ __forceinline__ void pdl_release_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

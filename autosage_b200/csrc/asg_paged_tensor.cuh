@@ -665,9 +665,10 @@ struct Tensor {
   }
 };
 
-// Stages of a ring and CTAs per SM: one tile is being used with the next, the others are in flight.  16-bit pages want
-// few bytes in flight (64 x 8192 float16 of 8 x 128 take 174 us with one tile of each ring under way, 183 with two:
-// more requests from more rows spoil the order in which HBM serves them), 8-bit pages want the warps for their decoding.
+// Stages of a ring and CTAs per SM: one tile is being used with the next, the others are in flight.  As many CTAs as registers and
+// shared memory hold, each with as few stages as that leaves: warps hide more than tiles in flight do.  (64 rows of up to 8192
+// tokens, measured in turn: float16 8 x 128 178 us with 3 stages and 2 CTAs, 246 with 6 and 1; bfloat16 8 x 64 99 with 3 and 4, 103
+// with 4 and 3; int8 8 x 128 120 with 4 and 3, 144 with 6 and 2.)
 template <typename T, int SHARE, bool WIDE>
 inline Choice choose_padded(const AttentionArgs& a) {
   if constexpr (WIDE) {

@@ -379,7 +379,7 @@ typedef struct asg_paged_cache_args {
 
 /*
  * Writes tokens into their slots.  A slot outside the cache is skipped (a padded batch); the other slots of one call
- * must differ from one another.  cache_type is token_type, or one of the 8-bit types: then scale = max|x| / 448 or
+ * must differ from one another, and keys and values that differ go to different pages and scales.  cache_type is token_type, or one of the 8-bit types: then scale = max|x| / 448 or
  * / 127 over the features of the row, held in float32, and code = x / scale rounded to the nearest code (ties
  * to even; the quotient is not rounded first).  A row with an infinity or a NaN reads back as NaN.
  */
@@ -391,14 +391,15 @@ int asg_paged_cache_write(const asg_paged_cache_args* args);
  */
 int asg_paged_cache_read(const asg_paged_cache_args* args);
 
-/* Bytes of workspace of asg_paged_attention (the partial results of rows that several CTAs share). */
+/* Bytes of workspace of asg_paged_attention on the current device (the partial results of rows that several CTAs share). */
 size_t asg_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
 
 /*
  * out[r, h, :] = softmax_t(scale * <q[r, h, :], k_t>) v_t over the tokens t of row r, for one query
  * token a row; lse[r, h] = log sum_t exp(scale * <q, k_t>) when lse is not NULL (natural logarithm).
  * A page id outside [0, n_pages) is a hole: its tokens are not seen.  A row that sees nothing gets out = 0,
- * lse = -inf.  The tokens behind a row's length are never read.  Scores, softmax and sums are held in float32.
+ * lse = -inf.  The tokens behind a row's length are never read.  Scores, softmax and sums are held in float32; an
+ * infinity among the values seen makes its feature infinite, or NaN where float32 calls its weight 0.
  */
 typedef struct asg_paged_attention_args {
   const int64_t *crow, *col; /* [n_rows + 1], [n_cols]: row r owns the pages col[crow[r] ... crow[r + 1]) */

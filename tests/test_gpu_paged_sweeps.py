@@ -50,7 +50,7 @@ def test_the_codes_of_every_pair_of_16_bit_mantissas(kind, bits, cache):
     """Every largest value of a binade with every smaller one of 21 binades, whether the scale is exact, rounded up or rounded down."""
     count = 1 << bits
     mantissas = 1 + torch.arange(count, device="cuda").double() / count
-    values = torch.ldexp(mantissas.view(1, -1), 14 - torch.arange(21, device="cuda").view(-1, 1)).view(-1)
+    values = torch.ldexp(mantissas.repeat(21, 1), 14 - torch.arange(21, device="cuda").view(-1, 1)).view(-1)
     rows = -(-values.numel() // 255)
     others = torch.zeros(rows * 255, dtype=torch.float64, device="cuda")
     others[:values.numel()] = values
@@ -79,7 +79,7 @@ def test_float32_quotients_beside_the_borders(cache):
     values = torch.arange(127, dtype=torch.uint8).view(E4M3).double() if cache == E4M3 else torch.arange(128).double()
     middle = ((values[1:] + values[:-1]) / 2).cuda()
     tops = torch.cat((torch.exp2(torch.linspace(-70, 80, 4032)).float() * (1 + torch.rand(4032, generator=gen)),
-                      torch.ldexp(torch.tensor(LARGEST[cache]), torch.arange(-32, 32)))).cuda()
+                      torch.ldexp(torch.full((64,), LARGEST[cache]), torch.arange(-32, 32)))).cuda()
     scale = (tops.double() / LARGEST[cache]).float()
     border = middle.view(1, -1) * scale.double().view(-1, 1)
     near = border.float()
