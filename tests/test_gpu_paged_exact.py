@@ -180,3 +180,41 @@ def test_a_workspace_that_is_too_small_is_refused(kinds, monkeypatch):
             case.run()
     monkeypatch.setattr(_native, "_scratch_on", whole)
     check(case, case.run())
+
+
+@pytest.mark.parametrize("kinds", [(F32, F32), (BF16, BF16)], ids=str)
+def test_another_operator_of_another_thread_on_the_same_stream(kinds, monkeypatch):
+    """An SpMM that builds its plan in the stream's scratch at every call, between the launches of the attention's calls."""
+    import threading
+
+    import autosage_b200
+
+    monkeypatch.setenv("AUTOSAGE_PLAN_CACHE", "0")
+    case = counted((4, 1, 64, 16), kinds, [9000, 40, 7000], seed=55)
+    fixed = dict(crow=case.crow.cuda(), col=case.col.cuda(), lengths=case.lengths.cuda(), query=case.query.cuda())
+    gen = torch.Generator().manual_seed(56)
+    degrees = torch.randint(0, 40, (3000,), generator=gen)
+    crow = torch.cat((torch.zeros(1, dtype=torch.long), degrees.cumsum(0))).cuda()
+    col = torch.randint(0, 3000, (int(degrees.sum()),), generator=gen).cuda()
+    val, x = torch.ones(col.numel(), device="cuda"), torch.randn(3000, 64, generator=gen).cuda()
+    wanted, sums = case.run(**fixed), autosage_b200.spmm_csr(crow, col, val, x)
+    check(case, wanted)
+    answers, others = [], []
+
+    def attend():
+        with torch.no_grad():
+            answers.extend(case.run(**fixed) for _ in range(200))
+
+    def aggregate():
+        with torch.no_grad():
+            others.extend(autosage_b200.spmm_csr(crow, col, val, x) for _ in range(200))
+
+    threads = [threading.Thread(target=work) for work in (attend, aggregate)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert len(answers) == len(others) == 200
+    assert all(torch.equal(out, wanted[0]) and torch.equal(lse, wanted[1]) for out, lse in answers)
+    assert all(torch.equal(y, sums) for y in others)
